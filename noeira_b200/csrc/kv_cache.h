@@ -1,0 +1,48 @@
+// Parameter blocks of the paged 8-bit cache kernels (kv_cache.cu) and of the attention over it (kv_attention.cu).
+#pragma once
+#include <stdint.h>
+
+// status code: a row found no free block, no room in its table or none in the token buffers
+#define NB_ST_CACHE_FULL 5u
+
+struct KvPlan {
+  const int *lengths, *new_lens;
+  int* tables;
+  const int *free_ids, *free_count;
+  int *free_count_out, *starts, *ends, *row_of, *positions, *slots;
+  int rows, width, block, free_size, tokens;
+  unsigned int* status;
+};
+
+struct KvAppend {
+  const void *k, *v;
+  uint8_t* codes;
+  float* scale;
+  const int* slots;
+  int tokens, heads, dim, block, blocks, limit;
+  long long k_token, k_head, v_token, v_head;   // element strides of the inputs
+  long long kv_stride;                          // bytes from the keys' codes to the values'
+};
+
+struct KvReorder {
+  uint8_t* codes;
+  float* scale;
+  const int *tables, *lengths, *parents, *spare;
+  int *tables_out, *lengths_out, *spare_out;
+  int blocks, heads, block, dim, rows, beams, width;
+  long long plane;                              // bytes of one layer's keys or values
+  unsigned int* status;
+};
+
+struct KvAttn {
+  const void* q;                                // bf16 [T, Hq, D], element strides q_token, q_head
+  void* out;                                    // bf16 [T, Hq, D], element strides o_token, o_head
+  const uint8_t* codes;                         // [2, N, H, bs, D]
+  const float* scale;                           // [2, N, H]
+  const int *tables, *starts, *ends;
+  int rows, tokens, hq, hk, block, blocks, width;
+  long long q_token, q_head, o_token, o_head, kv_stride, s_stride;
+  float scale_log2;
+  float *part_o, *part_ml;
+  unsigned int* status;
+};

@@ -10,7 +10,7 @@ import torch
 
 _STATUS = {}
 _CODES = {1: "mbarrier wait timed out", 2: "peer flag wait timed out", 3: "bounds check failed",
-          4: "non-finite value"}
+          4: "non-finite value", 5: "key / value cache: a row found no room"}
 
 
 class DeviceStatusError(RuntimeError):
