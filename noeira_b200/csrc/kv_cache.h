@@ -40,8 +40,12 @@ struct KvAttn {
   const uint8_t* codes;                         // [2, N, H, bs, D]
   const float* scale;                           // [2, N, H]
   const int *tables, *starts, *ends;
-  int rows, tokens, hq, hk, block, blocks, width;
-  long long q_token, q_head, o_token, o_head, kv_stride, s_stride;
+  int rows, tokens, hq, hk, group, block_log, blocks, width;
+  int q_vec, o_vec;                             // 16-byte loads of q and 8-byte stores of out are aligned
+  int few;                                      // rows of the batch with at most this many query rows per head are done here
+  int pieces;
+  long long q_token, q_head, o_token, o_head;
+  long long kv_stride, s_stride;                // from the keys' codes / scales to the values'
   float scale_log2;
   float *part_o, *part_ml;
   unsigned int* status;

@@ -12,6 +12,7 @@ word (``ops.check_status``) and never touches memory outside the tensors.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import NamedTuple
 
@@ -235,11 +236,25 @@ def paged_attention(q, kv, scale, tables, starts, ends, max_new=None, softmax_sc
     if guard is not None:
         with guard:
             return paged_attention(q, kv, scale, tables, starts, ends, max_new, softmax_scale, out)
+    # partial results of this call alone: calls on two streams, or in two graphs, share nothing
+    work = torch.empty(_work_floats(dim), dtype=torch.float32, device=dev)
     check(cuda_lib().nb_kv_attention(
         q.data_ptr(), out.data_ptr(), kv.data_ptr(), scale.data_ptr(), tables.data_ptr(), starts.data_ptr(), ends.data_ptr(), rows, tokens, max_new, hq, hk, dim,
-        kv.shape[3], kv.shape[1], width, q.stride(0), q.stride(1), out.stride(0), out.stride(1), kv.stride(0), scale.stride(0), softmax_scale, None, 0,
+        kv.shape[3], kv.shape[1], width, q.stride(0), q.stride(1), out.stride(0), out.stride(1), kv.stride(0), scale.stride(0), softmax_scale, work.data_ptr(), work.numel(),
         status_ptr(kv.get_device()), raw_stream()), "kv_attention")
     return out
+
+
+_WORK = {}
+
+
+def _work_floats(dim):
+    n = _WORK.get(dim)
+    if n is None:
+        fn = cuda_lib().nb_kv_attention_work
+        fn.restype = ctypes.c_longlong
+        n = _WORK[dim] = int(fn(ctypes.c_int(dim)))
+    return n
 
 
 def _attention_cpu(q, kv, scale, tables, starts, ends, softmax_scale, out):
