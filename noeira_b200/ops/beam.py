@@ -25,35 +25,43 @@ def beam_select(logits, scores, finished=None, eos=None):
 
     Returns ``(scores fp32, parents int32, tokens int32, finished bool)``, each ``[requests, beams]``, best first.
     """
-    _need(logits.dim() == 3 and logits.numel() > 0, f"logits: [requests, beams, vocab], got {tuple(logits.shape)}")
-    requests, beams, vocab = logits.shape
-    dev = logits.device
-    _need(beams <= MAX_BEAMS and requests * beams < 1 << 31, f"beam_select: at most {MAX_BEAMS} beams, got {beams}")
-    _need(scores.dtype is torch.float32 and scores.shape == (requests, beams) and scores.is_contiguous() and scores.device == dev,
-          f"scores: contiguous float32 {(requests, beams)}, got {scores.dtype} {tuple(scores.shape)}")
-    _need(eos is None or 0 <= eos < vocab, f"eos: a token of {vocab}, got {eos}")
+    shape = logits.shape
+    if len(shape) != 3 or logits.numel() == 0:
+        raise ValueError(f"logits: [requests, beams, vocab], got {tuple(shape)}")
+    requests, beams, vocab = shape
+    dev = logits.get_device()
+    if beams > MAX_BEAMS or requests * beams >= 1 << 31 or vocab >= 1 << 31:
+        raise ValueError(f"beam_select: at most {MAX_BEAMS} beams, got {tuple(shape)}")
+    if scores.dtype is not torch.float32 or scores.shape != shape[:2] or not scores.is_contiguous() or scores.get_device() != dev:
+        raise ValueError(f"scores: contiguous float32 {(requests, beams)}, got {scores.dtype} {tuple(scores.shape)}")
+    if eos is not None and not 0 <= eos < vocab:
+        raise ValueError(f"eos: a token of {vocab}, got {eos}")
     if finished is not None:
-        _need(eos is not None, "finished: needs eos")
-        _need(finished.dtype is torch.bool and finished.shape == scores.shape and finished.is_contiguous() and finished.device == dev,
-              f"finished: contiguous bool {(requests, beams)}, got {finished.dtype} {tuple(finished.shape)}")
-    if not logits.is_cuda:
+        if eos is None:
+            raise ValueError("finished: needs eos")
+        if finished.dtype is not torch.bool or finished.shape != shape[:2] or not finished.is_contiguous() or finished.get_device() != dev:
+            raise ValueError(f"finished: contiguous bool {(requests, beams)}, got {finished.dtype} {tuple(finished.shape)}")
+    if dev < 0:
         return _select_cpu(logits, scores, finished, eos)
     fp32 = logits.dtype is torch.float32
-    _need(fp32 or logits.dtype is torch.bfloat16, f"logits: bf16 or fp32, got {logits.dtype}")
+    if not fp32 and logits.dtype is not torch.bfloat16:
+        raise ValueError(f"logits: bf16 or fp32, got {logits.dtype}")
     s0, pitch, s2 = logits.stride()
     if beams == 1:
         pitch = s0 if requests > 1 else vocab
-    _need((s2 == 1 or vocab == 1) and pitch >= vocab and (requests == 1 or s0 == beams * pitch), f"logits: rows of unit stride at one pitch, got strides {logits.stride()}")
+    if (s2 != 1 and vocab > 1) or pitch < vocab or (requests > 1 and s0 != beams * pitch):
+        raise ValueError(f"logits: rows of unit stride at one pitch, got strides {logits.stride()}")
     guard = _on(logits)
     if guard is not None:
         with guard:
             return beam_select(logits, scores, finished, eos)
-    out = torch.empty(3, requests, beams, dtype=torch.int32, device=dev)
-    done = torch.empty(requests, beams, dtype=torch.bool, device=dev)
-    new_scores, parents, tokens = out[0].view(torch.float32), out[1], out[2]
-    check(cuda_lib().nb_beam_select(logits.data_ptr(), scores.data_ptr(), None if finished is None else finished.data_ptr(), new_scores.data_ptr(), parents.data_ptr(),
-                                    tokens.data_ptr(), done.data_ptr(), requests, beams, vocab, -1 if eos is None else eos, int(fp32), pitch, raw_stream()), "beam_select")
-    return new_scores, parents, tokens, done
+    out = torch.empty((3, requests, beams), dtype=torch.int32, device=logits.device)
+    done = torch.empty((requests, beams), dtype=torch.bool, device=logits.device)
+    new_scores, parents, tokens = out.unbind(0)
+    at, step = out.data_ptr(), 4 * requests * beams
+    check(cuda_lib().nb_beam_select(logits.data_ptr(), scores.data_ptr(), None if finished is None else finished.data_ptr(), at, at + step, at + 2 * step, done.data_ptr(),
+                                    requests, beams, vocab, -1 if eos is None else eos, int(fp32), pitch, raw_stream()), "beam_select")
+    return new_scores.view(torch.float32), parents, tokens, done
 
 
 def _select_cpu(logits, scores, finished, eos):
@@ -88,12 +96,16 @@ def beam_reorder(kv, scale, tables, lengths, parents, spare, tables_out=None, le
     The spare blocks have to be distinct and named by no table.  Returns ``(tables, lengths, spare)`` of the next step, written to the ``_out`` tensors if given; these may not be the
     inputs.
     """
-    _need(kv.dtype is F8 and kv.dim() == 6 and kv.shape[1] == 2 and kv.is_contiguous(), f"kv: contiguous {F8} [layers, 2, blocks, heads, block, head_dim], got {kv.dtype} {tuple(kv.shape)}")
-    layers, _, blocks, heads, block, dim = kv.shape
-    dev = kv.device
-    _need(scale.dtype is torch.float32 and scale.shape == kv.shape[:4] and scale.is_contiguous() and scale.device == dev, f"scale: contiguous float32 {tuple(kv.shape[:4])}, got {scale.dtype} {tuple(scale.shape)}")
-    _need(dim % 16 == 0 and block > 0, f"head_dim {dim}: a multiple of 16")
-    _need(parents.dim() == 2 and tables.dim() == 2 and parents.numel() == tables.shape[0] and parents.numel() > 0, f"parents [requests, beams] over tables [requests * beams, width], got {tuple(parents.shape)} and {tuple(tables.shape)}")
+    shape, dev = kv.shape, kv.get_device()
+    if kv.dtype is not F8 or len(shape) != 6 or shape[1] != 2 or not kv.is_contiguous():
+        raise ValueError(f"kv: contiguous {F8} [layers, 2, blocks, heads, block, head_dim], got {kv.dtype} {tuple(shape)}")
+    layers, _, blocks, heads, block, dim = shape
+    if scale.dtype is not torch.float32 or scale.shape != shape[:4] or not scale.is_contiguous() or scale.get_device() != dev:
+        raise ValueError(f"scale: contiguous float32 {tuple(shape[:4])}, got {scale.dtype} {tuple(scale.shape)}")
+    if dim % 16 or block <= 0:
+        raise ValueError(f"head_dim {dim}: a multiple of 16")
+    if parents.dim() != 2 or tables.dim() != 2 or parents.shape[0] * parents.shape[1] != tables.shape[0] or tables.shape[0] == 0:
+        raise ValueError(f"parents [requests, beams] over tables [requests * beams, width], got {tuple(parents.shape)} and {tuple(tables.shape)}")
     rows, width = tables.shape
     _ints("tables", tables, dev)
     _ints("lengths", lengths, dev, rows)
@@ -105,16 +117,17 @@ def beam_reorder(kv, scale, tables, lengths, parents, spare, tables_out=None, le
     _ints("tables_out", tables_out, dev, rows * width)
     _ints("lengths_out", lengths_out, dev, rows)
     _ints("spare_out", spare_out, dev, rows)
-    _need(tables_out.data_ptr() != tables.data_ptr() and lengths_out.data_ptr() != lengths.data_ptr() and spare_out.data_ptr() != spare.data_ptr(), "beam_reorder: outputs may not be the inputs")
-    if not kv.is_cuda:
+    tp, lp, sp, tpo, lpo, spo = tables.data_ptr(), lengths.data_ptr(), spare.data_ptr(), tables_out.data_ptr(), lengths_out.data_ptr(), spare_out.data_ptr()
+    if tp == tpo or lp == lpo or sp == spo:
+        raise ValueError("beam_reorder: outputs may not be the inputs")
+    if dev < 0:
         return _reorder_cpu(kv, scale, tables, lengths, parents, spare, tables_out, lengths_out, spare_out)
     guard = _on(kv)
     if guard is not None:
         with guard:
             return beam_reorder(kv, scale, tables, lengths, parents, spare, tables_out, lengths_out, spare_out)
-    check(cuda_lib().nb_kv_reorder(
-        kv.data_ptr(), scale.data_ptr(), tables.data_ptr(), lengths.data_ptr(), parents.data_ptr(), spare.data_ptr(), tables_out.data_ptr(), lengths_out.data_ptr(),
-        spare_out.data_ptr(), 2 * layers, blocks, heads, block, dim, rows, parents.shape[1], width, status_ptr(kv.get_device()), raw_stream()), "kv_reorder")
+    check(cuda_lib().nb_kv_reorder(kv.data_ptr(), scale.data_ptr(), tp, lp, parents.data_ptr(), sp, tpo, lpo, spo, 2 * layers, blocks, heads, block, dim, rows,
+                                   parents.shape[1], width, status_ptr(dev), raw_stream()), "kv_reorder")
     return tables_out, lengths_out, spare_out
 
 

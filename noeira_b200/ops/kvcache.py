@@ -45,12 +45,13 @@ def _need(ok, what):
 
 def _on(t):
     """Guard for a launch on the tensor's own device (its current stream); None where that device is current already."""
-    return None if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return None if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def _ints(name, t, device, numel=None):
-    _need(t.dtype is torch.int32 and t.is_contiguous() and t.device == device and (numel is None or t.numel() == numel),
-          f"{name}: contiguous int32 on {device}" + (f" with {numel} elements" if numel is not None else "") + f", got {t.dtype} {tuple(t.shape)} on {t.device}")
+    """``device``: the index that ``get_device`` gives, -1 for the CPU."""
+    if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != device or (numel is not None and t.numel() != numel):
+        raise ValueError(f"{name}: contiguous int32 on device {device}" + (f" with {numel} elements" if numel is not None else "") + f", got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 # ------------------------------------------------------------------------------------------------ plan
@@ -64,9 +65,11 @@ def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free
     negative; behind a row that the stack could not serve, only rows that need no new block are served.  ``free_count`` is
     updated in place unless ``free_count_out`` is given.
     """
-    dev = tables.device
-    _need(tables.dim() == 2 and 0 < tables.shape[0] <= MAX_ROWS and tables.shape[1] > 0, f"tables: int32 [rows <= {MAX_ROWS}, width], got {tuple(tables.shape)}")
-    rows, width = tables.shape
+    dev = tables.get_device()
+    shape = tables.shape
+    if len(shape) != 2 or not 0 < shape[0] <= MAX_ROWS or shape[1] == 0:
+        raise ValueError(f"tables: int32 [rows <= {MAX_ROWS}, width], got {tuple(shape)}")
+    rows, width = shape
     _ints("tables", tables, dev)
     _ints("lengths", lengths, dev, rows)
     _ints("new_lens", new_lens, dev, rows)
@@ -74,8 +77,9 @@ def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free
     _ints("free_count", free_count, dev, 1)
     if free_count_out is not None:
         _ints("free_count_out", free_count_out, dev, 1)
-    _need(block > 0 and tokens >= 0 and width * block < 1 << 31, f"block {block}, tokens {tokens}, width {width}: out of range")
-    if not tables.is_cuda:
+    if block <= 0 or tokens < 0 or width * block >= 1 << 31:
+        raise ValueError(f"block {block}, tokens {tokens}, width {width}: out of range")
+    if dev < 0:
         return _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out)
     guard = _on(tables)
     if guard is not None:
@@ -84,7 +88,7 @@ def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free
     in_place = free_count_out is None or free_count_out.data_ptr() == free_count.data_ptr()
     # one allocation: starts | ends | left | rows | positions | slots, each on a 16-byte boundary
     pr, pt = (rows + 4) & ~3, (tokens + 3) & ~3
-    buf = torch.empty(2 * pr + 4 + 3 * pt, dtype=torch.int32, device=dev)
+    buf = torch.empty(2 * pr + 4 + 3 * pt, dtype=torch.int32, device=tables.device)
     starts, ends, left = buf[: rows + 1], buf[pr: pr + rows], buf[2 * pr: 2 * pr + 1]
     at = 2 * pr + 4
     row_of, positions, slots = buf[at: at + tokens], buf[at + pt: at + pt + tokens], buf[at + 2 * pt: at + 2 * pt + tokens]
@@ -92,7 +96,7 @@ def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free
     base = buf.data_ptr()
     check(cuda_lib().nb_kv_plan(
         lengths.data_ptr(), new_lens.data_ptr(), tables.data_ptr(), free.data_ptr(), free_count.data_ptr(), out.data_ptr(), base, base + 4 * pr,
-        base + 4 * at, base + 4 * (at + pt), base + 4 * (at + 2 * pt), rows, width, block, free.numel(), tokens, status_ptr(tables.get_device()), raw_stream()), "kv_plan")
+        base + 4 * at, base + 4 * (at + pt), base + 4 * (at + 2 * pt), rows, width, block, free.numel(), tokens, status_ptr(dev), raw_stream()), "kv_plan")
     if in_place:
         free_count.copy_(left)
         out = free_count
@@ -135,11 +139,18 @@ def _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_c
 
 # ------------------------------------------------------------------------------------------------ append
 def _check_layer(kv, scale):
-    _need(kv.dtype is F8 and kv.dim() == 5 and kv.shape[0] == 2 and kv.is_contiguous(), f"kv: contiguous {F8} [2, blocks, heads, block, head_dim], got {kv.dtype} {tuple(kv.shape)}")
-    _need(scale.dtype is torch.float32 and scale.shape == kv.shape[:3] and scale.is_contiguous() and scale.device == kv.device,
-          f"scale: contiguous float32 {tuple(kv.shape[:3])} beside kv, got {scale.dtype} {tuple(scale.shape)}")
-    _need(kv.shape[3] in BLOCKS and kv.shape[4] in HEAD_DIMS, f"block {kv.shape[3]} and head_dim {kv.shape[4]}: blocks of {BLOCKS} tokens, heads of {HEAD_DIMS}")
-    _need(kv.shape[1] * kv.shape[3] < 1 << 31, "kv: a cache layer has at most 2^31 - 1 slots")
+    """→ (device index, blocks, heads, block, head_dim)"""
+    shape, dev = kv.shape, kv.get_device()
+    if kv.dtype is not F8 or len(shape) != 5 or shape[0] != 2 or not kv.is_contiguous():
+        raise ValueError(f"kv: contiguous {F8} [2, blocks, heads, block, head_dim], got {kv.dtype} {tuple(shape)}")
+    if scale.dtype is not torch.float32 or scale.shape != shape[:3] or not scale.is_contiguous() or scale.get_device() != dev:
+        raise ValueError(f"scale: contiguous float32 {tuple(shape[:3])} beside kv, got {scale.dtype} {tuple(scale.shape)}")
+    _, blocks, heads, block, dim = shape
+    if block not in BLOCKS or dim not in HEAD_DIMS:
+        raise ValueError(f"block {block} and head_dim {dim}: blocks of {BLOCKS} tokens, heads of {HEAD_DIMS}")
+    if blocks * block >= 1 << 31:
+        raise ValueError("kv: a cache layer has at most 2^31 - 1 slots")
+    return dev, blocks, heads, block, dim
 
 
 def scale_for(amax: torch.Tensor) -> torch.Tensor:
@@ -159,20 +170,24 @@ def append(kv, scale, k, v, slots) -> None:
     call that writes a block's first token starts the block afresh, one that continues it may raise the scale and then moves
     the codes of the earlier tokens.  Non-finite inputs become NaN and do not count for the scale.
     """
-    _check_layer(kv, scale)
-    heads, dim = kv.shape[2], kv.shape[4]
-    _need(k.dim() == 3 and k.shape[1] == heads and k.shape[2] == dim and v.shape == k.shape, f"k, v: [tokens, {heads}, {dim}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    _need(k.device == kv.device and v.device == kv.device, "k, v: on the cache's device")
-    _ints("slots", slots, kv.device, k.shape[0])
-    if not kv.is_cuda:
+    dev, blocks, heads, block, dim = _check_layer(kv, scale)
+    shape = k.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or v.shape != shape:
+        raise ValueError(f"k, v: [tokens, {heads}, {dim}], got {tuple(shape)} and {tuple(v.shape)}")
+    if k.get_device() != dev or v.get_device() != dev:
+        raise ValueError("k, v: on the cache's device")
+    _ints("slots", slots, dev, shape[0])
+    if dev < 0:
         return _append_cpu(kv, scale, k, v, slots)
-    _need(k.dtype is torch.bfloat16 and v.dtype is torch.bfloat16 and k.stride(2) == 1 and v.stride(2) == 1, "k, v: bf16 with unit stride over head_dim")
+    ks, vs = k.stride(), v.stride()
+    if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or ks[2] != 1 or vs[2] != 1:
+        raise ValueError("k, v: bf16 with unit stride over head_dim")
     guard = _on(kv)
     if guard is not None:
         with guard:
             return append(kv, scale, k, v, slots)
-    check(cuda_lib().nb_kv_append(k.data_ptr(), v.data_ptr(), kv.data_ptr(), scale.data_ptr(), slots.data_ptr(), k.shape[0], heads, dim, kv.shape[3], kv.shape[1],
-                                  k.stride(0), k.stride(1), v.stride(0), v.stride(1), kv.stride(0), raw_stream()), "kv_append")
+    check(cuda_lib().nb_kv_append(k.data_ptr(), v.data_ptr(), kv.data_ptr(), scale.data_ptr(), slots.data_ptr(), shape[0], heads, dim, block, blocks,
+                                  ks[0], ks[1], vs[0], vs[1], kv.stride(0), raw_stream()), "kv_append")
     return None
 
 
@@ -213,35 +228,40 @@ def paged_attention(q, kv, scale, tables, starts, ends, max_new=None, softmax_sc
     (starts[i + 1] - t)`` of its row.  ``max_new``: an upper bound of the tokens of one row (default: all); 1 in a decode step.
     Tokens behind ``starts[rows]`` are left as they are in ``out``; a token that sees nothing gets zeros.
     """
-    _check_layer(kv, scale)
-    tokens, hq, dim = q.shape
-    hk = kv.shape[2]
-    dev = kv.device
-    _need(dim == kv.shape[4] and hq % hk == 0 and hq > 0, f"q: [tokens, a multiple of {hk}, {kv.shape[4]}], got {tuple(q.shape)}")
-    _need(tables.dim() == 2 and q.device == dev, "tables: int32 [rows, width]; q on the cache's device")
+    dev, blocks, hk, block, dim = _check_layer(kv, scale)
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != dim or shape[1] == 0 or shape[1] % hk or q.get_device() != dev:
+        raise ValueError(f"q: [tokens, a multiple of {hk}, {dim}] on the cache's device, got {tuple(shape)} on {q.device}")
+    tokens, hq, _ = shape
+    if tables.dim() != 2 or not 0 < tables.shape[0] <= MAX_ROWS or tables.shape[1] == 0:
+        raise ValueError(f"tables: int32 [rows <= {MAX_ROWS}, width], got {tuple(tables.shape)}")
     rows, width = tables.shape
     _ints("tables", tables, dev)
     _ints("starts", starts, dev, rows + 1)
     _ints("ends", ends, dev, rows)
     softmax_scale = 1.0 / math.sqrt(dim) if softmax_scale is None else float(softmax_scale)
     max_new = tokens if max_new is None else min(int(max_new), tokens)
-    _need(max_new > 0 or tokens == 0, f"max_new: at least 1, got {max_new}")
-    if not kv.is_cuda:
+    if max_new <= 0 < tokens:
+        raise ValueError(f"max_new: at least 1, got {max_new}")
+    if dev < 0:
         return _attention_cpu(q, kv, scale, tables, starts, ends, softmax_scale, out)
-    _need(q.dtype is torch.bfloat16 and q.stride(2) == 1, "q: bf16 with unit stride over head_dim")
     if out is None:
-        out = torch.empty(tokens, hq, dim, dtype=torch.bfloat16, device=dev)
-    _need(out.dtype is torch.bfloat16 and out.shape == q.shape and out.stride(2) == 1 and out.device == dev, "out: bf16 like q with unit stride over head_dim")
+        out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
+    qs, os_ = q.stride(), out.stride()
+    if q.dtype is not torch.bfloat16 or qs[2] != 1:
+        raise ValueError("q: bf16 with unit stride over head_dim")
+    if out.dtype is not torch.bfloat16 or out.shape != shape or os_[2] != 1 or out.get_device() != dev:
+        raise ValueError("out: bf16 like q with unit stride over head_dim")
     guard = _on(kv)
     if guard is not None:
         with guard:
             return paged_attention(q, kv, scale, tables, starts, ends, max_new, softmax_scale, out)
     # partial results of this call alone: calls on two streams, or in two graphs, share nothing
-    work = torch.empty(_work_floats(dim), dtype=torch.float32, device=dev)
+    floats = _work_floats(dim)
+    work = torch.empty(floats, dtype=torch.float32, device=q.device)
     check(cuda_lib().nb_kv_attention(
         q.data_ptr(), out.data_ptr(), kv.data_ptr(), scale.data_ptr(), tables.data_ptr(), starts.data_ptr(), ends.data_ptr(), rows, tokens, max_new, hq, hk, dim,
-        kv.shape[3], kv.shape[1], width, q.stride(0), q.stride(1), out.stride(0), out.stride(1), kv.stride(0), scale.stride(0), softmax_scale, work.data_ptr(), work.numel(),
-        status_ptr(kv.get_device()), raw_stream()), "kv_attention")
+        block, blocks, width, qs[0], qs[1], os_[0], os_[1], kv.stride(0), scale.stride(0), softmax_scale, work.data_ptr(), floats, status_ptr(dev), raw_stream()), "kv_attention")
     return out
 
 
