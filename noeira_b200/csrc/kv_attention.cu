@@ -6,12 +6,13 @@
 //   * A tile has 16 query rows: all query heads of one cache head, of as many tokens as fit.  S = Q K^T and O += P V are
 //     m16n8k16 products in f16 with fp32 sums.  e4m3 codes are exact in f16; q (bf16) is exact in f16 down to 2^-38 of the row's
 //     largest element after a power-of-two scaling of the row; P keeps 11 bits.
-//   * A lane's fragment of K is 16 consecutive bytes of a key (the order of the contraction is free as long as q has the same),
-//     its fragment of V is D / 8 consecutive bytes of four keys (the order of the output columns is free).  No shared memory, no
-//     transposition; every sector that is fetched is used.
-//   * The key range of the whole batch is cut into equal pieces, one for each resident block (rows differ in length, so pieces
-//     run over the ends of rows), and a second, small kernel joins rows that lie in several pieces.  The four warps of a block
-//     take turns at steps of 4 KB and join in shared memory.
+//   * A warp works by itself: codes come by cp.async into its own ring in shared memory, 4 KB a step, and from there as they
+//     are into the fragments.  The order of the contraction is free as long as q has the same, so a lane's fragment of K is 16
+//     consecutive bytes of a key; the orders of keys and of output columns are free, so its fragment of V is D / 8 consecutive
+//     bytes of four keys.  The 16-byte chunks are swizzled so that both reads are free of bank conflicts.
+//   * The steps of the whole batch are cut into equal pieces, one for each resident warp (rows differ in length, so pieces run
+//     over the ends of rows, and the ring runs ahead into the next row); a second, small kernel joins rows that lie in several
+//     pieces.
 #include "common.cuh"
 #include "kv_cache.h"
 
@@ -19,7 +20,10 @@ namespace {
 using namespace nb;
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
-constexpr int CHUNK = 32;              // steps of a piece when the batch does not fill the GPU: at most eight per warp, no joining up to 1024 (512) keys
+constexpr int STAGES = 4;              // steps in flight: three ahead of the one in work
+constexpr int LEAD = 2;                // steps that starting a tile costs, in the measure by which the batch is cut
+constexpr int LEAST = 2;               // a piece has at least so many steps
+constexpr int SOLO = 8;                // tables of at most so many steps: a tile to a warp, nothing to join
 constexpr float RAISE = 8.f;           // the running maximum is raised when it falls behind by more than 2^8 ...
 constexpr float LIFT = 7.f;            // ... and weights are at most 2^(8 + 7), below f16's largest, so that small ones stay normal
 
@@ -58,70 +62,59 @@ __device__ __forceinline__ uint32_t nan_code(uint32_t w) {         // nonzero wh
 }
 
 // ---------------------------------------------------------------- how the batch is cut
-// Row i costs q-tiles x heads x steps; `upto` (shared memory, rows + 1) are the exclusive sums.  `piece` is what a block takes.
+// A job is a tile of 16 query rows and a cache head.  It costs LEAD + steps (one, where every job is one warp's).  `upto`
+// (shared memory, rows + 1): exclusive sums over the rows; `piece`: what a warp takes.
 struct Cut {
   long long total, piece;
-  int pad;                             // steps of a (q-tile, head) are rounded up to a multiple of this
 };
 struct Job {
-  int row, head, qt, steps;            // steps: rounded
-  long long begin;                     // its first step
+  int row, head, qt, cost;
+  long long begin;
 };
 
 template <int KEYS>
-__device__ __forceinline__ int row_steps(const KvAttn& p, int i) { return ceil_div(max(0, min(p.ends[i], p.width << p.block_log)), KEYS); }
+__device__ __forceinline__ int job_cost(const KvAttn& p, int i) {
+  return p.solo ? 1 : LEAD + ceil_div(max(1, min(p.ends[i], p.width << p.block_log)), KEYS);
+}
 __device__ __forceinline__ int row_tiles(const KvAttn& p, int i) {
   const int first = p.starts[i];
   const long long n = first < 0 ? 0 : (long long)min(p.starts[i + 1], p.tokens) - first;
   // rows with more query rows than `few` belong to the kernel of prompts
   return n <= 0 || n * p.group > p.few ? 0 : (int)((n * p.group + 15) / 16);
 }
-// A row without keys still gets its zeros written: one step.
 template <int KEYS>
 __device__ __forceinline__ Cut cut_batch(const KvAttn& p, long long* upto, long long* sh) {
   const int tid = threadIdx.x, per = ceil_div(p.rows, THREADS);
   const int lo = min(p.rows, tid * per), hi = min(p.rows, lo + per);
-  long long a = 0, b = 0;
-  for (int i = lo; i < hi; ++i) {
-    const long long jobs = (long long)row_tiles(p, i) * p.hk;
-    const int n = max(1, row_steps<KEYS>(p, i));
-    a += jobs * n;
-    b += jobs * ceil_div(n, CHUNK);
-  }
-  // sums over the block of both, and what lies before this thread
-  long long ia = a, ib = b;
+  long long sum = 0;
+  for (int i = lo; i < hi; ++i) sum += (long long)row_tiles(p, i) * p.hk * job_cost<KEYS>(p, i);
+  long long at = sum;
   const int lane = tid & 31, w = tid >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, ia, o), v = __shfl_up_sync(0xffffffffu, ib, o);
-    if (lane >= o) { ia += u; ib += v; }
+    const long long u = __shfl_up_sync(0xffffffffu, at, o);
+    if (lane >= o) at += u;
   }
+  if (lane == 31) sh[w] = at;
   __syncthreads();
-  if (lane == 31) { sh[w] = ia; sh[WARPS + w] = ib; }
-  __syncthreads();
-  long long ta = 0, tb = 0;
-  for (int i = 0; i < WARPS; ++i) {
-    if (i < w) { ia += sh[i]; ib += sh[WARPS + i]; }
-    ta += sh[i];
-    tb += sh[WARPS + i];
-  }
   Cut c;
-  const bool small = tb <= p.pieces;   // every (q-tile, head) in pieces of its own, none shared with the next
-  c.pad = small ? CHUNK : 1;
-  c.total = small ? tb * CHUNK : ta;
-  c.piece = small ? CHUNK : max(1LL, (ta + p.pieces - 1) / p.pieces);
-  long long at = small ? (ib - b) * CHUNK : ia - a;
+  c.total = 0;
+  for (int i = 0; i < WARPS; ++i) {
+    if (i < w) at += sh[i];
+    c.total += sh[i];
+  }
+  c.piece = p.solo ? 1 : max((long long)LEAST, (c.total + p.pieces - 1) / p.pieces);
+  at -= sum;
   for (int i = lo; i < hi; ++i) {
     upto[i] = at;
-    const int n = max(1, row_steps<KEYS>(p, i));
-    at += (long long)row_tiles(p, i) * p.hk * (small ? ceil_div(n, CHUNK) * CHUNK : n);
+    at += (long long)row_tiles(p, i) * p.hk * job_cost<KEYS>(p, i);
   }
   if (tid == 0) upto[p.rows] = c.total;
   __syncthreads();
   return c;
 }
 template <int KEYS>
-__device__ __forceinline__ Job job_at(const KvAttn& p, const Cut& c, const long long* upto, long long x) {
+__device__ __forceinline__ Job job_at(const KvAttn& p, const long long* upto, long long x) {
   int a = 0, b = p.rows;               // last row that begins at or before x (rows without work share their begin with the next)
   while (b - a > 1) {
     const int m = (a + b) >> 1;
@@ -129,80 +122,127 @@ __device__ __forceinline__ Job job_at(const KvAttn& p, const Cut& c, const long 
   }
   Job j;
   j.row = a;
-  j.steps = ceil_div(max(1, row_steps<KEYS>(p, a)), c.pad) * c.pad;
-  const long long n = (x - upto[a]) / j.steps;
+  j.cost = job_cost<KEYS>(p, a);
+  const long long n = (x - upto[a]) / j.cost;
   j.head = (int)(n % p.hk);
   j.qt = (int)(n / p.hk);
-  j.begin = upto[a] + n * j.steps;
+  j.begin = upto[a] + n * j.cost;
   return j;
 }
 
-// ---------------------------------------------------------------- the step
-template <int D>
-struct Raw {                           // one step of a warp: 4 KB of codes
-  static constexpr int SUB = 128 / D;  // sub-tiles of 16 keys
-  static constexpr int KEYS = 16 * SUB;
-  uint4 k[SUB][2][D / 64];             // [sub][n-block of 8 keys][64 dimensions]
-  uint32_t v[SUB][4][D / 32];          // [sub][key 2c, 2c+1, 2c+8, 2c+9][bytes of dimensions (lane / 4) D / 8 ...]
-  float ks[SUB], vs[SUB];
-  bool has[SUB];                       // false: no keys there (past the end, or a bad block)
+// The part of a job that lies in a piece: steps [from, last), none of them behind the last key that a row of the tile sees.
+template <int KEYS>
+struct Part {
+  Job j;
+  long long stop;                      // where it ends, in the measure of the cut
+  int first, count, rows16, end, new_tokens, sure, seen, from, last;
+  __device__ __forceinline__ void set(const KvAttn& p, const long long* upto, long long x, long long x1) {
+    j = job_at<KEYS>(p, upto, x);
+    stop = min(x1, j.begin + j.cost);
+    first = p.starts[j.row];
+    const int next = p.starts[j.row + 1];
+    new_tokens = next - first;
+    count = min(next, p.tokens) - first;
+    end = max(0, min(p.ends[j.row], p.width << p.block_log));
+    rows16 = min(16, count * p.group - j.qt * 16);                // real rows of the tile
+    const int tok0 = j.qt * 16 / p.group, tok1 = (j.qt * 16 + rows16 - 1) / p.group;
+    sure = max(0, min(end, end - new_tokens + tok0 + 1));         // the fewest keys that a real row sees
+    seen = max(0, min(end, end - new_tokens + tok1 + 1));         // the most
+    const int all = ceil_div(seen, KEYS);
+    from = p.solo ? 0 : max(0, (int)(x - j.begin) - LEAD);
+    last = p.solo ? all : min(all, max(0, (int)(stop - j.begin) - LEAD));
+  }
 };
 
+// ---------------------------------------------------------------- the ring
 template <int D>
-__device__ __forceinline__ void load_ids(const KvAttn& p, const int* table, int step, int limit, int (&id)[Raw<D>::SUB]) {
-#pragma unroll
-  for (int s = 0; s < Raw<D>::SUB; ++s) {
-    const int k0 = step * Raw<D>::KEYS + s * 16;
-    id[s] = k0 < limit ? table[k0 >> p.block_log] : -2;
-  }
+struct Shape {
+  static constexpr int SUB = 128 / D;  // sub-tiles of 16 keys in a step
+  static constexpr int KEYS = 16 * SUB;
+};
+struct __align__(16) Stage {
+  uint8_t k[2048], v[2048];
+  float ks[2], vs[2];                  // scales of the sub-tiles
+  int has[2];                          // 0: no keys there (past the end, or a bad block)
+  int pad[2];
+};
+
+// Byte of 16-byte chunk `ch` of key row `r` (0..15) in a sub-tile.
+template <int D>
+__device__ __forceinline__ int chunk_at(int r, int ch) {
+  if (D == 64) return (r >> 1) * 128 + ((((r & 1) * 4 + ch) ^ (((r >> 1) & 1) * 2 | ((r >> 2) & 1) * 4)) << 4);
+  return r * 128 + ((ch ^ ((r & 3) * 2) ^ (((r >> 2) & 1) * 4)) << 4);
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
 template <int D>
-__device__ __forceinline__ void load_raw(const KvAttn& p, int row, int head, int step, const int (&id)[Raw<D>::SUB], Raw<D>& r) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-#pragma unroll
-  for (int s = 0; s < Raw<D>::SUB; ++s) {
-    r.ks[s] = 0.f;
-    r.vs[s] = 0.f;
-    r.has[s] = (unsigned)id[s] < (unsigned)p.blocks;
-    if (!r.has[s]) {
-      if (id[s] != -2 && lane == 0) report(p.status, NB_ST_BOUNDS, 10, row);
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int u = 0; u < D / 64; ++u) r.k[s][n][u] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int u = 0; u < D / 32; ++u) r.v[s][k][u] = 0;
-      continue;
+struct Feed {                          // runs over the steps of a warp's piece, ahead of the work
+  Part<Shape<D>::KEYS> part;
+  long long x, x1, stride;
+  int step, page0, id;                 // lane l holds the block id of page page0 + l
+  bool more;
+  __device__ __forceinline__ void begin(const KvAttn& p, const long long* upto, long long at, long long end, long long by) {
+    x = at;
+    x1 = end;
+    stride = by;
+    more = true;
+    open(p, upto);
+  }
+  __device__ __forceinline__ void open(const KvAttn& p, const long long* upto) {     // the next part that has steps
+    for (;;) {
+      if (x >= x1) { more = false; return; }
+      part.set(p, upto, x, x1);
+      x = stride ? x + stride : part.stop;
+      if (part.from < part.last) break;
     }
-    const long long page = (long long)id[s] * p.hk + head;
-    const int in = (step * Raw<D>::KEYS + s * 16) & ((1 << p.block_log) - 1);
-    const uint8_t* base = p.codes + ((page << p.block_log) + in) * D;
+    step = part.from;
+    page0 = -64;
+  }
+  __device__ __forceinline__ void next(const KvAttn& p, const long long* upto, Stage* st) {
+    constexpr int SUB = Shape<D>::SUB, KEYS = Shape<D>::KEYS;
+    const int lane = threadIdx.x & 31;
+    if (more) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+      for (int s = 0; s < SUB; ++s) {
+        const int k0 = step * KEYS + s * 16, pg = k0 >> p.block_log;
+        int b = -2;
+        if (k0 < part.seen) {
+          if (pg - page0 >= 32) {
+            page0 = pg;
+            id = pg + lane < p.width ? __ldg(p.tables + (long long)part.j.row * p.width + pg + lane) : -2;
+          }
+          b = __shfl_sync(0xffffffffu, id, pg - page0);
+        }
+        const bool real = (unsigned)b < (unsigned)p.blocks;
+        if (!real && k0 < part.seen && lane == 0) report(p.status, NB_ST_BOUNDS, 10, part.j.row);
+        const long long page = real ? (long long)b * p.hk + part.j.head : 0;
+        const int in = k0 & ((1 << p.block_log) - 1);
+        const uint8_t* src = p.codes + (real ? ((page << p.block_log) + in) * D : 0) + lane * 16;
+        const uint32_t kd = smem_u32(st->k) + s * 1024, vd = smem_u32(st->v) + s * 1024;
 #pragma unroll
-      for (int u = 0; u < D / 64; ++u) r.k[s][n][u] = __ldg(reinterpret_cast<const uint4*>(base + (n * 8 + g) * D + u * 64 + c * 16));
-    const uint8_t* vb = base + p.kv_stride;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint8_t* a = vb + (2 * c + (k & 1) + (k >> 1) * 8) * D + g * (D / 8);
-      if (D == 64) {
-        const uint2 w = __ldg(reinterpret_cast<const uint2*>(a));
-        r.v[s][k][0] = w.x;
-        r.v[s][k][1] = w.y;
-      } else {
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(a));
-        r.v[s][k][0] = w.x;
-        r.v[s][k][1] = w.y;
-        r.v[s][k][D / 32 - 2] = w.z;
-        r.v[s][k][D / 32 - 1] = w.w;
+        for (int i = 0; i < D / 32; ++i) {                        // 16 keys: D chunks
+          const int n = i * 32 + lane, at = chunk_at<D>(n / (D / 16), n % (D / 16));
+          copy16(kd + at, src + i * 512, real);
+          copy16(vd + at, src + p.kv_stride + i * 512, real);
+        }
+        if (lane == 0) {
+          if (real) {
+            copy4(smem_u32(&st->ks[s]), p.scale + page);
+            copy4(smem_u32(&st->vs[s]), p.scale + p.s_stride + page);
+          }
+          st->has[s] = real;
+        }
       }
+      if (++step >= part.last) open(p, upto);
     }
-    r.ks[s] = __ldg(p.scale + page);
-    r.vs[s] = __ldg(p.scale + p.s_stride + page);
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
-}
+};
 
 template <int D>
 struct Tile {                          // what a warp keeps of a tile of 16 query rows
@@ -274,7 +314,7 @@ template <int D>
 __device__ __forceinline__ void times_v(float (&acc)[D / 8][4], const uint32_t (&pa)[4], const uint32_t (&v)[4][D / 32]) {
 #pragma unroll
   for (int w = 0; w < D / 32; ++w) {
-    // bytes of keys (2c, 2c + 1) and (2c + 8, 2c + 9) side by side: two dimensions per word
+    // bytes of two keys side by side: two dimensions per word
     const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
     const uint32_t b0 = __byte_perm(v[2][w], v[3][w], 0x5140), b1 = __byte_perm(v[2][w], v[3][w], 0x7362);
     mma(acc[w * 4 + 0], pa, f16_of_codes(a0), f16_of_codes(b0));
@@ -284,36 +324,57 @@ __device__ __forceinline__ void times_v(float (&acc)[D / 8][4], const uint32_t (
   }
 }
 
-// `seen`: the most keys that a row of the tile sees, `sure`: the fewest that a real row sees.
+// One step of a tile.  Column 2c + e of n-block n of the scores is key (2n + e) 4 + c of its sub-tile.
 template <int D>
-__device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D>& t, Raw<D>& r, int step, int seen, int sure) {
-  constexpr int SUB = Raw<D>::SUB;
-  const int lane = threadIdx.x & 31, c = lane & 3;
-  float s[SUB][2][4];
+__device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D>& t, const Stage* st, int step, int seen, int sure) {
+  constexpr int SUB = Shape<D>::SUB, KEYS = Shape<D>::KEYS;
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  float s[SUB][2][4], ks[SUB], vs[SUB];
+  bool has[SUB];
+  uint32_t v[SUB][4][D / 32];          // [key 4 r + c][bytes of dimensions g D / 8 ...]
 #pragma unroll
-  for (int u = 0; u < SUB; ++u)
+  for (int u = 0; u < SUB; ++u) {
+    ks[u] = st->ks[u];
+    vs[u] = st->vs[u];
+    has[u] = st->has[u] != 0;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[u][n][i] = 0.f;
 #pragma unroll
       for (int d = 0; d < D / 64; ++d) {
-        const uint32_t w[4] = {r.k[u][n][d].x, r.k[u][n][d].y, r.k[u][n][d].z, r.k[u][n][d].w};
+        const uint4 x = *reinterpret_cast<const uint4*>(st->k + u * 1024 + chunk_at<D>((n * 2 + (g & 1)) * 4 + (g >> 1), d * 4 + c));
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) mma(s[u][n], t.q[d * 4 + k], f16_of_codes(w[k]), f16_of_codes(w[k] >> 16));
       }
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (D == 64) {
+        const uint2 x = *reinterpret_cast<const uint2*>(st->v + u * 1024 + chunk_at<D>(k * 4 + c, g >> 1) + (g & 1) * 8);
+        v[u][k][0] = x.x;
+        v[u][k][1] = x.y;
+      } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(st->v + chunk_at<D>(k * 4 + c, g));
+        v[u][k][0] = x.x;
+        v[u][k][1] = x.y;
+        v[u][k][D / 32 - 2] = x.z;
+        v[u][k][D / 32 - 1] = x.w;
+      }
+    }
+  }
   // scores in log2 units, masked; a NaN score stays NaN (the comparisons below let it through)
-  const int k0 = step * Raw<D>::KEYS;
-  const bool whole = k0 + Raw<D>::KEYS <= sure;
+  const int k0 = step * KEYS;
+  const bool whole = k0 + KEYS <= sure;
   float top[2] = {-INFINITY, -INFINITY}, vtop = t.vref;
   bool lacks = false;
 #pragma unroll
-  for (int u = 0; u < SUB; ++u) lacks |= !r.has[u];
+  for (int u = 0; u < SUB; ++u) lacks |= !has[u];
 #pragma unroll
   for (int u = 0; u < SUB; ++u) {
-    const float f0 = t.f[0] * r.ks[u], f1 = t.f[1] * r.ks[u];
-    vtop = fmaxf(vtop, r.vs[u]);
+    const float f0 = t.f[0] * ks[u], f1 = t.f[1] * ks[u];
+    vtop = has[u] ? fmaxf(vtop, vs[u]) : vtop;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -326,15 +387,15 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D>& t, Raw<D>& r
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (k0 + u * 16 + n * 8 + 2 * c + (i & 1) >= t.lim[i >> 1] || !r.has[u]) s[u][n][i] = -INFINITY;
+          if (k0 + u * 16 + (n * 2 + (i & 1)) * 4 + c >= t.lim[i >> 1] || !has[u]) s[u][n][i] = -INFINITY;
     // values behind the last key that any row sees are not numbers to be multiplied by zero
 #pragma unroll
     for (int u = 0; u < SUB; ++u)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (k0 + u * 16 + 2 * c + (k & 1) + (k >> 1) * 8 >= seen) {
+        if (k0 + u * 16 + k * 4 + c >= seen) {
 #pragma unroll
-          for (int w = 0; w < D / 32; ++w) r.v[u][k][w] = 0;
+          for (int w = 0; w < D / 32; ++w) v[u][k][w] = 0;
         }
   }
 #pragma unroll
@@ -368,10 +429,10 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D>& t, Raw<D>& r
   const float b0 = (t.m[0] == -INFINITY ? 0.f : t.m[0]) - LIFT, b1 = (t.m[1] == -INFINITY ? 0.f : t.m[1]) - LIFT;
 #pragma unroll
   for (int u = 0; u < SUB; ++u) {
-    if (!r.has[u]) continue;
+    if (!has[u]) continue;
     // Weights relative to vref; a block whose values are less than 2^-24 of the largest block's would lose bits in f16, so
     // its product is taken by itself and added in fp32.
-    const float ratio = t.vref > 0.f ? r.vs[u] / t.vref : 0.f;
+    const float ratio = t.vref > 0.f ? vs[u] / t.vref : 0.f;
     const bool apart = ratio < 5.9604645e-8f;
     uint32_t pa[4];
     float sum0 = 0.f, sum1 = 0.f;
@@ -393,19 +454,19 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D>& t, Raw<D>& r
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x) any |= nan_code(r.v[u][k][x]);
+        for (int x = 0; x < D / 32; ++x) any |= nan_code(v[u][k][x]);
       if (__any_sync(0xffffffffu, any != 0)) {
         const int key = k0 + u * 16;
         for (int k = 0; k < 16 && key + k < seen; ++k)
           for (int x = 0; x < D / 32; ++x) {
-            // lane (g = column group, c = keys) that holds key k: its word x carries dimensions g D / 8 + 4 x ..
-            const int holder = (k & 7) >> 1, reg = (k & 1) + (k >> 3) * 2;
+            // key k lies with the lanes c = k & 3, in register k >> 2; word x carries dimensions g D / 8 + 4 x ..
+            const int holder = k & 3, reg = k >> 2;
             uint32_t word = 0;
 #pragma unroll
             for (int rr = 0; rr < 4; ++rr)
 #pragma unroll
               for (int xx = 0; xx < D / 32; ++xx)
-                if (rr == reg && xx == x) word = r.v[u][rr][xx];
+                if (rr == reg && xx == x) word = v[u][rr][xx];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               // this lane's output columns 2c + e of every n-block: dimensions (2c + e) D / 8 + j
@@ -422,20 +483,20 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D>& t, Raw<D>& r
         for (int k = 0; k < 4; ++k)
 #pragma unroll
           for (int x = 0; x < D / 32; ++x) {
-            const uint32_t hit = nan_code(r.v[u][k][x]) >> 7;     // 1 in the byte of a NaN
-            r.v[u][k][x] &= ~(hit * 0xffu);
+            const uint32_t hit = nan_code(v[u][k][x]) >> 7;     // 1 in the byte of a NaN
+            v[u][k][x] &= ~(hit * 0xffu);
           }
       }
     }
     if (!apart) {
-      times_v<D>(t.o, pa, r.v[u]);
+      times_v<D>(t.o, pa, v[u]);
     } else {
       float acc[D / 8][4];
 #pragma unroll
       for (int j = 0; j < D / 8; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
-      times_v<D>(acc, pa, r.v[u]);
+      times_v<D>(acc, pa, v[u]);
 #pragma unroll
       for (int j = 0; j < D / 8; ++j)
 #pragma unroll
@@ -459,174 +520,143 @@ __device__ __forceinline__ void store_out(const KvAttn& p, int first, int head, 
   }
 }
 
-// Partial results of a block: slot 1 for the job that begins in its piece and runs on, slot 0 for the one that came from before.
-template <int D>
+// Partial results of a warp: slot 1 for the job that begins in its piece and runs on, slot 0 for the one that came from before.
 __device__ __forceinline__ long long slot_at(long long piece, int slot) { return (piece * 2 + slot) * 16; }
 
 template <int D>
-__global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv_attn_kernel(KvAttn p) {
-  constexpr int KEYS = Raw<D>::KEYS;
+__global__ void __launch_bounds__(THREADS, 3) kv_attn_kernel(KvAttn p) {
+  constexpr int KEYS = Shape<D>::KEYS;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* s_o = reinterpret_cast<float*>(smem);                    // [WARPS][16][D]
-  float* s_m = s_o + WARPS * 16 * D;                              // [WARPS][16] maximum, then [WARPS][16] sum
-  long long* sh = reinterpret_cast<long long*>(s_m + 2 * WARPS * 16);
-  long long* upto = sh + 2 * WARPS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  Stage* ring = reinterpret_cast<Stage*>(smem) + warp * STAGES;
+  long long* sh = reinterpret_cast<long long*>(reinterpret_cast<Stage*>(smem) + WARPS * STAGES);
+  long long* upto = sh + WARPS;
   const Cut cut = cut_batch<KEYS>(p, upto, sh);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  long long x = (long long)blockIdx.x * cut.piece;
-  const long long x1 = min(cut.total, x + cut.piece);
-  while (x < x1) {
-    const Job j = job_at<KEYS>(p, cut, upto, x);
-    const long long stop = min(x1, j.begin + j.steps);
-    const int from = (int)(x - j.begin);
-    const bool alone = from == 0 && stop == j.begin + j.steps;
-    const int first = p.starts[j.row], new_tokens = p.starts[j.row + 1] - first, count = min(p.starts[j.row + 1], p.tokens) - first;
-    const int end = max(0, min(p.ends[j.row], p.width << p.block_log));
-    Tile<D> t;
-    load_q<D>(p, first, count, j.head, end, new_tokens, j.qt, t);
-    const int rows16 = min(16, count * p.group - j.qt * 16);       // real rows of the tile
-    const int tok0 = j.qt * 16 / p.group, tok1 = (j.qt * 16 + rows16 - 1) / p.group;
-    const int sure = max(0, min(end, end - new_tokens + tok0 + 1)), seen = max(0, min(end, end - new_tokens + tok1 + 1));
-    const int last = min(from + (int)(stop - x), ceil_div(seen, KEYS));
-    // three stages: block ids two steps ahead, codes one step ahead
-    const int* table = p.tables + (long long)j.row * p.width;
-    int id[Raw<D>::SUB];
-    Raw<D> r[2];
-    int st = from + warp;
-    if (st < last) {
-      load_ids<D>(p, table, st, seen, id);
-      load_raw<D>(p, j.row, j.head, st, id, r[0]);
-      if (st + WARPS < last) load_ids<D>(p, table, st + WARPS, seen, id);
-    }
-    while (st < last) {
+  const long long piece = (long long)blockIdx.x * WARPS + warp;
+  long long x = piece * cut.piece;
+  const long long x1 = p.solo ? cut.total : min(cut.total, x + cut.piece), stride = p.solo ? p.pieces : 0;
+  if (x >= x1) return;
+  Feed<D> feed;
+  feed.begin(p, upto, x, x1, stride);
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        if (st >= last) break;
-        if (st + WARPS < last) {
-          load_raw<D>(p, j.row, j.head, st + WARPS, id, r[b ^ 1]);
-          if (st + 2 * WARPS < last) load_ids<D>(p, table, st + 2 * WARPS, seen, id);
-        }
-        step_tile<D>(p, t, r[b], st, seen, sure);
-        st += WARPS;
-      }
+  for (int i = 0; i < STAGES - 1; ++i) feed.next(p, upto, ring + i);
+  int at = 0;                          // stage of the next step
+  while (x < x1) {
+    Part<KEYS> w;
+    w.set(p, upto, x, x1);
+    Tile<D> t;
+    load_q<D>(p, w.first, w.count, w.j.head, w.end, w.new_tokens, w.j.qt, t);
+    for (int st = w.from; st < w.last; ++st) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+      __syncwarp();                    // the step's codes are there for all lanes, and all are done with the step before
+      feed.next(p, upto, ring + (at + STAGES - 1) % STAGES);
+      step_tile<D>(p, t, ring + at, st, w.seen, w.sure);
+      at = (at + 1) % STAGES;
     }
-    // join the warps: sums relative to the largest maximum
-    t.l[0] = quad_sum(t.l[0]);
-    t.l[1] = quad_sum(t.l[1]);
-    __syncthreads();
-    if (c == 0) {
-      s_m[warp * 16 + g] = t.m[0];
-      s_m[warp * 16 + g + 8] = t.m[1];
-      s_m[(WARPS + warp) * 16 + g] = t.l[0];
-      s_m[(WARPS + warp) * 16 + g + 8] = t.l[1];
-    }
-    __syncthreads();
+    const bool alone = p.solo || (x == w.j.begin && w.stop == w.j.begin + w.j.cost);
+    const long long slot = slot_at(piece, x == w.j.begin);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int row = g + 8 * h;
-      if (row >= rows16) continue;
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_m[w * 16 + row]);
-      const float f = t.m[h] == -INFINITY ? (t.l[h] == 0.f ? 0.f : 1.f) * t.vref : ex2(t.m[h] - top) * t.vref;
-      float* o = s_o + (warp * 16 + row) * D;
+      const float l = quad_sum(t.l[h]);
+      if (row >= w.rows16) continue;
+      const float f = alone ? (l == 0.f ? 0.f : t.vref / l) : t.vref;
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int k = 0; k < D / 8; k += 4)
-          *reinterpret_cast<float4*>(o + (2 * c + e) * (D / 8) + k) =
-              make_float4(t.o[k][2 * h + e] * f, t.o[k + 1][2 * h + e] * f, t.o[k + 2][2 * h + e] * f, t.o[k + 3][2 * h + e] * f);
+        for (int k = 0; k < D / 8; k += 4) {
+          const int d = (2 * c + e) * (D / 8) + k;
+          const float4 o = make_float4(t.o[k][2 * h + e] * f, t.o[k + 1][2 * h + e] * f, t.o[k + 2][2 * h + e] * f, t.o[k + 3][2 * h + e] * f);
+          if (alone) store_out<D>(p, w.first, w.j.head, w.j.qt * 16 + row, d, o.x, o.y, o.z, o.w);
+          else *reinterpret_cast<float4*>(p.part_o + (slot + row) * D + d) = o;
+        }
+      if (!alone && c == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + row) * 2) = make_float2(t.m[h], l);
     }
-    __syncthreads();
-    const long long slot = slot_at<D>(blockIdx.x, from == 0 ? 1 : 0);
-    for (int i = threadIdx.x; i < rows16 * (D / 4); i += THREADS) {
-      const int row = i / (D / 4), d = i % (D / 4) * 4;
-      float top = -INFINITY, l = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_m[w * 16 + row]);
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float m = s_m[w * 16 + row], lw = s_m[(WARPS + w) * 16 + row];
-        l += m == -INFINITY ? lw : lw * ex2(m - top);              // without a maximum the sum is zero, or NaN
-        const float4 v = *reinterpret_cast<const float4*>(s_o + (w * 16 + row) * D + d);
-        o.x += v.x;
-        o.y += v.y;
-        o.z += v.z;
-        o.w += v.w;
-      }
-      if (alone) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        store_out<D>(p, first, j.head, j.qt * 16 + row, d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-      } else {
-        *reinterpret_cast<float4*>(p.part_o + (slot + row) * D + d) = o;
-        if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + row) * 2) = make_float2(top, l);
-      }
-    }
-    x = stop;
+    x = stride ? x + stride : w.stop;
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Joins the job that begins in piece blockIdx.x and runs past its end.
+// Joins the job that begins in piece blockIdx.x and runs past its end.  Threads: columns of four x a share of the pieces.
 template <int D>
 __global__ void __launch_bounds__(THREADS) kv_attn_join_kernel(KvAttn p) {
-  constexpr int KEYS = Raw<D>::KEYS;
+  constexpr int KEYS = Shape<D>::KEYS, COLS = D / 4, SHARES = THREADS / COLS;
   extern __shared__ __align__(16) uint8_t smem[];
-  long long* sh = reinterpret_cast<long long*>(smem);
-  long long* upto = sh + 2 * WARPS;
+  float4* s_o = reinterpret_cast<float4*>(smem);                  // [SHARES][COLS]
+  float* s_l = reinterpret_cast<float*>(s_o + THREADS);           // [SHARES], and [WARPS] maxima
+  long long* sh = reinterpret_cast<long long*>(s_l + SHARES + WARPS);
+  long long* upto = sh + WARPS;
   const Cut cut = cut_batch<KEYS>(p, upto, sh);
   const long long lo = (long long)blockIdx.x * cut.piece, hi = lo + cut.piece;
   // every block waits, also one with nothing to join: what follows in the stream may start when this kernel is done
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (hi >= cut.total) return;
-  const Job j = job_at<KEYS>(p, cut, upto, hi - 1);
-  if (j.begin < lo || j.begin + j.steps <= hi) return;
-  const long long last = (j.begin + j.steps - 1) / cut.piece;
+  const Job j = job_at<KEYS>(p, upto, hi - 1);
+  if (j.begin < lo || j.begin + j.cost <= hi) return;
+  const int n = (int)((j.begin + j.cost - 1) / cut.piece - blockIdx.x) + 1;
   const int first = p.starts[j.row], count = min(p.starts[j.row + 1], p.tokens) - first;
   const int rows16 = min(16, count * p.group - j.qt * 16);
-  for (int i = threadIdx.x; i < rows16 * (D / 4); i += THREADS) {
-    const int row = i / (D / 4), d = i % (D / 4) * 4;
+  const int tid = threadIdx.x, col = tid % COLS, share = tid / COLS;
+  for (int row = 0; row < rows16; ++row) {
     float top = -INFINITY;
-    for (long long w = blockIdx.x; w <= last; ++w) top = fmaxf(top, p.part_ml[(slot_at<D>(w, w == blockIdx.x) + row) * 2]);
+    for (int w = tid; w < n; w += THREADS) top = fmaxf(top, p.part_ml[(slot_at(blockIdx.x + w, w == 0) + row) * 2]);
+    top = block_max(top, s_l + SHARES);
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (long long w = blockIdx.x; w <= last; ++w) {
-      const long long s = slot_at<D>(w, w == blockIdx.x) + row;
+#pragma unroll 4
+    for (int w = share; w < n; w += SHARES) {
+      const long long s = slot_at(blockIdx.x + w, w == 0) + row;
       const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + s * 2);
-      const float f = ml.x == -INFINITY ? 1.f : ex2(ml.x - top);   // without a maximum all is zero, or NaN
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + s * D + d);
+      const float f = ml.x == -INFINITY ? 1.f : ex2(ml.x - top);  // without a maximum all is zero, or NaN
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + s * D + col * 4);
       l += ml.y * f;
       o.x += v.x * f;
       o.y += v.y * f;
       o.z += v.z * f;
       o.w += v.w * f;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    store_out<D>(p, first, j.head, j.qt * 16 + row, d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    s_o[tid] = o;
+    if (col == 0) s_l[share] = l;
+    __syncthreads();
+    if (share == 0) {
+#pragma unroll
+      for (int i = 1; i < SHARES; ++i) {
+        const float4 v = s_o[i * COLS + col];
+        o.x += v.x;
+        o.y += v.y;
+        o.z += v.z;
+        o.w += v.w;
+        l += s_l[i];
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      store_out<D>(p, first, j.head, j.qt * 16 + row, col * 4, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    }
+    __syncthreads();
   }
 }
 
 template <int D>
 int launch_few(KvAttn p, cudaStream_t stream) {
-  const int scan = (2 * WARPS + p.rows + 1) * 8, smem = (WARPS * 16 * D + 2 * WARPS * 16) * 4 + scan;
+  const int scan = (WARPS + p.rows + 1) * 8, smem = WARPS * STAGES * (int)sizeof(Stage) + scan;
+  const int join_smem = THREADS * 16 + (THREADS / (D / 4) + WARPS) * 4 + scan;
   static bool configured[64] = {};
   int dev = 0;
   NB_CUDA(cudaGetDevice(&dev));
   if (dev >= 64) return NB_ERR_BAD_ARG;
   if (!configured[dev]) {
-    NB_CUDA(cudaFuncSetAttribute(kv_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    NB_CUDA(cudaFuncSetAttribute(kv_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, WARPS * STAGES * (int)sizeof(Stage) + (WARPS + 8193) * 8));
     NB_CUDA(cudaFuncSetAttribute(kv_attn_join_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024));
     configured[dev] = true;
   }
-  kv_attn_kernel<D><<<p.pieces, THREADS, smem, stream>>>(p);
+  p.solo = ((long long)p.width << p.block_log) <= SOLO * Shape<D>::KEYS;
+  kv_attn_kernel<D><<<p.pieces / WARPS, THREADS, smem, stream>>>(p);
   NB_LAUNCH_CHECK();
-  if (((long long)p.width << p.block_log) <= (long long)CHUNK * Raw<D>::KEYS && (long long)p.rows * p.hk * ceil_div(min(p.few, p.tokens * p.group), 16) <= p.pieces)
-    return NB_OK;                      // no table is long enough for two pieces
+  if (p.solo) return NB_OK;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.pieces);
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = scan;
+  cfg.dynamicSmemBytes = join_smem;
   cfg.stream = stream;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its blocks start while the first kernel's last ones run
@@ -642,7 +672,7 @@ int launch_few(KvAttn p, cudaStream_t stream) {
 extern "C" {
 
 // Pieces that the batch is cut into, and floats of work space that nb_kv_attention needs.
-int nb_kv_attention_pieces(int dim) { return 148 * (dim == 64 ? 3 : 2); }
+int nb_kv_attention_pieces(int) { return 148 * WARPS * 3; }
 long long nb_kv_attention_work(int dim) { return (long long)nb_kv_attention_pieces(dim) * 2 * 16 * (dim + 2); }
 
 int nb_kv_attention(const void* q, void* out, const void* codes, const float* scale, const int* tables, const int* starts,
