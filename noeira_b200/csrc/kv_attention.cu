@@ -3,9 +3,11 @@
 // Few query rows per row of the batch (decode steps, short chunks).  The work is bound by the bytes of the cache: 2 D bytes per
 // key and head at the copy rate, against 2 D operations per byte and query row.  So the cache is read once, straight from global
 // memory into the registers of the matrix instructions, and nothing else is in the way:
-//   * A tile has 16 query rows: all query heads of one cache head, of as many tokens as fit.  S = Q K^T and O += P V are
-//     m16n8k16 products in f16 with fp32 sums.  e4m3 codes are exact in f16; q (bf16) is exact in f16 down to 2^-38 of the row's
-//     largest element after a power-of-two scaling of the row; P keeps 11 bits.
+//   * A tile has 8 or 16 query rows: all query heads of one cache head, of as many tokens as fit.  The products are transposed,
+//     S^T = K Q^T and O^T += V^T P^T, as m16n8k16 in f16 with fp32 sums: the 16 rows of an instruction are keys or dimensions,
+//     which there are enough of, and its 8 columns are query rows, which in a decode step there are not.  e4m3 codes are exact
+//     in f16; q (bf16) is exact in f16 down to 2^-38 of the row's largest element after a power-of-two scaling of the row; P
+//     keeps 11 bits.
 //   * A warp works by itself: codes come by cp.async into its own ring in shared memory, 4 KB a step, and from there as they
 //     are into the fragments.  The order of the contraction is free as long as q has the same, so a lane's fragment of K is 16
 //     consecutive bytes of a key; the orders of keys and of output columns are free, so its fragment of V is D / 8 consecutive
@@ -26,16 +28,16 @@ constexpr int LEAST = 2;               // a piece has at least so many steps
 constexpr int SOLO = 8;                // tables of at most so many steps: a tile to a warp, nothing to join
 constexpr float RAISE = 8.f;           // the running maximum is raised when it falls behind by more than 2^8 ...
 constexpr float LIFT = 7.f;            // ... and weights are at most 2^(8 + 7), below f16's largest, so that small ones stay normal
+constexpr float NONE = -3e38f;         // the running maximum of a row that has seen nothing
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t f16_of_codes(uint32_t two) {   // two e4m3 codes (bits 0..15) as f16 pair
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
-  return r;
+// four e4m3 codes as two f16 pairs
+__device__ __forceinline__ void f16_of_codes(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
 __device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
   uint32_t r;
@@ -47,14 +49,31 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// the largest of a row / the sum of a row over the four lanes that hold it
+// the largest of a row over the four lanes that hold it
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+// the same over the eight lanes that hold a column
+__device__ __forceinline__ float column_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+}
+__device__ __forceinline__ float column_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 4);
+  v += __shfl_xor_sync(0xffffffffu, v, 8);
+  return v + __shfl_xor_sync(0xffffffffu, v, 16);
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {       // 8 x 8 matrix of 16-bit elements
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) { // f16 pairs
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 __device__ __forceinline__ uint32_t nan_code(uint32_t w) {         // nonzero where one of four codes is NaN
   const uint32_t m = w & 0x7f7f7f7fu;
@@ -62,7 +81,7 @@ __device__ __forceinline__ uint32_t nan_code(uint32_t w) {         // nonzero wh
 }
 
 // ---------------------------------------------------------------- how the batch is cut
-// A job is a tile of 16 query rows and a cache head.  It costs LEAD + steps (one, where every job is one warp's).  `upto`
+// A job is a tile of query rows and a cache head.  It costs LEAD + steps (one, where every job is one warp's).  `upto`
 // (shared memory, rows + 1): exclusive sums over the rows; `piece`: what a warp takes.
 struct Cut {
   long long total, piece;
@@ -80,7 +99,7 @@ __device__ __forceinline__ int row_tiles(const KvAttn& p, int i) {
   const int first = p.starts[i];
   const long long n = first < 0 ? 0 : (long long)min(p.starts[i + 1], p.tokens) - first;
   // rows with more query rows than `few` belong to the kernel of prompts
-  return n <= 0 || n * p.group > p.few ? 0 : (int)((n * p.group + 15) / 16);
+  return n <= 0 || n * p.group > p.few ? 0 : (int)((n * p.group + p.tile - 1) / p.tile);
 }
 template <int KEYS>
 __device__ __forceinline__ Cut cut_batch(const KvAttn& p, long long* upto, long long* sh) {
@@ -135,7 +154,7 @@ template <int KEYS>
 struct Part {
   Job j;
   long long stop;                      // where it ends, in the measure of the cut
-  int first, count, rows16, end, new_tokens, sure, seen, from, last;
+  int first, count, real, end, new_tokens, sure, seen, from, last;
   __device__ __forceinline__ void set(const KvAttn& p, const long long* upto, long long x, long long x1) {
     j = job_at<KEYS>(p, upto, x);
     stop = min(x1, j.begin + j.cost);
@@ -144,8 +163,8 @@ struct Part {
     new_tokens = next - first;
     count = min(next, p.tokens) - first;
     end = max(0, min(p.ends[j.row], p.width << p.block_log));
-    rows16 = min(16, count * p.group - j.qt * 16);                // real rows of the tile
-    const int tok0 = j.qt * 16 / p.group, tok1 = (j.qt * 16 + rows16 - 1) / p.group;
+    real = min(p.tile, count * p.group - j.qt * p.tile);          // real rows of the tile
+    const int tok0 = j.qt * p.tile / p.group, tok1 = (j.qt * p.tile + real - 1) / p.group;
     sure = max(0, min(end, end - new_tokens + tok0 + 1));         // the fewest keys that a real row sees
     seen = max(0, min(end, end - new_tokens + tok1 + 1));         // the most
     const int all = ceil_div(seen, KEYS);
@@ -185,12 +204,15 @@ struct Feed {                          // runs over the steps of a warp's piece,
   Part<Shape<D>::KEYS> part;
   long long x, x1, stride;
   int step, page0, id;                 // lane l holds the block id of page page0 + l
+  uint32_t place;                      // of this lane's chunk among 32
   bool more;
   __device__ __forceinline__ void begin(const KvAttn& p, const long long* upto, long long at, long long end, long long by) {
     x = at;
     x1 = end;
     stride = by;
     more = true;
+    const int lane = threadIdx.x & 31;
+    place = chunk_at<D>(lane / (D / 16), lane % (D / 16));
     open(p, upto);
   }
   __device__ __forceinline__ void open(const KvAttn& p, const long long* upto) {     // the next part that has steps
@@ -225,8 +247,8 @@ struct Feed {                          // runs over the steps of a warp's piece,
         const uint8_t* src = p.codes + (real ? ((page << p.block_log) + in) * D : 0) + lane * 16;
         const uint32_t kd = smem_u32(st->k) + s * 1024, vd = smem_u32(st->v) + s * 1024;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {                        // 16 keys: D chunks
-          const int n = i * 32 + lane, at = chunk_at<D>(n / (D / 16), n % (D / 16));
+        for (int i = 0; i < D / 32; ++i) {                        // 16 keys: D chunks; 512 bytes on, a row's bit 2 changes (D = 128) or none
+          const uint32_t at = i * 512 + (D == 128 && (i & 1) ? place ^ 64 : place);
           copy16(kd + at, src + i * 512, real);
           copy16(vd + at, src + p.kv_stride + i * 512, real);
         }
@@ -244,25 +266,22 @@ struct Feed {                          // runs over the steps of a warp's piece,
   }
 };
 
-template <int D>
-struct Tile {                          // what a warp keeps of a tile of 16 query rows
-  uint32_t q[D / 16][4];
-  float o[D / 8][4];                   // in units of vref
-  float m[2], l[2], f[2];              // rows g and g + 8: maximum (log2), this lane's sum, factor of a raw score
-  int lim[2];                          // keys that the row sees
+template <int D, int NB>
+struct Tile {                          // what a warp keeps of a tile of 8 NB query rows
+  uint32_t q[NB][D / 16][2];           // row g of each 8
+  float o[NB][D / 16][4];              // dimensions g D / 8 + 2 b, + 1 of rows 2c, 2c + 1; in units of vref
+  float m[NB][2], l[NB][2], f[NB][2];  // rows 2c, 2c + 1: maximum (log2), this lane's sum, factor of a raw score
+  int lim[NB][2];                      // keys that the row sees
   float vref;
 };
 
-template <int D>
-__device__ __forceinline__ void load_q(const KvAttn& p, int first, int count, int head, int end, int new_tokens, int qt, Tile<D>& t) {
+template <int D, int NB>
+__device__ __forceinline__ void load_q(const KvAttn& p, int first, int count, int head, int end, int new_tokens, int qt, Tile<D, NB>& t) {
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int idx = qt * 16 + r * 8 + g, tok = idx / p.group;
+  for (int b = 0; b < NB; ++b) {
+    const int idx = qt * p.tile + b * 8 + g, tok = idx / p.group;
     const bool real = tok < count;
-    t.lim[r] = real ? max(0, min(end, end - new_tokens + tok + 1)) : 0;
-    t.m[r] = -INFINITY;
-    t.l[r] = 0.f;
     float x[D / 4], top = 0.f;
     const __nv_bfloat16* q = (const __nv_bfloat16*)p.q + (long long)(first + tok) * p.q_token + (long long)(head * p.group + idx - tok * p.group) * p.q_head;
 #pragma unroll
@@ -275,8 +294,8 @@ __device__ __forceinline__ void load_q(const KvAttn& p, int first, int count, in
           if (p.q_vec) {
             w = *reinterpret_cast<const uint4*>(a);
           } else {
-            const unsigned short* b = reinterpret_cast<const unsigned short*>(a);
-            w = make_uint4(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16, b[4] | (uint32_t)b[5] << 16, b[6] | (uint32_t)b[7] << 16);
+            const unsigned short* e = reinterpret_cast<const unsigned short*>(a);
+            w = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
           }
         }
         const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
@@ -293,214 +312,224 @@ __device__ __forceinline__ void load_q(const KvAttn& p, int first, int count, in
     int e = (int)(__float_as_uint(top) >> 23) - 127;
     e = top > 0.f && e < 128 ? max(-100, min(112, e - 14)) : 0;
     const float s = __uint_as_float((uint32_t)(127 - e) << 23);
-    t.f[r] = p.scale_log2 * __uint_as_float((uint32_t)(127 + e) << 23);
+    const float back = p.scale_log2 * __uint_as_float((uint32_t)(127 + e) << 23);
+    const int lim = real ? max(0, min(end, end - new_tokens + tok + 1)) : 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      t.f[b][h] = __shfl_sync(0xffffffffu, back, (2 * c + h) * 4);
+      t.lim[b][h] = __shfl_sync(0xffffffffu, lim, (2 * c + h) * 4);
+      t.m[b][h] = NONE;
+      t.l[b][h] = 0.f;
+    }
 #pragma unroll
     for (int u = 0; u < D / 64; ++u)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        t.q[u * 4 + k][r] = f16_pair(x[u * 16 + k * 4] * s, x[u * 16 + k * 4 + 1] * s);
-        t.q[u * 4 + k][2 + r] = f16_pair(x[u * 16 + k * 4 + 2] * s, x[u * 16 + k * 4 + 3] * s);
-      }
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) t.q[b][u * 4 + k][h] = f16_pair(x[u * 16 + k * 4 + 2 * h] * s, x[u * 16 + k * 4 + 2 * h + 1] * s);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t.o[b][j][i] = 0.f;
   }
-#pragma unroll
-  for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t.o[j][i] = 0.f;
   t.vref = 0.f;
 }
 
-// P V of one sub-tile: acc += P (16 x 16) V (16 x D)
-template <int D>
-__device__ __forceinline__ void times_v(float (&acc)[D / 8][4], const uint32_t (&pa)[4], const uint32_t (&v)[4][D / 32]) {
+// V^T P^T of one sub-tile: acc += V^T (D x 16 keys) P^T (16 keys x 8 rows)
+template <int D, int NB>
+__device__ __forceinline__ void times_v(float (&acc)[NB][D / 16][4], const uint32_t (&pt)[NB][2], const uint32_t (&v)[4][D / 32]) {
 #pragma unroll
   for (int w = 0; w < D / 32; ++w) {
     // bytes of two keys side by side: two dimensions per word
-    const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
-    const uint32_t b0 = __byte_perm(v[2][w], v[3][w], 0x5140), b1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-    mma(acc[w * 4 + 0], pa, f16_of_codes(a0), f16_of_codes(b0));
-    mma(acc[w * 4 + 1], pa, f16_of_codes(a0 >> 16), f16_of_codes(b0 >> 16));
-    mma(acc[w * 4 + 2], pa, f16_of_codes(a1), f16_of_codes(b1));
-    mma(acc[w * 4 + 3], pa, f16_of_codes(a1 >> 16), f16_of_codes(b1 >> 16));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t a[4];
+      f16_of_codes(__byte_perm(v[0][w], v[1][w], h ? 0x7362 : 0x5140), a[0], a[1]);
+      f16_of_codes(__byte_perm(v[2][w], v[3][w], h ? 0x7362 : 0x5140), a[2], a[3]);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) mma(acc[b][w * 2 + h], a, pt[b][0], pt[b][1]);
+    }
   }
 }
 
-// One step of a tile.  Column 2c + e of n-block n of the scores is key (2n + e) 4 + c of its sub-tile.
-template <int D>
-__device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D>& t, const Stage* st, int step, int seen, int sure) {
+// One step of a tile.  Row g + 8 h of the transposed scores is key (2h + (g & 1)) 4 + (g >> 1) of its sub-tile.  `seen`: the
+// most keys that a row of the tile sees, `sure`: the fewest that a real row sees.
+template <int D, int NB>
+__device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const Stage* st, int step, int seen, int sure) {
   constexpr int SUB = Shape<D>::SUB, KEYS = Shape<D>::KEYS;
-  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  float s[SUB][2][4], ks[SUB], vs[SUB];
-  bool has[SUB];
-  uint32_t v[SUB][4][D / 32];          // [key 4 r + c][bytes of dimensions g D / 8 ...]
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, key = (g & 1) * 4 + (g >> 1);
+  const int k0 = step * KEYS;
+  const bool whole = k0 + KEYS <= sure;
+  float s[SUB][NB][4];                 // keys `key` and `key + 8` of rows 2c, 2c + 1
 #pragma unroll
   for (int u = 0; u < SUB; ++u) {
-    ks[u] = st->ks[u];
-    vs[u] = st->vs[u];
-    has[u] = st->has[u] != 0;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[u][n][i] = 0.f;
+      for (int i = 0; i < 4; ++i) s[u][b][i] = 0.f;
 #pragma unroll
-      for (int d = 0; d < D / 64; ++d) {
-        const uint4 x = *reinterpret_cast<const uint4*>(st->k + u * 1024 + chunk_at<D>((n * 2 + (g & 1)) * 4 + (g >> 1), d * 4 + c));
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    for (int d = 0; d < D / 64; ++d) {
+      const uint4 x = *reinterpret_cast<const uint4*>(st->k + u * 1024 + chunk_at<D>(key, d * 4 + c));
+      const uint4 y = *reinterpret_cast<const uint4*>(st->k + u * 1024 + chunk_at<D>(key + 8, d * 4 + c));
+      const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mma(s[u][n], t.q[d * 4 + k], f16_of_codes(w[k]), f16_of_codes(w[k] >> 16));
-      }
-    }
+      for (int k = 0; k < 4; ++k) {
+        uint32_t a[4];
+        f16_of_codes(xw[k], a[0], a[2]);
+        f16_of_codes(yw[k], a[1], a[3]);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (D == 64) {
-        const uint2 x = *reinterpret_cast<const uint2*>(st->v + u * 1024 + chunk_at<D>(k * 4 + c, g >> 1) + (g & 1) * 8);
-        v[u][k][0] = x.x;
-        v[u][k][1] = x.y;
-      } else {
-        const uint4 x = *reinterpret_cast<const uint4*>(st->v + chunk_at<D>(k * 4 + c, g));
-        v[u][k][0] = x.x;
-        v[u][k][1] = x.y;
-        v[u][k][D / 32 - 2] = x.z;
-        v[u][k][D / 32 - 1] = x.w;
+        for (int b = 0; b < NB; ++b) mma(s[u][b], a, t.q[b][d * 4 + k][0], t.q[b][d * 4 + k][1]);
       }
     }
   }
-  // scores in log2 units, masked; a NaN score stays NaN (the comparisons below let it through)
-  const int k0 = step * KEYS;
-  const bool whole = k0 + KEYS <= sure;
-  float top[2] = {-INFINITY, -INFINITY}, vtop = t.vref;
-  bool lacks = false;
-#pragma unroll
-  for (int u = 0; u < SUB; ++u) lacks |= !has[u];
+  float f[SUB][NB][2], vs[SUB], vtop = t.vref;
+  bool has[SUB], lacks = false;
 #pragma unroll
   for (int u = 0; u < SUB; ++u) {
-    const float f0 = t.f[0] * ks[u], f1 = t.f[1] * ks[u];
+    const float ks = st->ks[u];
+    vs[u] = st->vs[u];
+    has[u] = st->has[u] != 0;
+    lacks |= !has[u];
     vtop = has[u] ? fmaxf(vtop, vs[u]) : vtop;
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[u][n][i] *= i < 2 ? f0 : f1;
+    for (int b = 0; b < NB; ++b) {
+      f[u][b][0] = fmaxf(t.f[b][0] * ks, 1.2e-38f);   // not zero, which would make a masked -inf a NaN
+      f[u][b][1] = fmaxf(t.f[b][1] * ks, 1.2e-38f);
+    }
   }
   if (!whole || lacks) {
 #pragma unroll
     for (int u = 0; u < SUB; ++u)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int b = 0; b < NB; ++b) {
+        if (!has[u]) f[u][b][0] = f[u][b][1] = 1.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (k0 + u * 16 + (n * 2 + (i & 1)) * 4 + c >= t.lim[i >> 1] || !has[u]) s[u][n][i] = -INFINITY;
-    // values behind the last key that any row sees are not numbers to be multiplied by zero
+          if (k0 + u * 16 + key + (i >> 1) * 8 >= t.lim[b][i & 1] || !has[u]) s[u][b][i] = -INFINITY;
+      }
+  }
+  // exponents; where one is too large for f16 the maxima are raised first.  A NaN lets itself through.
+  float big = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < SUB; ++u)
+  for (int u = 0; u < SUB; ++u)
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) big = fmaxf(big, fmaf(s[u][b][i], f[u][b][i & 1], -t.m[b][i & 1]));
+  if (__any_sync(0xffffffffu, big > RAISE) || vtop > t.vref) {
+    const float v = t.vref > 0.f ? t.vref / vtop : 0.f;
+    t.vref = vtop;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      float a[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) top = fmaxf(top, fmaxf(s[u][b][i], s[u][b][2 + i]) * f[u][b][i]);
+        top = column_max(top);
+        const bool raise = top > t.m[b][i] + RAISE;
+        a[i] = raise ? ex2(t.m[b][i] - top) : 1.f;
+        if (raise) t.m[b][i] = top;
+        t.l[b][i] *= a[i];
+        a[i] *= v;
+      }
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t.o[b][j][i] *= a[i & 1];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < SUB; ++u) {
+    uint32_t v[4][D / 32];             // [key 4 r + c][bytes of dimensions g D / 8 ...]
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (D == 64) {
+        const uint2 x = *reinterpret_cast<const uint2*>(st->v + u * 1024 + chunk_at<D>(k * 4 + c, g >> 1) + (g & 1) * 8);
+        v[k][0] = x.x;
+        v[k][1] = x.y;
+      } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(st->v + chunk_at<D>(k * 4 + c, g));
+        v[k][0] = x.x;
+        v[k][1] = x.y;
+        v[k][D / 32 - 2] = x.z;
+        v[k][D / 32 - 1] = x.w;
+      }
+    }
+    if (!has[u]) continue;
+    // Weights relative to vref; a block whose values are less than 2^-14 of the largest block's would lose bits in f16, so its
+    // product is taken by itself and added in fp32.
+    const float ratio = t.vref > 0.f ? vs[u] / t.vref : 0.f;
+    const bool apart = ratio < 6.1035156e-5f;
+    const uint32_t w2 = f16_pair(apart ? 1.f : ratio, apart ? 1.f : ratio);
+    uint32_t pt[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e[i] = ex2(fmaf(s[u][b][i], f[u][b][i & 1], LIFT - t.m[b][i & 1]));
+        t.l[b][i & 1] += e[i];
+      }
+      pt[b][0] = times(transposed(f16_pair(e[0], e[1])), w2);
+      pt[b][1] = times(transposed(f16_pair(e[2], e[3])), w2);
+    }
+    if (!whole) {
+      // values behind the last key that any row sees are not numbers to be multiplied by zero
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         if (k0 + u * 16 + k * 4 + c >= seen) {
 #pragma unroll
-          for (int w = 0; w < D / 32; ++w) v[u][k][w] = 0;
+          for (int x = 0; x < D / 32; ++x) v[k][x] = 0;
         }
-  }
-#pragma unroll
-  for (int u = 0; u < SUB; ++u)
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      top[0] = fmaxf(top[0], fmaxf(s[u][n][0], s[u][n][1]));
-      top[1] = fmaxf(top[1], fmaxf(s[u][n][2], s[u][n][3]));
-    }
-  top[0] = quad_max(top[0]);
-  top[1] = quad_max(top[1]);
-  const bool raise0 = top[0] > t.m[0] + RAISE || (t.m[0] == -INFINITY && top[0] > -INFINITY);
-  const bool raise1 = top[1] > t.m[1] + RAISE || (t.m[1] == -INFINITY && top[1] > -INFINITY);
-  if (__any_sync(0xffffffffu, raise0 || raise1) || vtop > t.vref) {
-    const float v = t.vref > 0.f ? t.vref / vtop : 0.f;
-    float a[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bool raise = i ? raise1 : raise0;
-      a[i] = raise ? ex2(t.m[i] - top[i]) : 1.f;
-      if (raise) t.m[i] = top[i];
-      t.l[i] *= a[i];
-      a[i] *= v;
-    }
-    t.vref = vtop;
-#pragma unroll
-    for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) t.o[j][i] *= a[i >> 1];
-  }
-  const float b0 = (t.m[0] == -INFINITY ? 0.f : t.m[0]) - LIFT, b1 = (t.m[1] == -INFINITY ? 0.f : t.m[1]) - LIFT;
-#pragma unroll
-  for (int u = 0; u < SUB; ++u) {
-    if (!has[u]) continue;
-    // Weights relative to vref; a block whose values are less than 2^-24 of the largest block's would lose bits in f16, so
-    // its product is taken by itself and added in fp32.
-    const float ratio = t.vref > 0.f ? vs[u] / t.vref : 0.f;
-    const bool apart = ratio < 5.9604645e-8f;
-    uint32_t pa[4];
-    float sum0 = 0.f, sum1 = 0.f;
-    const float w = apart ? 1.f : ratio;
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      float e0 = ex2(s[u][n][0] - b0), e1 = ex2(s[u][n][1] - b0), e2 = ex2(s[u][n][2] - b1), e3 = ex2(s[u][n][3] - b1);
-      sum0 += e0 + e1;
-      sum1 += e2 + e3;
-      pa[2 * n] = f16_pair(e0 * w, e1 * w);
-      pa[2 * n + 1] = f16_pair(e2 * w, e3 * w);
-    }
-    t.l[0] += sum0;
-    t.l[1] += sum1;
-    if (!whole) {
       // Rows that do not see a key that others see would multiply its value by zero; NaN there is taken out, and put into the
       // rows that do see it.
       uint32_t any = 0;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x) any |= nan_code(v[u][k][x]);
+        for (int x = 0; x < D / 32; ++x) any |= nan_code(v[k][x]);
       if (__any_sync(0xffffffffu, any != 0)) {
-        const int key = k0 + u * 16;
-        for (int k = 0; k < 16 && key + k < seen; ++k)
+        for (int k = 0; k < 16; ++k) {
+          // key k lies with the lanes c = k & 3, in register k >> 2; word x carries dimensions g D / 8 + 4 x ..
+#pragma unroll
           for (int x = 0; x < D / 32; ++x) {
-            // key k lies with the lanes c = k & 3, in register k >> 2; word x carries dimensions g D / 8 + 4 x ..
-            const int holder = k & 3, reg = k >> 2;
-            uint32_t word = 0;
+            const uint32_t mine = k < 4 ? v[0][x] : k < 8 ? v[1][x] : k < 12 ? v[2][x] : v[3][x];
+            const uint32_t got = __shfl_sync(0xffffffffu, mine, g * 4 + (k & 3));
 #pragma unroll
-            for (int rr = 0; rr < 4; ++rr)
+            for (int j = 0; j < 4; ++j)
+              if (((got >> (8 * j)) & 0x7fu) == 0x7fu)
 #pragma unroll
-              for (int xx = 0; xx < D / 32; ++xx)
-                if (rr == reg && xx == x) word = v[u][rr][xx];
+                for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              // this lane's output columns 2c + e of every n-block: dimensions (2c + e) D / 8 + j
-              const uint32_t got = __shfl_sync(0xffffffffu, word, (2 * c + e) * 4 + holder);
-#pragma unroll
-              for (int j = 0; j < D / 8; ++j)
-                if (j / 4 == x && ((got >> (8 * (j & 3))) & 0x7fu) == 0x7fu) {
-                  if (key + k < t.lim[0]) t.o[j][e] = __int_as_float(0x7fffffff);
-                  if (key + k < t.lim[1]) t.o[j][2 + e] = __int_as_float(0x7fffffff);
-                }
-            }
+                  for (int i = 0; i < 2; ++i)
+                    if (k0 + u * 16 + k < t.lim[b][i]) t.o[b][x * 2 + (j >> 1)][(j & 1) * 2 + i] = __int_as_float(0x7fffffff);
           }
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            const uint32_t hit = nan_code(v[u][k][x]) >> 7;     // 1 in the byte of a NaN
-            v[u][k][x] &= ~(hit * 0xffu);
-          }
+          for (int x = 0; x < D / 32; ++x) v[k][x] &= ~((nan_code(v[k][x]) >> 7) * 0xffu);
       }
     }
     if (!apart) {
-      times_v<D>(t.o, pa, v[u]);
+      times_v<D, NB>(t.o, pt, v);
     } else {
-      float acc[D / 8][4];
+      float acc[NB][D / 16][4];
 #pragma unroll
-      for (int j = 0; j < D / 8; ++j)
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
-      times_v<D>(acc, pa, v[u]);
+        for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-      for (int j = 0; j < D / 8; ++j)
+          for (int i = 0; i < 4; ++i) acc[b][j][i] = 0.f;
+      times_v<D, NB>(acc, pt, v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) t.o[j][i] += acc[j][i] * ratio;
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t.o[b][j][i] += acc[b][j][i] * ratio;
     }
   }
 }
@@ -523,7 +552,7 @@ __device__ __forceinline__ void store_out(const KvAttn& p, int first, int head, 
 // Partial results of a warp: slot 1 for the job that begins in its piece and runs on, slot 0 for the one that came from before.
 __device__ __forceinline__ long long slot_at(long long piece, int slot) { return (piece * 2 + slot) * 16; }
 
-template <int D>
+template <int D, int NB>
 __global__ void __launch_bounds__(THREADS, 3) kv_attn_kernel(KvAttn p) {
   constexpr int KEYS = Shape<D>::KEYS;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -545,34 +574,34 @@ __global__ void __launch_bounds__(THREADS, 3) kv_attn_kernel(KvAttn p) {
   while (x < x1) {
     Part<KEYS> w;
     w.set(p, upto, x, x1);
-    Tile<D> t;
-    load_q<D>(p, w.first, w.count, w.j.head, w.end, w.new_tokens, w.j.qt, t);
+    Tile<D, NB> t;
+    load_q<D, NB>(p, w.first, w.count, w.j.head, w.end, w.new_tokens, w.j.qt, t);
     for (int st = w.from; st < w.last; ++st) {
       asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
       __syncwarp();                    // the step's codes are there for all lanes, and all are done with the step before
       feed.next(p, upto, ring + (at + STAGES - 1) % STAGES);
-      step_tile<D>(p, t, ring + at, st, w.seen, w.sure);
+      step_tile<D, NB>(p, t, ring + at, st, w.seen, w.sure);
       at = (at + 1) % STAGES;
     }
     const bool alone = p.solo || (x == w.j.begin && w.stop == w.j.begin + w.j.cost);
     const long long slot = slot_at(piece, x == w.j.begin);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = g + 8 * h;
-      const float l = quad_sum(t.l[h]);
-      if (row >= w.rows16) continue;
-      const float f = alone ? (l == 0.f ? 0.f : t.vref / l) : t.vref;
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int h = 0; h < 2; ++h) {
+        const int row = b * 8 + 2 * c + h;
+        const float l = column_sum(t.l[b][h]);
+        if (row >= w.real) continue;
+        const float f = alone ? (l == 0.f ? 0.f : t.vref / l) : t.vref;
 #pragma unroll
-        for (int k = 0; k < D / 8; k += 4) {
-          const int d = (2 * c + e) * (D / 8) + k;
-          const float4 o = make_float4(t.o[k][2 * h + e] * f, t.o[k + 1][2 * h + e] * f, t.o[k + 2][2 * h + e] * f, t.o[k + 3][2 * h + e] * f);
-          if (alone) store_out<D>(p, w.first, w.j.head, w.j.qt * 16 + row, d, o.x, o.y, o.z, o.w);
+        for (int k = 0; k < D / 16; k += 2) {
+          const int d = g * (D / 8) + 2 * k;
+          const float4 o = make_float4(t.o[b][k][h] * f, t.o[b][k][2 + h] * f, t.o[b][k + 1][h] * f, t.o[b][k + 1][2 + h] * f);
+          if (alone) store_out<D>(p, w.first, w.j.head, w.j.qt * p.tile + row, d, o.x, o.y, o.z, o.w);
           else *reinterpret_cast<float4*>(p.part_o + (slot + row) * D + d) = o;
         }
-      if (!alone && c == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + row) * 2) = make_float2(t.m[h], l);
-    }
+        if (!alone && g == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + row) * 2) = make_float2(t.m[b][h], l);
+      }
     x = stride ? x + stride : w.stop;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
@@ -596,10 +625,10 @@ __global__ void __launch_bounds__(THREADS) kv_attn_join_kernel(KvAttn p) {
   if (j.begin < lo || j.begin + j.cost <= hi) return;
   const int n = (int)((j.begin + j.cost - 1) / cut.piece - blockIdx.x) + 1;
   const int first = p.starts[j.row], count = min(p.starts[j.row + 1], p.tokens) - first;
-  const int rows16 = min(16, count * p.group - j.qt * 16);
+  const int real = min(p.tile, count * p.group - j.qt * p.tile);
   const int tid = threadIdx.x, col = tid % COLS, share = tid / COLS;
-  for (int row = 0; row < rows16; ++row) {
-    float top = -INFINITY;
+  for (int row = 0; row < real; ++row) {
+    float top = NONE;
     for (int w = tid; w < n; w += THREADS) top = fmaxf(top, p.part_ml[(slot_at(blockIdx.x + w, w == 0) + row) * 2]);
     top = block_max(top, s_l + SHARES);
     float l = 0.f;
@@ -608,7 +637,7 @@ __global__ void __launch_bounds__(THREADS) kv_attn_join_kernel(KvAttn p) {
     for (int w = share; w < n; w += SHARES) {
       const long long s = slot_at(blockIdx.x + w, w == 0) + row;
       const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + s * 2);
-      const float f = ml.x == -INFINITY ? 1.f : ex2(ml.x - top);  // without a maximum all is zero, or NaN
+      const float f = ml.x == NONE ? 1.f : ex2(ml.x - top);        // without a maximum all is zero, or NaN
       const float4 v = *reinterpret_cast<const float4*>(p.part_o + s * D + col * 4);
       l += ml.y * f;
       o.x += v.x * f;
@@ -630,13 +659,13 @@ __global__ void __launch_bounds__(THREADS) kv_attn_join_kernel(KvAttn p) {
         l += s_l[i];
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      store_out<D>(p, first, j.head, j.qt * 16 + row, col * 4, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+      store_out<D>(p, first, j.head, j.qt * p.tile + row, col * 4, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     }
     __syncthreads();
   }
 }
 
-template <int D>
+template <int D, int NB>
 int launch_few(KvAttn p, cudaStream_t stream) {
   const int scan = (WARPS + p.rows + 1) * 8, smem = WARPS * STAGES * (int)sizeof(Stage) + scan;
   const int join_smem = THREADS * 16 + (THREADS / (D / 4) + WARPS) * 4 + scan;
@@ -645,12 +674,13 @@ int launch_few(KvAttn p, cudaStream_t stream) {
   NB_CUDA(cudaGetDevice(&dev));
   if (dev >= 64) return NB_ERR_BAD_ARG;
   if (!configured[dev]) {
-    NB_CUDA(cudaFuncSetAttribute(kv_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, WARPS * STAGES * (int)sizeof(Stage) + (WARPS + 8193) * 8));
+    NB_CUDA(cudaFuncSetAttribute(kv_attn_kernel<D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, WARPS * STAGES * (int)sizeof(Stage) + (WARPS + 8193) * 8));
     NB_CUDA(cudaFuncSetAttribute(kv_attn_join_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024));
     configured[dev] = true;
   }
+  p.tile = 8 * NB;
   p.solo = ((long long)p.width << p.block_log) <= SOLO * Shape<D>::KEYS;
-  kv_attn_kernel<D><<<p.pieces / WARPS, THREADS, smem, stream>>>(p);
+  kv_attn_kernel<D, NB><<<p.pieces / WARPS, THREADS, smem, stream>>>(p);
   NB_LAUNCH_CHECK();
   if (p.solo) return NB_OK;
   cudaLaunchConfig_t cfg = {};
@@ -681,6 +711,7 @@ int nb_kv_attention(const void* q, void* out, const void* codes, const float* sc
                     float softmax_scale, float* work, long long work_floats, unsigned int* status, void* stream) {
   if (rows <= 0 || rows > 8192 || tokens < 0 || hk <= 0 || hq <= 0 || hq % hk || (dim != 64 && dim != 128) || blocks <= 0 || width <= 0) return NB_ERR_BAD_ARG;
   if ((block & (block - 1)) || block < 16 || (long long)width * block > 0x7fffffffLL || (long long)blocks * block > 0x7fffffffLL) return NB_ERR_BAD_ARG;
+  if (!(softmax_scale > 0.f)) return NB_ERR_BAD_ARG;
   if ((long long)tokens * hq > 0x7fffffffLL) return NB_ERR_TOO_LARGE;
   if (tokens == 0) return NB_OK;
   if ((reinterpret_cast<uintptr_t>(codes) & 15) || (kv_stride & 15)) return NB_ERR_UNALIGNED;
@@ -698,7 +729,11 @@ int nb_kv_attention(const void* q, void* out, const void* codes, const float* sc
   p.part_ml = work + (long long)p.pieces * 2 * 16 * dim;
   p.few = 0x7fffffff;
   p.status = status;
-  return dim == 64 ? launch_few<64>(p, (cudaStream_t)stream) : launch_few<128>(p, (cudaStream_t)stream);
+  const cudaStream_t s = (cudaStream_t)stream;
+  // one group of eight query rows where no row of the batch has more; with more, two groups share every conversion of a code
+  const bool one = (long long)min(max_new, tokens) * p.group <= 8;
+  if (dim == 64) return one ? launch_few<64, 1>(p, s) : launch_few<64, 2>(p, s);
+  return one ? launch_few<128, 1>(p, s) : launch_few<128, 2>(p, s);
 }
 
 }  // extern "C"

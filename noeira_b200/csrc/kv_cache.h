@@ -43,6 +43,7 @@ struct KvAttn {
   int rows, tokens, hq, hk, group, block_log, blocks, width;
   int q_vec, o_vec;                             // 16-byte loads of q and 8-byte stores of out are aligned
   int few;                                      // rows of the batch with at most this many query rows per head are done here
+  int tile;                                     // query rows of a tile
   int pieces, solo;                             // warps; every tile is one warp's
   long long q_token, q_head, o_token, o_head;
   long long kv_stride, s_stride;                // from the keys' codes / scales to the values'

@@ -243,6 +243,8 @@ def paged_attention(q, kv, scale, tables, starts, ends, max_new=None, softmax_sc
     max_new = tokens if max_new is None else min(int(max_new), tokens)
     if max_new <= 0 < tokens:
         raise ValueError(f"max_new: at least 1, got {max_new}")
+    if not softmax_scale > 0:
+        raise ValueError(f"softmax_scale: positive, got {softmax_scale}")
     if dev < 0:
         return _attention_cpu(q, kv, scale, tables, starts, ends, softmax_scale, out)
     if out is None:
