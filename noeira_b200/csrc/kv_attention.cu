@@ -8,13 +8,16 @@
 //     which there are enough of, and its 8 columns are query rows, which in a decode step there are not.  e4m3 codes are exact
 //     in f16; q (bf16) is exact in f16 down to 2^-38 of the row's largest element after a power-of-two scaling of the row; P
 //     keeps 11 bits.
-//   * A warp works by itself: codes come by cp.async into its own ring in shared memory, 4 KB a step, and from there as they
-//     are into the fragments.  The order of the contraction is free as long as q has the same, so a lane's fragment of K is 16
-//     consecutive bytes of a key; the orders of keys and of output columns are free, so its fragment of V is D / 8 consecutive
-//     bytes of four keys.  The 16-byte chunks are swizzled so that both reads are free of bank conflicts.
+//   * A warp works by itself: TMA brings the codes into its own ring in shared memory, 4 KB a step (two boxes of 16 keys each for
+//     keys and values at D = 64, one at 128; a block id that is none becomes a box outside the tensor, which arrives as zeros),
+//     and from there they go as they are into the fragments.  The order of the contraction is free as long as q has the same,
+//     so a lane's fragment of K is 16 consecutive bytes of a key; the order of the output rows is free, so its fragment of V is
+//     D / 8 consecutive bytes of four keys.  The copies' swizzle keeps both reads at two bank conflicts or fewer.
 //   * The steps of the whole batch are cut into equal pieces, one for each resident warp (rows differ in length, so pieces run
 //     over the ends of rows, and the ring runs ahead into the next row); a second, small kernel joins rows that lie in several
 //     pieces.
+#include <cuda.h>
+
 #include "common.cuh"
 #include "kv_cache.h"
 
@@ -91,6 +94,10 @@ struct Job {
   long long begin;
 };
 
+// a / b; batches whose sums pass 32 bits are rare, and a 64-bit division takes as long as a step
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
 template <int KEYS>
 __device__ __forceinline__ int job_cost(const KvAttn& p, int i) {
   return p.solo ? 1 : LEAD + ceil_div(max(1, min(p.ends[i], p.width << p.block_log)), KEYS);
@@ -122,7 +129,7 @@ __device__ __forceinline__ Cut cut_batch(const KvAttn& p, long long* upto, long 
     if (i < w) at += sh[i];
     c.total += sh[i];
   }
-  c.piece = p.solo ? 1 : max((long long)LEAST, (c.total + p.pieces - 1) / p.pieces);
+  c.piece = p.solo ? 1 : max((long long)LEAST, quotient(c.total + p.pieces - 1, p.pieces));
   at -= sum;
   for (int i = lo; i < hi; ++i) {
     upto[i] = at;
@@ -142,9 +149,9 @@ __device__ __forceinline__ Job job_at(const KvAttn& p, const long long* upto, lo
   Job j;
   j.row = a;
   j.cost = job_cost<KEYS>(p, a);
-  const long long n = (x - upto[a]) / j.cost;
-  j.head = (int)(n % p.hk);
-  j.qt = (int)(n / p.hk);
+  const long long n = quotient(x - upto[a], j.cost);
+  j.qt = (int)n / p.hk;                // jobs of a row: at most tokens * heads, 31 bits
+  j.head = (int)n - j.qt * p.hk;
   j.begin = upto[a] + n * j.cost;
   return j;
 }
@@ -179,40 +186,29 @@ struct Shape {
   static constexpr int SUB = 128 / D;  // sub-tiles of 16 keys in a step
   static constexpr int KEYS = 16 * SUB;
 };
-struct __align__(16) Stage {
-  uint8_t k[2048], v[2048];
-  float ks[2], vs[2];                  // scales of the sub-tiles
-  int has[2];                          // 0: no keys there (past the end, or a bad block)
-  int pad[2];
+constexpr int STAGE = 4096;            // 2 KB of keys, 2 KB of values
+struct Head {                          // of a stage
+  float ks[2], vs[2];                  // scales of the sub-tiles; a scale below zero: no keys there
 };
 
-// Byte of 16-byte chunk `ch` of key row `r` (0..15) in a sub-tile.
+// Byte of 16-byte chunk `ch` of row `r` (0..15) of a sub-tile, as the copy's swizzle leaves it.
 template <int D>
 __device__ __forceinline__ int chunk_at(int r, int ch) {
-  if (D == 64) return (r >> 1) * 128 + ((((r & 1) * 4 + ch) ^ (((r >> 1) & 1) * 2 | ((r >> 2) & 1) * 4)) << 4);
-  return r * 128 + ((ch ^ ((r & 3) * 2) ^ (((r >> 2) & 1) * 4)) << 4);
-}
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+  return D == 64 ? r * 64 + ((ch ^ ((r >> 1) & 3)) << 4) : r * 128 + ((ch ^ (r & 7)) << 4);
 }
 
 template <int D>
 struct Feed {                          // runs over the steps of a warp's piece, ahead of the work
   Part<Shape<D>::KEYS> part;
   long long x, x1, stride;
-  int step, page0, id;                 // lane l holds the block id of page page0 + l
-  uint32_t place;                      // of this lane's chunk among 32
+  int step, page0, base;               // lane l: first row of page page0 + l among the tensor's rows, none: behind the last
+  float ks, vs;                        // and its scales
   bool more;
   __device__ __forceinline__ void begin(const KvAttn& p, const long long* upto, long long at, long long end, long long by) {
     x = at;
     x1 = end;
     stride = by;
     more = true;
-    const int lane = threadIdx.x & 31;
-    place = chunk_at<D>(lane / (D / 16), lane % (D / 16));
     open(p, upto);
   }
   __device__ __forceinline__ void open(const KvAttn& p, const long long* upto) {     // the next part that has steps
@@ -223,46 +219,53 @@ struct Feed {                          // runs over the steps of a warp's piece,
       if (part.from < part.last) break;
     }
     step = part.from;
-    page0 = -64;
+    turn(p, step * Shape<D>::KEYS >> p.block_log);
   }
-  __device__ __forceinline__ void next(const KvAttn& p, const long long* upto, Stage* st) {
-    constexpr int SUB = Shape<D>::SUB, KEYS = Shape<D>::KEYS;
-    const int lane = threadIdx.x & 31;
-    if (more) {
-#pragma unroll
-      for (int s = 0; s < SUB; ++s) {
-        const int k0 = step * KEYS + s * 16, pg = k0 >> p.block_log;
-        int b = -2;
-        if (k0 < part.seen) {
-          if (pg - page0 >= 32) {
-            page0 = pg;
-            id = pg + lane < p.width ? __ldg(p.tables + (long long)part.j.row * p.width + pg + lane) : -2;
-          }
-          b = __shfl_sync(0xffffffffu, id, pg - page0);
-        }
-        const bool real = (unsigned)b < (unsigned)p.blocks;
-        if (!real && k0 < part.seen && lane == 0) report(p.status, NB_ST_BOUNDS, 10, part.j.row);
-        const long long page = real ? (long long)b * p.hk + part.j.head : 0;
-        const int in = k0 & ((1 << p.block_log) - 1);
-        const uint8_t* src = p.codes + (real ? ((page << p.block_log) + in) * D : 0) + lane * 16;
-        const uint32_t kd = smem_u32(st->k) + s * 1024, vd = smem_u32(st->v) + s * 1024;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {                        // 16 keys: D chunks; 512 bytes on, a row's bit 2 changes (D = 128) or none
-          const uint32_t at = i * 512 + (D == 128 && (i & 1) ? place ^ 64 : place);
-          copy16(kd + at, src + i * 512, real);
-          copy16(vd + at, src + p.kv_stride + i * 512, real);
-        }
-        if (lane == 0) {
-          if (real) {
-            copy4(smem_u32(&st->ks[s]), p.scale + page);
-            copy4(smem_u32(&st->vs[s]), p.scale + p.s_stride + page);
-          }
-          st->has[s] = real;
-        }
+  __device__ __forceinline__ void turn(const KvAttn& p, int page) {                  // the next 32 pages
+    page0 = page;
+    const int pg = page + (int)(threadIdx.x & 31);
+    base = p.kv_rows;
+    ks = vs = -1.f;
+    if ((long long)pg << p.block_log < part.seen) {
+      const int b = p.tables[(long long)part.j.row * p.width + pg];
+      if ((unsigned)b < (unsigned)p.blocks) {
+        const int page_head = b * p.hk + part.j.head;
+        base = page_head << p.block_log;
+        ks = p.scale[page_head];
+        vs = p.scale[p.s_stride + page_head];
+      } else {
+        report(p.status, NB_ST_BOUNDS, 10, part.j.row);
       }
-      if (++step >= part.last) open(p, upto);
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ __forceinline__ void next(const KvAttn& p, const CUtensorMap& map, const long long* upto, uint32_t stage, Head* head, uint32_t bar) {
+    constexpr int SUB = Shape<D>::SUB, KEYS = Shape<D>::KEYS;
+    if (!more) return;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) mbar_expect_tx_at(bar, STAGE);
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      const int k0 = step * KEYS + s * 16, pg = k0 >> p.block_log;
+      if (pg - page0 >= 32) turn(p, pg);
+      const int row = __shfl_sync(0xffffffffu, base, pg - page0) + (k0 & ((1 << p.block_log) - 1));
+      if (lane == pg - page0) {
+        head->ks[s] = ks;
+        head->vs[s] = vs;
+      }
+      if (lane == 0) {
+        copy_box(stage + s * 1024, map, bar, row, 0);
+        copy_box(stage + 2048 + s * 1024, map, bar, row, 1);
+      }
+    }
+    if (++step >= part.last) open(p, upto);
+  }
+  static __device__ __forceinline__ void mbar_expect_tx_at(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+  }
+  static __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap& map, uint32_t bar, int row, int which) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(&map)), "r"(bar), "r"(0), "r"(row), "r"(which)
+                 : "memory");
   }
 };
 
@@ -272,7 +275,7 @@ struct Tile {                          // what a warp keeps of a tile of 8 NB qu
   float o[NB][D / 16][4];              // dimensions g D / 8 + 2 b, + 1 of rows 2c, 2c + 1; in units of vref
   float m[NB][2], l[NB][2], f[NB][2];  // rows 2c, 2c + 1: maximum (log2), this lane's sum, factor of a raw score
   int lim[NB][2];                      // keys that the row sees
-  float vref;
+  float vref, vinv;                    // the largest scale of the values so far, and its inverse
 };
 
 template <int D, int NB>
@@ -332,7 +335,7 @@ __device__ __forceinline__ void load_q(const KvAttn& p, int first, int count, in
 #pragma unroll
       for (int i = 0; i < 4; ++i) t.o[b][j][i] = 0.f;
   }
-  t.vref = 0.f;
+  t.vref = t.vinv = 0.f;
 }
 
 // V^T P^T of one sub-tile: acc += V^T (D x 16 keys) P^T (16 keys x 8 rows)
@@ -352,15 +355,14 @@ __device__ __forceinline__ void times_v(float (&acc)[NB][D / 16][4], const uint3
   }
 }
 
-// One step of a tile.  Row g + 8 h of the transposed scores is key (2h + (g & 1)) 4 + (g >> 1) of its sub-tile.  `seen`: the
-// most keys that a row of the tile sees, `sure`: the fewest that a real row sees.
+// One step of a tile.  Row g + 8 h of the transposed scores is that key of its sub-tile.  `seen`: the most keys that a row of the tile sees, `sure`: the fewest that a real row sees.
 template <int D, int NB>
-__device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const Stage* st, int step, int seen, int sure) {
+__device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const uint8_t* st, const Head* head, int step, int seen, int sure) {
   constexpr int SUB = Shape<D>::SUB, KEYS = Shape<D>::KEYS;
-  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, key = (g & 1) * 4 + (g >> 1);
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int k0 = step * KEYS;
   const bool whole = k0 + KEYS <= sure;
-  float s[SUB][NB][4];                 // keys `key` and `key + 8` of rows 2c, 2c + 1
+  float s[SUB][NB][4];                 // keys g and g + 8 of rows 2c, 2c + 1
 #pragma unroll
   for (int u = 0; u < SUB; ++u) {
 #pragma unroll
@@ -369,8 +371,8 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
       for (int i = 0; i < 4; ++i) s[u][b][i] = 0.f;
 #pragma unroll
     for (int d = 0; d < D / 64; ++d) {
-      const uint4 x = *reinterpret_cast<const uint4*>(st->k + u * 1024 + chunk_at<D>(key, d * 4 + c));
-      const uint4 y = *reinterpret_cast<const uint4*>(st->k + u * 1024 + chunk_at<D>(key + 8, d * 4 + c));
+      const uint4 x = *reinterpret_cast<const uint4*>(st + u * 1024 + chunk_at<D>(g, d * 4 + c));
+      const uint4 y = *reinterpret_cast<const uint4*>(st + u * 1024 + chunk_at<D>(g + 8, d * 4 + c));
       const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -386,11 +388,11 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
   bool has[SUB], lacks = false;
 #pragma unroll
   for (int u = 0; u < SUB; ++u) {
-    const float ks = st->ks[u];
-    vs[u] = st->vs[u];
-    has[u] = st->has[u] != 0;
+    const float ks = head->ks[u];
+    vs[u] = head->vs[u];
+    has[u] = ks >= 0.f;
     lacks |= !has[u];
-    vtop = has[u] ? fmaxf(vtop, vs[u]) : vtop;
+    vtop = fmaxf(vtop, vs[u]);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       f[u][b][0] = fmaxf(t.f[b][0] * ks, 1.2e-38f);   // not zero, which would make a masked -inf a NaN
@@ -405,7 +407,7 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
         if (!has[u]) f[u][b][0] = f[u][b][1] = 1.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (k0 + u * 16 + key + (i >> 1) * 8 >= t.lim[b][i & 1] || !has[u]) s[u][b][i] = -INFINITY;
+          if (k0 + u * 16 + g + (i >> 1) * 8 >= t.lim[b][i & 1] || !has[u]) s[u][b][i] = -INFINITY;
       }
   }
   // exponents; where one is too large for f16 the maxima are raised first.  A NaN lets itself through.
@@ -419,6 +421,7 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
   if (__any_sync(0xffffffffu, big > RAISE) || vtop > t.vref) {
     const float v = t.vref > 0.f ? t.vref / vtop : 0.f;
     t.vref = vtop;
+    t.vinv = vtop > 0.f ? 1.f / vtop : 0.f;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       float a[2];
@@ -442,15 +445,15 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
   }
 #pragma unroll
   for (int u = 0; u < SUB; ++u) {
-    uint32_t v[4][D / 32];             // [key 4 r + c][bytes of dimensions g D / 8 ...]
+    uint32_t v[4][D / 32];             // [keys 2c, 2c + 1, 2c + 8, 2c + 9][bytes of dimensions g D / 8 ...]
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (D == 64) {
-        const uint2 x = *reinterpret_cast<const uint2*>(st->v + u * 1024 + chunk_at<D>(k * 4 + c, g >> 1) + (g & 1) * 8);
+        const uint2 x = *reinterpret_cast<const uint2*>(st + 2048 + u * 1024 + chunk_at<D>(2 * c + (k & 1) + (k >> 1) * 8, g >> 1) + (g & 1) * 8);
         v[k][0] = x.x;
         v[k][1] = x.y;
       } else {
-        const uint4 x = *reinterpret_cast<const uint4*>(st->v + chunk_at<D>(k * 4 + c, g));
+        const uint4 x = *reinterpret_cast<const uint4*>(st + 2048 + u * 1024 + chunk_at<D>(2 * c + (k & 1) + (k >> 1) * 8, g));
         v[k][0] = x.x;
         v[k][1] = x.y;
         v[k][D / 32 - 2] = x.z;
@@ -460,7 +463,7 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
     if (!has[u]) continue;
     // Weights relative to vref; a block whose values are less than 2^-14 of the largest block's would lose bits in f16, so its
     // product is taken by itself and added in fp32.
-    const float ratio = t.vref > 0.f ? vs[u] / t.vref : 0.f;
+    const float ratio = vs[u] * t.vinv;
     const bool apart = ratio < 6.1035156e-5f;
     const uint32_t w2 = f16_pair(apart ? 1.f : ratio, apart ? 1.f : ratio);
     uint32_t pt[NB][2];
@@ -479,7 +482,7 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
       // values behind the last key that any row sees are not numbers to be multiplied by zero
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (k0 + u * 16 + k * 4 + c >= seen) {
+        if (k0 + u * 16 + 2 * c + (k & 1) + (k >> 1) * 8 >= seen) {
 #pragma unroll
           for (int x = 0; x < D / 32; ++x) v[k][x] = 0;
         }
@@ -492,11 +495,12 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
         for (int x = 0; x < D / 32; ++x) any |= nan_code(v[k][x]);
       if (__any_sync(0xffffffffu, any != 0)) {
         for (int k = 0; k < 16; ++k) {
-          // key k lies with the lanes c = k & 3, in register k >> 2; word x carries dimensions g D / 8 + 4 x ..
+          // key k lies with the lanes c = (k & 7) / 2, in register (k & 1) + k / 8 * 2; word x carries dimensions g D / 8 + 4 x ..
+          const int reg = (k & 1) + (k >> 3) * 2;
 #pragma unroll
           for (int x = 0; x < D / 32; ++x) {
-            const uint32_t mine = k < 4 ? v[0][x] : k < 8 ? v[1][x] : k < 12 ? v[2][x] : v[3][x];
-            const uint32_t got = __shfl_sync(0xffffffffu, mine, g * 4 + (k & 3));
+            const uint32_t mine = reg == 0 ? v[0][x] : reg == 1 ? v[1][x] : reg == 2 ? v[2][x] : v[3][x];
+            const uint32_t got = __shfl_sync(0xffffffffu, mine, g * 4 + ((k & 7) >> 1));
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               if (((got >> (8 * j)) & 0x7fu) == 0x7fu)
@@ -553,35 +557,55 @@ __device__ __forceinline__ void store_out(const KvAttn& p, int first, int head, 
 __device__ __forceinline__ long long slot_at(long long piece, int slot) { return (piece * 2 + slot) * 16; }
 
 template <int D, int NB>
-__global__ void __launch_bounds__(THREADS, 3) kv_attn_kernel(KvAttn p) {
+__global__ void __launch_bounds__(THREADS, 3) kv_attn_kernel(const __grid_constant__ CUtensorMap map, const KvAttn p) {
   constexpr int KEYS = Shape<D>::KEYS;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  Stage* ring = reinterpret_cast<Stage*>(smem) + warp * STAGES;
-  long long* sh = reinterpret_cast<long long*>(reinterpret_cast<Stage*>(smem) + WARPS * STAGES);
+  const uint8_t* ring = smem + warp * STAGES * STAGE;
+  Head* heads = reinterpret_cast<Head*>(smem + WARPS * STAGES * STAGE) + warp * STAGES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WARPS * STAGES * (STAGE + sizeof(Head))) + warp * STAGES;
+  long long* sh = reinterpret_cast<long long*>(smem + WARPS * STAGES * (STAGE + sizeof(Head) + 8));
   long long* upto = sh + WARPS;
+  if (lane == 0) {
+    prefetch_tensormap(&map);
+    for (int i = 0; i < STAGES; ++i) mbar_init(&bars[i], 1);
+    fence_barrier_init();
+  }
   const Cut cut = cut_batch<KEYS>(p, upto, sh);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const long long piece = (long long)blockIdx.x * WARPS + warp;
   long long x = piece * cut.piece;
   const long long x1 = p.solo ? cut.total : min(cut.total, x + cut.piece), stride = p.solo ? p.pieces : 0;
   if (x >= x1) return;
+  const uint32_t ring_a = smem_u32(ring), bars_a = smem_u32(bars);
   Feed<D> feed;
   feed.begin(p, upto, x, x1, stride);
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) feed.next(p, upto, ring + i);
+  for (int i = 0; i < STAGES - 1; ++i) feed.next(p, map, upto, ring_a + i * STAGE, heads + i, bars_a + 8 * i);
   int at = 0;                          // stage of the next step
+  uint32_t phase = 0;
   while (x < x1) {
     Part<KEYS> w;
     w.set(p, upto, x, x1);
     Tile<D, NB> t;
     load_q<D, NB>(p, w.first, w.count, w.j.head, w.end, w.new_tokens, w.j.qt, t);
     for (int st = w.from; st < w.last; ++st) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-      __syncwarp();                    // the step's codes are there for all lanes, and all are done with the step before
-      feed.next(p, upto, ring + (at + STAGES - 1) % STAGES);
-      step_tile<D, NB>(p, t, ring + at, st, w.seen, w.sure);
+      __syncwarp();                    // all lanes are done with the step before, whose stage is filled anew
+      const int ahead = (at + STAGES - 1) % STAGES;
+      feed.next(p, map, upto, ring_a + ahead * STAGE, heads + ahead, bars_a + 8 * ahead);
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars[at], phase, p.status, 401))) {
+        // Copies that do not come: give the others in flight their time, so that none writes into memory that is no longer
+        // this block's, and leave.
+        for (int i = 1; i < STAGES; ++i) {
+          const int b = (at + i) % STAGES;
+          mbar_wait(&bars[b], phase ^ (b < at ? 1u : 0u), p.status, 402);
+        }
+        return;
+      }
+      step_tile<D, NB>(p, t, ring + at * STAGE, heads + at, st, w.seen, w.sure);
       at = (at + 1) % STAGES;
+      phase ^= at == 0 ? 1u : 0u;
     }
     const bool alone = p.solo || (x == w.j.begin && w.stop == w.j.begin + w.j.cost);
     const long long slot = slot_at(piece, x == w.j.begin);
@@ -604,36 +628,35 @@ __global__ void __launch_bounds__(THREADS, 3) kv_attn_kernel(KvAttn p) {
       }
     x = stride ? x + stride : w.stop;
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Joins the job that begins in piece blockIdx.x and runs past its end.  Threads: columns of four x a share of the pieces.
+// Joins the job that begins in piece blockIdx.x and runs past its end: a warp per row, lanes over the columns (and at D = 64 over
+// halves of the pieces).
 template <int D>
-__global__ void __launch_bounds__(THREADS) kv_attn_join_kernel(KvAttn p) {
-  constexpr int KEYS = Shape<D>::KEYS, COLS = D / 4, SHARES = THREADS / COLS;
+__global__ void __launch_bounds__(THREADS) kv_attn_join_kernel(const KvAttn p) {
+  constexpr int KEYS = Shape<D>::KEYS, COLS = D / 4, SHARES = 32 / COLS;
   extern __shared__ __align__(16) uint8_t smem[];
-  float4* s_o = reinterpret_cast<float4*>(smem);                  // [SHARES][COLS]
-  float* s_l = reinterpret_cast<float*>(s_o + THREADS);           // [SHARES], and [WARPS] maxima
-  long long* sh = reinterpret_cast<long long*>(s_l + SHARES + WARPS);
+  long long* sh = reinterpret_cast<long long*>(smem);
   long long* upto = sh + WARPS;
   const Cut cut = cut_batch<KEYS>(p, upto, sh);
   const long long lo = (long long)blockIdx.x * cut.piece, hi = lo + cut.piece;
+  const bool mine = hi < cut.total;
+  Job j = {};
+  if (mine) j = job_at<KEYS>(p, upto, hi - 1);
   // every block waits, also one with nothing to join: what follows in the stream may start when this kernel is done
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (hi >= cut.total) return;
-  const Job j = job_at<KEYS>(p, upto, hi - 1);
-  if (j.begin < lo || j.begin + j.cost <= hi) return;
-  const int n = (int)((j.begin + j.cost - 1) / cut.piece - blockIdx.x) + 1;
+  if (!mine || j.begin < lo || j.begin + j.cost <= hi) return;
+  const int n = (int)(quotient(j.begin + j.cost - 1, cut.piece) - blockIdx.x) + 1;
   const int first = p.starts[j.row], count = min(p.starts[j.row + 1], p.tokens) - first;
   const int real = min(p.tile, count * p.group - j.qt * p.tile);
-  const int tid = threadIdx.x, col = tid % COLS, share = tid / COLS;
-  for (int row = 0; row < real; ++row) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = lane % COLS, share = lane / COLS;
+  for (int row = warp; row < real; row += WARPS) {
     float top = NONE;
-    for (int w = tid; w < n; w += THREADS) top = fmaxf(top, p.part_ml[(slot_at(blockIdx.x + w, w == 0) + row) * 2]);
-    top = block_max(top, s_l + SHARES);
+    for (int w = lane; w < n; w += 32) top = fmaxf(top, p.part_ml[(slot_at(blockIdx.x + w, w == 0) + row) * 2]);
+    top = warp_max(top);
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
     for (int w = share; w < n; w += SHARES) {
       const long long s = slot_at(blockIdx.x + w, w == 0) + row;
       const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + s * 2);
@@ -645,48 +668,66 @@ __global__ void __launch_bounds__(THREADS) kv_attn_join_kernel(KvAttn p) {
       o.z += v.z * f;
       o.w += v.w * f;
     }
-    s_o[tid] = o;
-    if (col == 0) s_l[share] = l;
-    __syncthreads();
-    if (share == 0) {
-#pragma unroll
-      for (int i = 1; i < SHARES; ++i) {
-        const float4 v = s_o[i * COLS + col];
-        o.x += v.x;
-        o.y += v.y;
-        o.z += v.z;
-        o.w += v.w;
-        l += s_l[i];
-      }
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      store_out<D>(p, first, j.head, j.qt * p.tile + row, col * 4, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    if (SHARES == 2) {
+      o.x += __shfl_xor_sync(0xffffffffu, o.x, 16);
+      o.y += __shfl_xor_sync(0xffffffffu, o.y, 16);
+      o.z += __shfl_xor_sync(0xffffffffu, o.z, 16);
+      o.w += __shfl_xor_sync(0xffffffffu, o.w, 16);
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
     }
-    __syncthreads();
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (share == 0) store_out<D>(p, first, j.head, j.qt * p.tile + row, col * 4, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
   }
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = nullptr;
+  if (!fn) {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult res;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &res) == cudaSuccess && res == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(sym);
+  }
+  return fn;
+}
+// The codes as [2][blocks * heads * block rows][dim bytes], boxes of 16 rows.
+int make_map(CUtensorMap* m, const KvAttn& p, int dim) {
+  EncodeFn enc = encode_fn();
+  if (!enc) return NB_ERR_NO_DRIVER_SYMBOL;
+  cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)p.kv_rows, 2}, strides[2] = {(cuuint64_t)dim, (cuuint64_t)p.kv_stride};
+  cuuint32_t box[3] = {(cuuint32_t)dim, 16, 1}, one[3] = {1, 1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(p.codes), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? NB_OK : NB_ERR_TENSORMAP;
 }
 
 template <int D, int NB>
 int launch_few(KvAttn p, cudaStream_t stream) {
-  const int scan = (WARPS + p.rows + 1) * 8, smem = WARPS * STAGES * (int)sizeof(Stage) + scan;
-  const int join_smem = THREADS * 16 + (THREADS / (D / 4) + WARPS) * 4 + scan;
+  constexpr int fixed = 1024 + WARPS * STAGES * (STAGE + (int)sizeof(Head) + 8);
+  const int scan = (WARPS + p.rows + 1) * 8;
   static bool configured[64] = {};
   int dev = 0;
   NB_CUDA(cudaGetDevice(&dev));
   if (dev >= 64) return NB_ERR_BAD_ARG;
   if (!configured[dev]) {
-    NB_CUDA(cudaFuncSetAttribute(kv_attn_kernel<D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, WARPS * STAGES * (int)sizeof(Stage) + (WARPS + 8193) * 8));
-    NB_CUDA(cudaFuncSetAttribute(kv_attn_join_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024));
+    NB_CUDA(cudaFuncSetAttribute(kv_attn_kernel<D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + (WARPS + 8193) * 8));
+    NB_CUDA(cudaFuncSetAttribute(kv_attn_join_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (WARPS + 8193) * 8));
     configured[dev] = true;
   }
+  CUtensorMap map;
+  const int rc = make_map(&map, p, D);
+  if (rc) return rc;
   p.tile = 8 * NB;
   p.solo = ((long long)p.width << p.block_log) <= SOLO * Shape<D>::KEYS;
-  kv_attn_kernel<D, NB><<<p.pieces / WARPS, THREADS, smem, stream>>>(p);
+  kv_attn_kernel<D, NB><<<p.pieces / WARPS, THREADS, fixed + scan, stream>>>(map, p);
   NB_LAUNCH_CHECK();
   if (p.solo) return NB_OK;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.pieces);
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = join_smem;
+  cfg.dynamicSmemBytes = scan;
   cfg.stream = stream;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its blocks start while the first kernel's last ones run
@@ -713,12 +754,13 @@ int nb_kv_attention(const void* q, void* out, const void* codes, const float* sc
   if ((block & (block - 1)) || block < 16 || (long long)width * block > 0x7fffffffLL || (long long)blocks * block > 0x7fffffffLL) return NB_ERR_BAD_ARG;
   if (!(softmax_scale > 0.f)) return NB_ERR_BAD_ARG;
   if ((long long)tokens * hq > 0x7fffffffLL) return NB_ERR_TOO_LARGE;
+  if ((long long)blocks * hk * block > 0x7fffffffLL - 256) return NB_ERR_TOO_LARGE;   // rows of the copies' tensor
   if (tokens == 0) return NB_OK;
   if ((reinterpret_cast<uintptr_t>(codes) & 15) || (kv_stride & 15)) return NB_ERR_UNALIGNED;
   if (!work || work_floats < nb_kv_attention_work(dim) || (reinterpret_cast<uintptr_t>(work) & 15)) return NB_ERR_BAD_ARG;
   KvAttn p{};
   p.q = q; p.out = out; p.codes = (const uint8_t*)codes; p.scale = scale; p.tables = tables; p.starts = starts; p.ends = ends;
-  p.rows = rows; p.tokens = tokens; p.hq = hq; p.hk = hk; p.group = hq / hk; p.blocks = blocks; p.width = width;
+  p.rows = rows; p.tokens = tokens; p.hq = hq; p.hk = hk; p.group = hq / hk; p.blocks = blocks; p.width = width; p.kv_rows = blocks * hk * block;
   while ((1 << p.block_log) < block) ++p.block_log;
   p.q_token = q_token; p.q_head = q_head; p.o_token = o_token; p.o_head = o_head; p.kv_stride = kv_stride; p.s_stride = s_stride;
   p.q_vec = !((reinterpret_cast<uintptr_t>(q) & 15) || (q_token & 7) || (q_head & 7));

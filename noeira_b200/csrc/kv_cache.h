@@ -41,6 +41,7 @@ struct KvAttn {
   const float* scale;                           // [2, N, H]
   const int *tables, *starts, *ends;
   int rows, tokens, hq, hk, group, block_log, blocks, width;
+  int kv_rows;                                  // blocks * hk * block
   int q_vec, o_vec;                             // 16-byte loads of q and 8-byte stores of out are aligned
   int few;                                      // rows of the batch with at most this many query rows per head are done here
   int tile;                                     // query rows of a tile
