@@ -87,17 +87,12 @@ __device__ __forceinline__ uint32_t nan_code(uint32_t w) {         // nonzero wh
 // A job is a tile of query rows and a cache head.  It costs LEAD + steps (one, where every job is one warp's).  `upto`
 // (shared memory, rows + 1): exclusive sums over the rows; `piece`: what a warp takes.
 struct Cut {
-  long long total, piece;
+  int total, piece;
 };
 struct Job {
-  int row, head, qt, cost;
-  long long begin;
+  int row, head, qt, cost, begin;
 };
 
-// a / b; batches whose sums pass 32 bits are rare, and a 64-bit division takes as long as a step
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-  return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
-}
 template <int KEYS>
 __device__ __forceinline__ int job_cost(const KvAttn& p, int i) {
   return p.solo ? 1 : LEAD + ceil_div(max(1, min(p.ends[i], p.width << p.block_log)), KEYS);
@@ -108,8 +103,9 @@ __device__ __forceinline__ int row_tiles(const KvAttn& p, int i) {
   // rows with more query rows than `few` belong to the kernel of prompts
   return n <= 0 || n * p.group > p.few ? 0 : (int)((n * p.group + p.tile - 1) / p.tile);
 }
+// A batch of 2^31 steps (8 TB of codes) is refused: reported, and nothing is done.
 template <int KEYS>
-__device__ __forceinline__ Cut cut_batch(const KvAttn& p, long long* upto, long long* sh) {
+__device__ __forceinline__ Cut cut_batch(const KvAttn& p, int* upto, long long* sh) {
   const int tid = threadIdx.x, per = ceil_div(p.rows, THREADS);
   const int lo = min(p.rows, tid * per), hi = min(p.rows, lo + per);
   long long sum = 0;
@@ -123,24 +119,30 @@ __device__ __forceinline__ Cut cut_batch(const KvAttn& p, long long* upto, long 
   }
   if (lane == 31) sh[w] = at;
   __syncthreads();
-  Cut c;
-  c.total = 0;
+  long long total = 0;
+#pragma unroll
   for (int i = 0; i < WARPS; ++i) {
     if (i < w) at += sh[i];
-    c.total += sh[i];
+    total += sh[i];
   }
-  c.piece = p.solo ? 1 : max((long long)LEAST, quotient(c.total + p.pieces - 1, p.pieces));
-  at -= sum;
+  if (total > 0x7fff0000LL) {
+    if (tid == 0 && blockIdx.x == 0) report(p.status, NB_ST_BOUNDS, 11, 0);
+    total = at = sum = 0;
+  }
+  Cut c;
+  c.total = (int)total;
+  c.piece = p.solo ? 1 : max(LEAST, (c.total + p.pieces - 1) / p.pieces);
+  int begin = (int)(at - sum);
   for (int i = lo; i < hi; ++i) {
-    upto[i] = at;
-    at += (long long)row_tiles(p, i) * p.hk * job_cost<KEYS>(p, i);
+    upto[i] = begin;
+    begin += row_tiles(p, i) * p.hk * job_cost<KEYS>(p, i);
   }
   if (tid == 0) upto[p.rows] = c.total;
   __syncthreads();
   return c;
 }
 template <int KEYS>
-__device__ __forceinline__ Job job_at(const KvAttn& p, const long long* upto, long long x) {
+__device__ __forceinline__ Job job_at(const KvAttn& p, const int* upto, int x) {
   int a = 0, b = p.rows;               // last row that begins at or before x (rows without work share their begin with the next)
   while (b - a > 1) {
     const int m = (a + b) >> 1;
@@ -149,9 +151,9 @@ __device__ __forceinline__ Job job_at(const KvAttn& p, const long long* upto, lo
   Job j;
   j.row = a;
   j.cost = job_cost<KEYS>(p, a);
-  const long long n = quotient(x - upto[a], j.cost);
-  j.qt = (int)n / p.hk;                // jobs of a row: at most tokens * heads, 31 bits
-  j.head = (int)n - j.qt * p.hk;
+  const int n = (x - upto[a]) / j.cost;
+  j.qt = n / p.hk;
+  j.head = n - j.qt * p.hk;
   j.begin = upto[a] + n * j.cost;
   return j;
 }
@@ -160,9 +162,9 @@ __device__ __forceinline__ Job job_at(const KvAttn& p, const long long* upto, lo
 template <int KEYS>
 struct Part {
   Job j;
-  long long stop;                      // where it ends, in the measure of the cut
+  int stop;                            // where it ends, in the measure of the cut
   int first, count, real, end, new_tokens, sure, seen, from, last;
-  __device__ __forceinline__ void set(const KvAttn& p, const long long* upto, long long x, long long x1) {
+  __device__ __forceinline__ void set(const KvAttn& p, const int* upto, int x, int x1) {
     j = job_at<KEYS>(p, upto, x);
     stop = min(x1, j.begin + j.cost);
     first = p.starts[j.row];
@@ -175,8 +177,8 @@ struct Part {
     sure = max(0, min(end, end - new_tokens + tok0 + 1));         // the fewest keys that a real row sees
     seen = max(0, min(end, end - new_tokens + tok1 + 1));         // the most
     const int all = ceil_div(seen, KEYS);
-    from = p.solo ? 0 : max(0, (int)(x - j.begin) - LEAD);
-    last = p.solo ? all : min(all, max(0, (int)(stop - j.begin) - LEAD));
+    from = p.solo ? 0 : max(0, x - j.begin - LEAD);
+    last = p.solo ? all : min(all, max(0, stop - j.begin - LEAD));
   }
 };
 
@@ -200,26 +202,14 @@ __device__ __forceinline__ int chunk_at(int r, int ch) {
 template <int D>
 struct Feed {                          // runs over the steps of a warp's piece, ahead of the work
   Part<Shape<D>::KEYS> part;
-  long long x, x1, stride;
+  int x, x1, stride;
   int step, page0, base;               // lane l: first row of page page0 + l among the tensor's rows, none: behind the last
   float ks, vs;                        // and its scales
-  bool more;
-  __device__ __forceinline__ void begin(const KvAttn& p, const long long* upto, long long at, long long end, long long by) {
+  __device__ __forceinline__ void begin(int at, int end, int by) {
     x = at;
     x1 = end;
     stride = by;
-    more = true;
-    open(p, upto);
-  }
-  __device__ __forceinline__ void open(const KvAttn& p, const long long* upto) {     // the next part that has steps
-    for (;;) {
-      if (x >= x1) { more = false; return; }
-      part.set(p, upto, x, x1);
-      x = stride ? x + stride : part.stop;
-      if (part.from < part.last) break;
-    }
-    step = part.from;
-    turn(p, step * Shape<D>::KEYS >> p.block_log);
+    step = part.last = 0;
   }
   __device__ __forceinline__ void turn(const KvAttn& p, int page) {                  // the next 32 pages
     page0 = page;
@@ -238,9 +228,15 @@ struct Feed {                          // runs over the steps of a warp's piece,
       }
     }
   }
-  __device__ __forceinline__ void next(const KvAttn& p, const CUtensorMap& map, const long long* upto, uint32_t stage, Head* head, uint32_t bar) {
+  __device__ __forceinline__ void next(const KvAttn& p, const CUtensorMap& map, const int* upto, uint32_t stage, Head* head, uint32_t bar) {
     constexpr int SUB = Shape<D>::SUB, KEYS = Shape<D>::KEYS;
-    if (!more) return;
+    while (step >= part.last) {        // the next part that has steps
+      if (x >= x1) return;
+      part.set(p, upto, x, x1);
+      x = stride ? x + stride : part.stop;
+      step = part.from;
+      page0 = -64;
+    }
     const int lane = threadIdx.x & 31;
     if (lane == 0) mbar_expect_tx_at(bar, STAGE);
 #pragma unroll
@@ -257,7 +253,7 @@ struct Feed {                          // runs over the steps of a warp's piece,
         copy_box(stage + 2048 + s * 1024, map, bar, row, 1);
       }
     }
-    if (++step >= part.last) open(p, upto);
+    ++step;
   }
   static __device__ __forceinline__ void mbar_expect_tx_at(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -279,57 +275,54 @@ struct Tile {                          // what a warp keeps of a tile of 8 NB qu
 };
 
 template <int D, int NB>
-__device__ __forceinline__ void load_q(const KvAttn& p, int first, int count, int head, int end, int new_tokens, int qt, Tile<D, NB>& t) {
+__device__ __forceinline__ void open_tile(const KvAttn& p, const Part<Shape<D>::KEYS>& w, Tile<D, NB>& t) {
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    const int idx = qt * p.tile + b * 8 + g, tok = idx / p.group;
-    const bool real = tok < count;
-    float x[D / 4], top = 0.f;
-    const __nv_bfloat16* q = (const __nv_bfloat16*)p.q + (long long)(first + tok) * p.q_token + (long long)(head * p.group + idx - tok * p.group) * p.q_head;
+    // 16 dimensions of each 64, of row g
+    const int idx = w.j.qt * p.tile + b * 8 + g, tok = idx / p.group;
+    const __nv_bfloat16* q = (const __nv_bfloat16*)p.q + (long long)(w.first + tok) * p.q_token + (long long)(w.j.head * p.group + idx - tok * p.group) * p.q_head + c * 16;
+    uint32_t x[D / 8];
 #pragma unroll
-    for (int u = 0; u < D / 64; ++u)
+    for (int i = 0; i < D / 8; ++i) x[i] = 0;
+    if (tok < w.count) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        const __nv_bfloat16* a = q + u * 64 + c * 16 + h * 8;
-        if (real) {
-          if (p.q_vec) {
-            w = *reinterpret_cast<const uint4*>(a);
-          } else {
-            const unsigned short* e = reinterpret_cast<const unsigned short*>(a);
-            w = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
-          }
-        }
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+      for (int u = 0; u < D / 32; ++u) {
+        const __nv_bfloat16* a = q + (u >> 1) * 64 + (u & 1) * 8;
+        if (p.q_vec) {
+          const uint4 r = *reinterpret_cast<const uint4*>(a);
+          x[4 * u] = r.x;
+          x[4 * u + 1] = r.y;
+          x[4 * u + 2] = r.z;
+          x[4 * u + 3] = r.w;
+        } else {
+          const unsigned short* e = reinterpret_cast<const unsigned short*>(a);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[u * 16 + h * 8 + 2 * i] = __uint_as_float(ww[i] << 16);
-          x[u * 16 + h * 8 + 2 * i + 1] = __uint_as_float(ww[i] & 0xffff0000u);
+          for (int i = 0; i < 4; ++i) x[4 * u + i] = e[2 * i] | (uint32_t)e[2 * i + 1] << 16;
         }
       }
+    }
+    // power of two that takes the row's largest element to [2^14, 2^15); the row's scores are scaled back by its inverse
+    float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
+    for (int i = 0; i < D / 8; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(x[i] << 16)), fabsf(__uint_as_float(x[i] & 0xffff0000u))));
     top = quad_max(top);
-    // power of two that takes the largest element to [2^14, 2^15); the row's scores are scaled back by its inverse
     int e = (int)(__float_as_uint(top) >> 23) - 127;
     e = top > 0.f && e < 128 ? max(-100, min(112, e - 14)) : 0;
     const float s = __uint_as_float((uint32_t)(127 - e) << 23);
     const float back = p.scale_log2 * __uint_as_float((uint32_t)(127 + e) << 23);
-    const int lim = real ? max(0, min(end, end - new_tokens + tok + 1)) : 0;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) t.q[b][k][h] = f16_pair(__uint_as_float(x[2 * k + h] << 16) * s, __uint_as_float(x[2 * k + h] & 0xffff0000u) * s);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      const int row = b * 8 + 2 * c + h;
       t.f[b][h] = __shfl_sync(0xffffffffu, back, (2 * c + h) * 4);
-      t.lim[b][h] = __shfl_sync(0xffffffffu, lim, (2 * c + h) * 4);
+      t.lim[b][h] = row < w.real ? max(0, min(w.end, w.end - w.new_tokens + (w.j.qt * p.tile + row) / p.group + 1)) : 0;
       t.m[b][h] = NONE;
       t.l[b][h] = 0.f;
     }
-#pragma unroll
-    for (int u = 0; u < D / 64; ++u)
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) t.q[b][u * 4 + k][h] = f16_pair(x[u * 16 + k * 4 + 2 * h] * s, x[u * 16 + k * 4 + 2 * h + 1] * s);
 #pragma unroll
     for (int j = 0; j < D / 16; ++j)
 #pragma unroll
@@ -566,7 +559,7 @@ __global__ void __launch_bounds__(THREADS, 3) kv_attn_kernel(const __grid_consta
   Head* heads = reinterpret_cast<Head*>(smem + WARPS * STAGES * STAGE) + warp * STAGES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WARPS * STAGES * (STAGE + sizeof(Head))) + warp * STAGES;
   long long* sh = reinterpret_cast<long long*>(smem + WARPS * STAGES * (STAGE + sizeof(Head) + 8));
-  long long* upto = sh + WARPS;
+  int* upto = reinterpret_cast<int*>(sh + WARPS);
   if (lane == 0) {
     prefetch_tensormap(&map);
     for (int i = 0; i < STAGES; ++i) mbar_init(&bars[i], 1);
@@ -574,14 +567,14 @@ __global__ void __launch_bounds__(THREADS, 3) kv_attn_kernel(const __grid_consta
   }
   const Cut cut = cut_batch<KEYS>(p, upto, sh);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const long long piece = (long long)blockIdx.x * WARPS + warp;
-  long long x = piece * cut.piece;
-  const long long x1 = p.solo ? cut.total : min(cut.total, x + cut.piece), stride = p.solo ? p.pieces : 0;
-  if (x >= x1) return;
+  const int piece = blockIdx.x * WARPS + warp;
+  int x = (int)min((long long)cut.total, (long long)piece * cut.piece);
+  const int x1 = p.solo ? cut.total : (int)min((long long)cut.total, (long long)x + cut.piece), stride = p.solo ? p.pieces : 0;
+  if (!p.solo && lane == 0) p.part_job[piece].w = 0;
   const uint32_t ring_a = smem_u32(ring), bars_a = smem_u32(bars);
   Feed<D> feed;
-  feed.begin(p, upto, x, x1, stride);
-#pragma unroll
+  feed.begin(x, x1, stride);
+#pragma unroll 1
   for (int i = 0; i < STAGES - 1; ++i) feed.next(p, map, upto, ring_a + i * STAGE, heads + i, bars_a + 8 * i);
   int at = 0;                          // stage of the next step
   uint32_t phase = 0;
@@ -589,7 +582,8 @@ __global__ void __launch_bounds__(THREADS, 3) kv_attn_kernel(const __grid_consta
     Part<KEYS> w;
     w.set(p, upto, x, x1);
     Tile<D, NB> t;
-    load_q<D, NB>(p, w.first, w.count, w.j.head, w.end, w.new_tokens, w.j.qt, t);
+    open_tile<D, NB>(p, w, t);
+#pragma unroll 1
     for (int st = w.from; st < w.last; ++st) {
       __syncwarp();                    // all lanes are done with the step before, whose stage is filled anew
       const int ahead = (at + STAGES - 1) % STAGES;
@@ -609,6 +603,8 @@ __global__ void __launch_bounds__(THREADS, 3) kv_attn_kernel(const __grid_consta
     }
     const bool alone = p.solo || (x == w.j.begin && w.stop == w.j.begin + w.j.cost);
     const long long slot = slot_at(piece, x == w.j.begin);
+    if (!alone && x == w.j.begin && lane == 0)   // this piece's warp of the join kernel does this job, of so many pieces
+      p.part_job[piece] = make_int4(w.first, w.j.head, w.j.qt, ((w.j.begin + w.j.cost - 1) / cut.piece - piece + 1) | w.real << 16);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -630,53 +626,49 @@ __global__ void __launch_bounds__(THREADS, 3) kv_attn_kernel(const __grid_consta
   }
 }
 
-// Joins the job that begins in piece blockIdx.x and runs past its end: a warp per row, lanes over the columns (and at D = 64 over
-// halves of the pieces).
+// Joins the jobs that begin in one piece and run past its end, as the warps of the first kernel noted them: a block for four
+// pieces, a warp per row, lanes over the columns (and at D = 64 over halves of the pieces).
 template <int D>
 __global__ void __launch_bounds__(THREADS) kv_attn_join_kernel(const KvAttn p) {
-  constexpr int KEYS = Shape<D>::KEYS, COLS = D / 4, SHARES = 32 / COLS;
-  extern __shared__ __align__(16) uint8_t smem[];
-  long long* sh = reinterpret_cast<long long*>(smem);
-  long long* upto = sh + WARPS;
-  const Cut cut = cut_batch<KEYS>(p, upto, sh);
-  const long long lo = (long long)blockIdx.x * cut.piece, hi = lo + cut.piece;
-  const bool mine = hi < cut.total;
-  Job j = {};
-  if (mine) j = job_at<KEYS>(p, upto, hi - 1);
+  constexpr int COLS = D / 4, SHARES = 32 / COLS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = lane % COLS, share = lane / COLS;
   // every block waits, also one with nothing to join: what follows in the stream may start when this kernel is done
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!mine || j.begin < lo || j.begin + j.cost <= hi) return;
-  const int n = (int)(quotient(j.begin + j.cost - 1, cut.piece) - blockIdx.x) + 1;
-  const int first = p.starts[j.row], count = min(p.starts[j.row + 1], p.tokens) - first;
-  const int real = min(p.tile, count * p.group - j.qt * p.tile);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = lane % COLS, share = lane / COLS;
-  for (int row = warp; row < real; row += WARPS) {
-    float top = NONE;
-    for (int w = lane; w < n; w += 32) top = fmaxf(top, p.part_ml[(slot_at(blockIdx.x + w, w == 0) + row) * 2]);
-    top = warp_max(top);
-    float l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int i = 0; i < WARPS; ++i) {
+    const int piece = blockIdx.x * WARPS + i;
+    const int4 job = p.part_job[piece];
+    const int n = job.w & 0xffff, real = job.w >> 16, qt = job.z;
+    if (n == 0) continue;
+#pragma unroll 1
+    for (int row = warp; row < real; row += WARPS) {
+      float top = NONE;
+      for (int w = lane; w < n; w += 32) top = fmaxf(top, p.part_ml[(slot_at(piece + w, w == 0) + row) * 2]);
+      top = warp_max(top);
+      float l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-    for (int w = share; w < n; w += SHARES) {
-      const long long s = slot_at(blockIdx.x + w, w == 0) + row;
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + s * 2);
-      const float f = ml.x == NONE ? 1.f : ex2(ml.x - top);        // without a maximum all is zero, or NaN
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + s * D + col * 4);
-      l += ml.y * f;
-      o.x += v.x * f;
-      o.y += v.y * f;
-      o.z += v.z * f;
-      o.w += v.w * f;
+      for (int w = share; w < n; w += SHARES) {
+        const long long s = slot_at(piece + w, w == 0) + row;
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + s * 2);
+        const float f = ml.x == NONE ? 1.f : ex2(ml.x - top);      // without a maximum all is zero, or NaN
+        const float4 v = *reinterpret_cast<const float4*>(p.part_o + s * D + col * 4);
+        l += ml.y * f;
+        o.x += v.x * f;
+        o.y += v.y * f;
+        o.z += v.z * f;
+        o.w += v.w * f;
+      }
+      if (SHARES == 2) {
+        o.x += __shfl_xor_sync(0xffffffffu, o.x, 16);
+        o.y += __shfl_xor_sync(0xffffffffu, o.y, 16);
+        o.z += __shfl_xor_sync(0xffffffffu, o.z, 16);
+        o.w += __shfl_xor_sync(0xffffffffu, o.w, 16);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      if (share == 0) store_out<D>(p, job.x, job.y, qt * p.tile + row, col * 4, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     }
-    if (SHARES == 2) {
-      o.x += __shfl_xor_sync(0xffffffffu, o.x, 16);
-      o.y += __shfl_xor_sync(0xffffffffu, o.y, 16);
-      o.z += __shfl_xor_sync(0xffffffffu, o.z, 16);
-      o.w += __shfl_xor_sync(0xffffffffu, o.w, 16);
-      l += __shfl_xor_sync(0xffffffffu, l, 16);
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (share == 0) store_out<D>(p, first, j.head, j.qt * p.tile + row, col * 4, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
   }
 }
 
@@ -706,14 +698,13 @@ int make_map(CUtensorMap* m, const KvAttn& p, int dim) {
 template <int D, int NB>
 int launch_few(KvAttn p, cudaStream_t stream) {
   constexpr int fixed = 1024 + WARPS * STAGES * (STAGE + (int)sizeof(Head) + 8);
-  const int scan = (WARPS + p.rows + 1) * 8;
+  const int scan = WARPS * 8 + (p.rows + 1) * 4;
   static bool configured[64] = {};
   int dev = 0;
   NB_CUDA(cudaGetDevice(&dev));
   if (dev >= 64) return NB_ERR_BAD_ARG;
   if (!configured[dev]) {
-    NB_CUDA(cudaFuncSetAttribute(kv_attn_kernel<D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + (WARPS + 8193) * 8));
-    NB_CUDA(cudaFuncSetAttribute(kv_attn_join_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (WARPS + 8193) * 8));
+    NB_CUDA(cudaFuncSetAttribute(kv_attn_kernel<D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + WARPS * 8 + 8193 * 4));
     configured[dev] = true;
   }
   CUtensorMap map;
@@ -725,9 +716,8 @@ int launch_few(KvAttn p, cudaStream_t stream) {
   NB_LAUNCH_CHECK();
   if (p.solo) return NB_OK;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.pieces);
+  cfg.gridDim = dim3(p.pieces / WARPS);
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = scan;
   cfg.stream = stream;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its blocks start while the first kernel's last ones run
@@ -744,7 +734,7 @@ extern "C" {
 
 // Pieces that the batch is cut into, and floats of work space that nb_kv_attention needs.
 int nb_kv_attention_pieces(int) { return 148 * WARPS * 3; }
-long long nb_kv_attention_work(int dim) { return (long long)nb_kv_attention_pieces(dim) * 2 * 16 * (dim + 2); }
+long long nb_kv_attention_work(int dim) { return (long long)nb_kv_attention_pieces(dim) * (2 * 16 * (dim + 2) + 4); }
 
 int nb_kv_attention(const void* q, void* out, const void* codes, const float* scale, const int* tables, const int* starts,
                     const int* ends, int rows, int tokens, int max_new, int hq, int hk, int dim, int block, int blocks, int width,
@@ -769,6 +759,7 @@ int nb_kv_attention(const void* q, void* out, const void* codes, const float* sc
   p.pieces = nb_kv_attention_pieces(dim);
   p.part_o = work;
   p.part_ml = work + (long long)p.pieces * 2 * 16 * dim;
+  p.part_job = (int4*)(p.part_ml + (long long)p.pieces * 2 * 16 * 2);
   p.few = 0x7fffffff;
   p.status = status;
   const cudaStream_t s = (cudaStream_t)stream;

@@ -1,5 +1,6 @@
 // Parameter blocks of the paged 8-bit cache kernels (kv_cache.cu) and of the attention over it (kv_attention.cu).
 #pragma once
+#include <cuda_runtime.h>
 #include <stdint.h>
 
 // status code: a row found no free block, no room in its table or none in the token buffers
@@ -49,6 +50,7 @@ struct KvAttn {
   long long q_token, q_head, o_token, o_head;
   long long kv_stride, s_stride;                // from the keys' codes / scales to the values'
   float scale_log2;
-  float *part_o, *part_ml;
+  float *part_o, *part_ml;                      // partial outputs, (maximum, sum)
+  int4* part_job;                               // of each piece: the job that it begins and does not end
   unsigned int* status;
 };
