@@ -3,10 +3,20 @@
 // value(b, v) = score_b + x_bv - log sum_u exp x_bu.  Within a beam the order of the values is the order of the logits, so
 // the candidates of a beam are found by its logits alone, exactly; only the winners of the beams are compared by value, in
 // 64 bits.  Ties go to the lowest b * vocab + v.  NaN counts as -inf, +inf as the largest finite number.
+//
+// One pass over the logits, which is all that there is to read (R * beams * vocab elements at the copy rate), split over blocks of
+// one part of one beam's row each, the elements in registers.  The block's maximum and sum come first; then the K = beams best of
+// its elements: the K-th largest of a warp's lane maxima is a lower bound of the block's K-th element, and the largest of these
+// bounds over the warps leaves few elements above it (about 2 K of 8192 in random order, and never more than K lanes' shares per
+// warp), which are ranked by counting.  A second kernel, a block per request, joins the parts of each beam and ranks the beams.
 #include "common.cuh"
 
 namespace {
 using namespace nb;
+
+constexpr int THREADS = 256;
+constexpr float TOP = 3.4028235e38f;
+typedef unsigned long long Key;              // order of the value above, inverse index below: larger is better, all distinct
 
 struct BeamSel {
   const void* logits;
@@ -15,93 +25,263 @@ struct BeamSel {
   float* scores_out;
   int *parents, *tokens;
   unsigned char* done;
-  int requests, beams, vocab, eos, fp32;
+  int requests, beams, vocab, eos, parts;
   long long pitch;                 // elements between beams' rows
+  float2* part_ms;                 // [R * beams, parts] maximum, sum of exponentials
+  Key* part_key;                   // [R * beams, parts, beams] best first
 };
 
-__device__ __forceinline__ float logit(const BeamSel& p, long long row, int v) {
-  float x = p.fp32 ? ((const float*)p.logits)[row * p.pitch + v] : __bfloat162float(((const __nv_bfloat16*)p.logits)[row * p.pitch + v]);
-  return x != x ? -INFINITY : fminf(x, 3.4028235e38f);
+__device__ __forceinline__ Key key_of(float x, int v) {
+  uint32_t u = __float_as_uint(x + 0.f);             // -0 and 0 are the same value
+  u ^= (uint32_t)((int)u >> 31) | 0x80000000u;
+  return (Key)u << 32 | (uint32_t)~v;
+}
+__device__ __forceinline__ float value_of(Key k) {
+  uint32_t u = (uint32_t)(k >> 32);
+  u ^= (u >> 31) ? 0x80000000u : 0xffffffffu;
+  return __uint_as_float(u);
+}
+__device__ __forceinline__ float fit(float x) { return x != x ? -INFINITY : fminf(x, TOP); }
+
+// Largest of the warp's keys; all lanes get it.
+__device__ __forceinline__ Key warp_best(Key k) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+  return (Key)hi << 32 | lo;
 }
 
-// One block per request: log-sum-exp of each beam, then `beams` rounds of a maximum over what has not been taken.
-__global__ void __launch_bounds__(1024) beam_select_kernel(BeamSel p) {
+template <bool FP32, int EACH, bool WIDE>
+__global__ void __launch_bounds__(THREADS) beam_part_kernel(const BeamSel p) {
+  constexpr int VEC = WIDE ? (FP32 ? 4 : 8) : 1, SIZE = FP32 ? 4 : 2;   // neighbouring elements of a thread, bytes of an element
   __shared__ float sh[32];
-  __shared__ double top[32], lsum[32];   // maximum and log of the sum of each beam; together they would lose the sum beside a huge maximum
-  __shared__ double bv[32];
-  __shared__ long long bi[32];
-  __shared__ double last_v;
-  __shared__ long long last_i;
-  const int r = blockIdx.x, tid = threadIdx.x;
-  for (int b = 0; b < p.beams; ++b) {
-    const long long row = (long long)r * p.beams + b;
-    float m = -INFINITY;
-    for (int v = tid; v < p.vocab; v += 1024) m = fmaxf(m, logit(p, row, v));
-    m = block_max(m, sh);
-    if (m == -INFINITY) m = 0.f;
-    float s = 0.f;
-    for (int v = tid; v < p.vocab; v += 1024) s += expf(logit(p, row, v) - m);
-    s = block_sum(s, sh);
-    if (tid == 0) {
-      top[b] = (double)m;
-      lsum[b] = log((double)s);
-    }
-  }
-  if (tid == 0) { last_v = INFINITY; last_i = -1; }
-  __syncthreads();
-  for (int k = 0; k < p.beams; ++k) {
-    double best = -INFINITY;
-    long long at = 0x7fffffffffffffffLL;
-    const double lv = last_v;
-    const long long li = last_i;
-    for (int b = 0; b < p.beams; ++b) {
-      const long long row = (long long)r * p.beams + b;
-      const bool fin = p.finished && p.finished[row];
-      const float s0 = p.scores[row];
-      const double sc = s0 != s0 ? -INFINITY : (double)s0;
-      for (int v = tid; v < p.vocab; v += 1024) {
-        const long long i = (long long)b * p.vocab + v;
-        double val = -INFINITY;
-        if (fin) {
-          if (v == p.eos) val = sc;
+  __shared__ Key bound_sh[THREADS / 32];
+  __shared__ int found;
+  extern __shared__ Key cand[];                      // the elements above the bound
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.beams;
+  const long long row = blockIdx.x / p.parts;
+  const int part = blockIdx.x - (int)row * p.parts;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (p.finished && p.finished[row]) return;         // its one continuation is known
+  // Where every row begins on a 16-byte boundary a thread reads 16 bytes at a time, else neighbouring threads read neighbouring
+  // elements.  One or the other for all rows of a call: beams with equal logits then have equal sums, and their ties are ties.
+  const char* base = (const char*)p.logits + row * p.pitch * SIZE;
+  const int first = part * THREADS * EACH + tid * VEC;
+  float x[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH / VEC; ++i) {
+    const int v0 = first + i * THREADS * VEC;
+    if (WIDE && v0 + VEC <= p.vocab) {
+      const uint4 w = __ldcs(reinterpret_cast<const uint4*>(base + (long long)v0 * SIZE));
+      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (FP32) {
+          x[i * VEC + e % VEC] = __uint_as_float(ww[e]);
         } else {
-          const float x = logit(p, row, v);
-          if (x > -INFINITY && sc > -INFINITY) val = sc + ((double)x - top[b] - lsum[b]);
+          x[i * VEC + (2 * e) % VEC] = __uint_as_float(ww[e] << 16);
+          x[i * VEC + (2 * e + 1) % VEC] = __uint_as_float(ww[e] & 0xffff0000u);
         }
-        if ((val < lv || (val == lv && i > li)) && (val > best || (val == best && i < at))) { best = val; at = i; }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int v = v0 + e;
+        x[i * VEC + e] = v >= p.vocab ? -INFINITY : FP32 ? __ldcs((const float*)base + v) : __bfloat162float(__ldcs((const __nv_bfloat16*)base + v));
       }
     }
+  }
+  Key mine = 0;                                      // this thread's best; 0: it has no element
+  float m = -INFINITY;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double ov = __shfl_xor_sync(0xffffffffu, best, o);
-      const long long oi = __shfl_xor_sync(0xffffffffu, at, o);
-      if (ov > best || (ov == best && oi < at)) { best = ov; at = oi; }
+  for (int i = 0; i < EACH; ++i) {
+    x[i] = x[i] != x[i] ? -INFINITY : fminf(x[i], TOP);
+    const int v = first + (i / VEC) * THREADS * VEC + i % VEC;
+    if ((x[i] > m || mine == 0) && v < p.vocab) {
+      m = x[i];
+      mine = key_of(x[i], v);
     }
-    if ((tid & 31) == 0) { bv[tid >> 5] = best; bi[tid >> 5] = at; }
-    __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < 32; ++w)
-        if (bv[w] > best || (bv[w] == best && bi[w] < at)) { best = bv[w]; at = bi[w]; }
-      last_v = best;
-      last_i = at;
-      const long long o = (long long)r * p.beams + k;
-      const int b = (int)(at / p.vocab), v = (int)(at % p.vocab);
-      p.scores_out[o] = (float)best;
+  }
+  if (tid == 0) found = 0;
+  const float top = block_max(m, sh);                // its barriers publish `found` too
+  const float from = top == -INFINITY ? 0.f : top;
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const float d = x[i] - from;
+    s += exp2f(fmaf(d, 1.44269502f, d * 1.92596303e-8f));   // log2(e) in two parts: the first alone is off by 2^-26, always the same way
+  }
+  Key left = mine, bound = 0;
+  for (int k = 0; k < K; ++k) {
+    bound = warp_best(left);
+    if (left == bound) left = 0;
+  }
+  if (lane == 0) bound_sh[warp] = bound;
+  s = block_sum(s, sh);                              // publishes the bounds
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) bound = max(bound, bound_sh[w]);
+  if (mine >= bound && mine != 0) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int v = first + (i / VEC) * THREADS * VEC + i % VEC;
+      const Key k = key_of(x[i], v);
+      if (k >= bound && v < p.vocab) cand[atomicAdd(&found, 1)] = k;
+    }
+  }
+  __syncthreads();
+  const long long at = row * p.parts + part;
+  if (tid == 0) p.part_ms[at] = make_float2(top, s);
+  const int n = found;
+  for (int i = tid; i < n; i += THREADS) {
+    const Key k = cand[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += cand[j] > k;
+    if (rank < K) p.part_key[at * K + rank] = k;
+  }
+  for (int i = n + tid; i < K; i += THREADS) p.part_key[at * K + i] = 0;   // a part of fewer elements
+}
+
+// Joins the parts of a request: the K best and the log-sum-exp of each beam, a warp per beam; then the ranks of beams x K.
+__global__ void __launch_bounds__(THREADS) beam_join_kernel(const BeamSel p) {
+  __shared__ unsigned long long val[32 * 32];        // order of the value as an unsigned number; 0: no candidate
+  __shared__ long long idx[32 * 32];                 // b * vocab + v
+  const int r = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, K = p.beams;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int b = warp; b < K; b += THREADS / 32) {
+    const long long row = (long long)r * K + b;
+    const float s0 = p.scores[row];
+    const double score = s0 != s0 ? -INFINITY : (double)s0;
+    long long at = 0x7fffffffffffffffLL;
+    double v = -INFINITY;
+    if (p.finished && p.finished[row]) {
+      // eos at the beam's score; behind it, in order, what it does not continue with
+      const int t = lane == 0 ? p.eos : lane - 1 + (lane - 1 >= p.eos);
+      if (t < p.vocab) at = (long long)b * p.vocab + t;
+      if (lane == 0) v = score;
+    } else {
+      float top = -INFINITY;
+      for (int i = lane; i < p.parts; i += 32) top = fmaxf(top, p.part_ms[row * p.parts + i].x);
+      top = warp_max(top);
+      const float from = top == -INFINITY ? 0.f : top;
+      double s = 0.0;
+      for (int i = lane; i < p.parts; i += 32) {
+        const float2 ms = p.part_ms[row * p.parts + i];
+        if (ms.x > -INFINITY) s += (double)ms.y * (double)expf(ms.x - from);   // of weight one at the largest
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      const double lsum = log(s);
+      // K rounds of the largest key below the last one; each lane looks through its own
+      const int m = p.parts * K;
+      const Key* keys = p.part_key + row * m;
+      constexpr int HELD = 8;                        // in registers, more are read again
+      Key held[HELD];
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) held[i] = lane + 32 * i < m ? keys[lane + 32 * i] : 0;
+      Key last = ~0ULL;
+      for (int k = 0; k < K; ++k) {
+        Key best = 0;
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) best = held[i] < last && held[i] > best ? held[i] : best;
+        for (int i = lane + 32 * HELD; i < m; i += 32) {
+          const Key y = keys[i];
+          best = y < last && y > best ? y : best;
+        }
+        last = warp_best(best);
+        if (lane == k && last) {
+          const float x = value_of(last);
+          at = (long long)b * p.vocab + (int)~(uint32_t)last;
+          if (x > -INFINITY && score > -INFINITY) v = score + ((double)x - (double)from - lsum);
+        }
+        if (last == 0) break;                        // fewer tokens than beams
+      }
+    }
+    if (lane < K) {
+      unsigned long long u = __double_as_longlong(v + 0.0);
+      u ^= (unsigned long long)((long long)u >> 63) | 0x8000000000000000ULL;
+      val[b * K + lane] = at == 0x7fffffffffffffffLL ? 0 : u;
+      idx[b * K + lane] = at;
+    }
+  }
+  __syncthreads();
+  const int n = K * K;
+  for (int i = tid; i < n; i += THREADS) {
+    const unsigned long long u = val[i];
+    const long long at = idx[i];
+    if (u == 0) continue;
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += val[j] > u || (val[j] == u && idx[j] < at);
+    if (rank < K) {
+      const long long o = (long long)r * K + rank;
+      const int b = (int)(at / p.vocab), v = (int)(at - (long long)b * p.vocab);
+      p.scores_out[o] = (float)__longlong_as_double((long long)(u ^ ((u >> 63) ? 0x8000000000000000ULL : ~0ULL)));
       p.parents[o] = b;
       p.tokens[o] = v;
-      p.done[o] = p.eos >= 0 && ((p.finished && p.finished[(long long)r * p.beams + b]) || v == p.eos);
+      p.done[o] = p.eos >= 0 && ((p.finished && p.finished[(long long)r * K + b]) || v == p.eos);
     }
-    __syncthreads();
   }
 }
 
-}  // namespace
-
-extern "C" int nb_beam_select(const void* logits, const float* scores, const unsigned char* finished, float* scores_out, int* parents, int* tokens,
-                              unsigned char* done, int requests, int beams, int vocab, int eos, int fp32, long long pitch, void* stream) {
-  if (requests <= 0 || beams <= 0 || beams > 32 || vocab <= 0 || eos >= vocab || pitch < vocab || (finished && eos < 0)) return NB_ERR_BAD_ARG;
-  BeamSel p{logits, scores, finished, scores_out, parents, tokens, done, requests, beams, vocab, eos, fp32, pitch};
-  beam_select_kernel<<<requests, 1024, 0, (cudaStream_t)stream>>>(p);
+template <bool FP32, int EACH, bool WIDE>
+int launch_parts(const BeamSel& p, cudaStream_t s) {
+  const int smem = THREADS / 32 * p.beams * EACH * 8;
+  if (smem > 48 * 1024) {
+    static bool configured[64] = {};
+    int dev = 0;
+    NB_CUDA(cudaGetDevice(&dev));
+    if (dev >= 64) return NB_ERR_BAD_ARG;
+    if (!configured[dev]) {
+      NB_CUDA(cudaFuncSetAttribute(beam_part_kernel<FP32, EACH, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, THREADS * EACH * 8));
+      configured[dev] = true;
+    }
+  }
+  beam_part_kernel<FP32, EACH, WIDE><<<(unsigned)(p.requests * p.beams * p.parts), THREADS, smem, s>>>(p);
   NB_LAUNCH_CHECK();
   return NB_OK;
 }
+
+// Elements of a thread: long parts read with more loads in flight and leave less to join; short ones spread few rows over the GPU.
+int elements_each(long long rows, int vocab) { return rows * ceil_div(vocab, THREADS * 32) >= 148 ? 32 : 8; }
+
+}  // namespace
+
+extern "C" {
+
+// Bytes of work space that nb_beam_select needs.
+long long nb_beam_select_work(int requests, int beams, int vocab) {
+  const long long rows = (long long)requests * beams, parts = ceil_div(vocab, THREADS * elements_each(rows, vocab));
+  return rows * parts * (8 + 8LL * beams);
+}
+
+int nb_beam_select(const void* logits, const float* scores, const unsigned char* finished, float* scores_out, int* parents, int* tokens,
+                   unsigned char* done, int requests, int beams, int vocab, int eos, int fp32, long long pitch, void* work, long long work_bytes, void* stream) {
+  if (requests <= 0 || beams <= 0 || beams > 32 || vocab <= 0 || vocab > 0x7fffff00 || eos >= vocab || pitch < vocab || (finished && eos < 0)) return NB_ERR_BAD_ARG;
+  if (reinterpret_cast<uintptr_t>(logits) & (fp32 ? 3 : 1)) return NB_ERR_UNALIGNED;
+  const long long rows = (long long)requests * beams;
+  if (!work || work_bytes < nb_beam_select_work(requests, beams, vocab) || (reinterpret_cast<uintptr_t>(work) & 15)) return NB_ERR_BAD_ARG;
+  const int each = elements_each(rows, vocab), parts = ceil_div(vocab, THREADS * each);
+  if (rows * parts > 0x7fffffffLL) return NB_ERR_TOO_LARGE;
+  BeamSel p{logits, scores, finished, scores_out, parents, tokens, done, requests, beams, vocab, eos, parts, pitch, nullptr, nullptr};
+  p.part_key = (Key*)work;
+  p.part_ms = (float2*)(p.part_key + rows * parts * beams);
+  const cudaStream_t s = (cudaStream_t)stream;
+  int rc;
+  const bool wide = !(reinterpret_cast<uintptr_t>(logits) & 15) && (rows == 1 || !(pitch & (fp32 ? 3 : 7)));
+  if (fp32 && wide) rc = each == 32 ? launch_parts<true, 32, true>(p, s) : launch_parts<true, 8, true>(p, s);
+  else if (fp32) rc = each == 32 ? launch_parts<true, 32, false>(p, s) : launch_parts<true, 8, false>(p, s);
+  else if (wide) rc = each == 32 ? launch_parts<false, 32, true>(p, s) : launch_parts<false, 8, true>(p, s);
+  else rc = each == 32 ? launch_parts<false, 32, false>(p, s) : launch_parts<false, 8, false>(p, s);
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(requests);
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = s;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its blocks start while the first kernel's last ones run
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  NB_CUDA(cudaLaunchKernelEx(&cfg, beam_join_kernel, p));
+  return NB_OK;
+}
+
+}  // extern "C"

@@ -2,6 +2,8 @@
 (csrc/kv_cache.cu); CPU tensors take the same definitions in PyTorch."""
 from __future__ import annotations
 
+import ctypes
+import functools
 import math
 
 import torch
@@ -30,7 +32,7 @@ def beam_select(logits, scores, finished=None, eos=None):
         raise ValueError(f"logits: [requests, beams, vocab], got {tuple(shape)}")
     requests, beams, vocab = shape
     dev = logits.get_device()
-    if beams > MAX_BEAMS or requests * beams >= 1 << 31 or vocab >= 1 << 31:
+    if beams > MAX_BEAMS or requests * beams >= 1 << 31 or vocab >= 0x7fffff00:
         raise ValueError(f"beam_select: at most {MAX_BEAMS} beams, got {tuple(shape)}")
     if scores.dtype is not torch.float32 or scores.shape != shape[:2] or not scores.is_contiguous() or scores.get_device() != dev:
         raise ValueError(f"scores: contiguous float32 {(requests, beams)}, got {scores.dtype} {tuple(scores.shape)}")
@@ -57,11 +59,20 @@ def beam_select(logits, scores, finished=None, eos=None):
             return beam_select(logits, scores, finished, eos)
     out = torch.empty((3, requests, beams), dtype=torch.int32, device=logits.device)
     done = torch.empty((requests, beams), dtype=torch.bool, device=logits.device)
+    nbytes = _work_bytes(requests, beams, vocab)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)      # of this call alone
     new_scores, parents, tokens = out.unbind(0)
     at, step = out.data_ptr(), 4 * requests * beams
     check(cuda_lib().nb_beam_select(logits.data_ptr(), scores.data_ptr(), None if finished is None else finished.data_ptr(), at, at + step, at + 2 * step, done.data_ptr(),
-                                    requests, beams, vocab, -1 if eos is None else eos, int(fp32), pitch, raw_stream()), "beam_select")
+                                    requests, beams, vocab, -1 if eos is None else eos, int(fp32), pitch, work.data_ptr(), nbytes, raw_stream()), "beam_select")
     return new_scores.view(torch.float32), parents, tokens, done
+
+
+@functools.lru_cache(maxsize=256)
+def _work_bytes(requests, beams, vocab):
+    fn = cuda_lib().nb_beam_select_work
+    fn.restype = ctypes.c_longlong
+    return int(fn(ctypes.c_int(requests), ctypes.c_int(beams), ctypes.c_int(vocab)))
 
 
 def _select_cpu(logits, scores, finished, eos):
