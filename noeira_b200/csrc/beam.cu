@@ -43,6 +43,11 @@ __device__ __forceinline__ float value_of(Key k) {
 }
 __device__ __forceinline__ float fit(float x) { return x != x ? -INFINITY : fminf(x, TOP); }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // Largest of the warp's keys; all lanes get it.
 __device__ __forceinline__ Key warp_best(Key k) {
   const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
@@ -67,40 +72,46 @@ __global__ void __launch_bounds__(THREADS) beam_part_kernel(const BeamSel p) {
   const char* base = (const char*)p.logits + row * p.pitch * SIZE;
   const int first = part * THREADS * EACH + tid * VEC;
   float x[EACH];
+  if ((part + 1) * THREADS * EACH <= p.vocab) {      // all loads at once, none behind a condition
 #pragma unroll
-  for (int i = 0; i < EACH / VEC; ++i) {
-    const int v0 = first + i * THREADS * VEC;
-    if (WIDE && v0 + VEC <= p.vocab) {
-      const uint4 w = __ldcs(reinterpret_cast<const uint4*>(base + (long long)v0 * SIZE));
-      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+    for (int i = 0; i < EACH / VEC; ++i) {
+      const int v = first + i * THREADS * VEC;
+      if (WIDE) {
+        const uint4 w = __ldcs(reinterpret_cast<const uint4*>(base + (long long)v * SIZE));
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (FP32) {
-          x[i * VEC + e % VEC] = __uint_as_float(ww[e]);
-        } else {
-          x[i * VEC + (2 * e) % VEC] = __uint_as_float(ww[e] << 16);
-          x[i * VEC + (2 * e + 1) % VEC] = __uint_as_float(ww[e] & 0xffff0000u);
+        for (int e = 0; e < 4; ++e) {
+          if (FP32) {
+            x[i * VEC + e % VEC] = __uint_as_float(ww[e]);
+          } else {
+            x[i * VEC + (2 * e) % VEC] = __uint_as_float(ww[e] << 16);
+            x[i * VEC + (2 * e + 1) % VEC] = __uint_as_float(ww[e] & 0xffff0000u);
+          }
         }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const int v = v0 + e;
-        x[i * VEC + e] = v >= p.vocab ? -INFINITY : FP32 ? __ldcs((const float*)base + v) : __bfloat162float(__ldcs((const __nv_bfloat16*)base + v));
+      } else {
+        x[i] = FP32 ? __ldcs((const float*)base + v) : __bfloat162float(__ldcs((const __nv_bfloat16*)base + v));
       }
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int v = first + (i / VEC) * THREADS * VEC + i % VEC, at = min(v, p.vocab - 1);
+      x[i] = FP32 ? ((const float*)base)[at] : __bfloat162float(((const __nv_bfloat16*)base)[at]);
+      if (v >= p.vocab) x[i] = -INFINITY;
+    }
   }
-  Key mine = 0;                                      // this thread's best; 0: it has no element
   float m = -INFINITY;
+  int best = 0;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    x[i] = x[i] != x[i] ? -INFINITY : fminf(x[i], TOP);
-    const int v = first + (i / VEC) * THREADS * VEC + i % VEC;
-    if ((x[i] > m || mine == 0) && v < p.vocab) {
+    x[i] = fminf(fmaxf(x[i], -INFINITY), TOP);       // the maximum of NaN and -inf is -inf
+    if (x[i] > m) {
       m = x[i];
-      mine = key_of(x[i], v);
+      best = i;
     }
   }
+  const int at_best = first + (best / VEC) * THREADS * VEC + best % VEC;
+  const Key mine = at_best < p.vocab ? key_of(m, at_best) : 0;   // this thread's best; 0: it has no element
   if (tid == 0) found = 0;
   const float top = block_max(m, sh);                // its barriers publish `found` too
   const float from = top == -INFINITY ? 0.f : top;
@@ -108,7 +119,7 @@ __global__ void __launch_bounds__(THREADS) beam_part_kernel(const BeamSel p) {
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const float d = x[i] - from;
-    s += exp2f(fmaf(d, 1.44269502f, d * 1.92596303e-8f));   // log2(e) in two parts: the first alone is off by 2^-26, always the same way
+    s += ex2(fmaf(d, 1.44269502f, d * 1.92596303e-8f));     // log2(e) in two parts: the first alone is off by 2^-26, always the same way
   }
   Key left = mine, bound = 0;
   for (int k = 0; k < K; ++k) {
@@ -120,11 +131,14 @@ __global__ void __launch_bounds__(THREADS) beam_part_kernel(const BeamSel p) {
 #pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) bound = max(bound, bound_sh[w]);
   if (mine >= bound && mine != 0) {
+    const float least = bound ? value_of(bound) : -INFINITY;   // 0: a block of fewer elements than K
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-      const int v = first + (i / VEC) * THREADS * VEC + i % VEC;
-      const Key k = key_of(x[i], v);
-      if (k >= bound && v < p.vocab) cand[atomicAdd(&found, 1)] = k;
+      if (x[i] >= least) {
+        const int v = first + (i / VEC) * THREADS * VEC + i % VEC;
+        const Key k = key_of(x[i], v);
+        if (k >= bound && v < p.vocab) cand[atomicAdd(&found, 1)] = k;
+      }
     }
   }
   __syncthreads();
