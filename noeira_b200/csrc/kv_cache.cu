@@ -61,6 +61,7 @@ __global__ void __launch_bounds__(256) kv_plan_kernel(KvPlan p) {
   extern __shared__ int sm[];
   int* s_start = sm;                 // [rows + 1]
   int* s_off = sm + p.rows + 1;      // [rows] first block of the row among the new ones, -1: refused
+  int* s_len = s_off + p.rows;       // [rows]
   __shared__ long long sh[8];
   const int tid = threadIdx.x, per = ceil_div(p.rows, 256);
   const int lo = min(p.rows, tid * per), hi = min(p.rows, lo + per);
@@ -73,9 +74,10 @@ __global__ void __launch_bounds__(256) kv_plan_kernel(KvPlan p) {
   for (int i = lo; i < hi; ++i) {
     const int len = p.lengths[i], add = max(0, p.new_lens[i]);
     s_start[i] = (int)min(at, 0x7fffffffLL);
+    s_len[i] = len;
     at += add;
-    const bool fits = len >= 0 && p.new_lens[i] >= 0 && (long long)len + add <= (long long)p.width * p.block && at <= p.tokens;
-    s_off[i] = fits ? ceil_div(len + add, p.block) - ceil_div(len, p.block) : -1;
+    const bool fits = len >= 0 && p.new_lens[i] >= 0 && (long long)len + add <= ((long long)p.width << p.block_log) && at <= p.tokens;
+    s_off[i] = fits ? ((len + add + (1 << p.block_log) - 1) >> p.block_log) - ((len + (1 << p.block_log) - 1) >> p.block_log) : -1;
     sum += max(0, s_off[i]);
   }
   long long off = block_scan(sum, sh, total) - sum, taken = 0;
@@ -102,34 +104,48 @@ __global__ void __launch_bounds__(256) kv_plan_kernel(KvPlan p) {
       *p.free_count_out = free_count - (int)taken;
     }
   }
-  for (long long t = (long long)blockIdx.x * 256 + tid; t < p.tokens; t += (long long)gridDim.x * 256) {
-    if (t >= s_start[p.rows]) {
-      p.slots[t] = -1;
-      p.positions[t] = 0;
-      p.row_of[t] = -1;
-      continue;
-    }
-    int a = 0, b = p.rows;             // last row with start <= t
+  // four neighbouring tokens a thread: one search, one look into the table per page, 16-byte stores
+  for (long long t0 = ((long long)blockIdx.x * 256 + tid) * 4; t0 < p.tokens; t0 += (long long)gridDim.x * 1024) {
+    int a = 0, b = p.rows;             // last row with start <= t0
     while (b - a > 1) {
       const int m = (a + b) >> 1;
-      if (s_start[m] <= (int)t) a = m; else b = m;
+      if (s_start[m] <= (int)t0) a = m; else b = m;
     }
-    const int len = p.lengths[a], pos = len + (int)t - s_start[a], pg = pos / p.block, in = pos - pg * p.block;
-    int slot = -1;
-    if (s_off[a] >= 0) {
-      const int have = ceil_div(len, p.block);
-      int id;
-      if (pg < have) {
-        id = p.tables[(long long)a * p.width + pg];
-      } else {
-        id = p.free_ids[free_count - 1 - (s_off[a] + pg - have)];
-        if (in == 0) p.tables[(long long)a * p.width + pg] = id;
+    int slot[4], pos[4], row[4], page = -1, id = -1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int t = (int)t0 + e;       // may pass the last token by three: below 2^31 by the launcher's limit
+      while (a + 1 < p.rows && s_start[a + 1] <= t) {
+        ++a;
+        page = -1;
       }
-      if (id >= 0) slot = id * p.block + in;
+      const bool real = t < s_start[p.rows] && t < p.tokens;
+      const int len = s_len[a], at_pos = len + t - s_start[a];
+      slot[e] = -1;
+      pos[e] = real ? at_pos : 0;
+      row[e] = real ? a : -1;
+      if (real && s_off[a] >= 0) {
+        const int pg = at_pos >> p.block_log, in = at_pos - (pg << p.block_log);
+        if (pg != page) {
+          const int have = (int)(((long long)len + (1 << p.block_log) - 1) >> p.block_log);
+          id = pg < have ? p.tables[(long long)a * p.width + pg] : p.free_ids[free_count - 1 - (s_off[a] + pg - have)];
+          page = pg;
+        }
+        if (in == 0) p.tables[(long long)a * p.width + pg] = id;   // the first token of a block: the block is new
+        if (id >= 0) slot[e] = (id << p.block_log) + in;
+      }
     }
-    p.slots[t] = slot;
-    p.positions[t] = pos;
-    p.row_of[t] = a;
+    if (p.vec && t0 + 4 <= p.tokens) {
+      *reinterpret_cast<int4*>(p.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+      *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+      *reinterpret_cast<int4*>(p.row_of + t0) = make_int4(row[0], row[1], row[2], row[3]);
+    } else {
+      for (int e = 0; e < 4 && t0 + e < p.tokens; ++e) {
+        p.slots[t0 + e] = slot[e];
+        p.positions[t0 + e] = pos[e];
+        p.row_of[t0 + e] = row[e];
+      }
+    }
   }
 }
 
@@ -154,53 +170,123 @@ __device__ __forceinline__ long long valid_from(const KvAppend& p, long long t) 
   return p.tokens;
 }
 
-// One warp per (token, head, K or V).  A run is a stretch of neighbouring tokens and slots inside one block; the warp of a
-// run's first token does the run, and what continues it in the same block behind skipped tokens.
-__global__ void __launch_bounds__(128) kv_append_kernel(KvAppend p) {
-  const int lane = threadIdx.x & 31;
-  long long t0 = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (t0 >= p.tokens) return;
-  const int h = blockIdx.y % p.heads, which = blockIdx.y / p.heads;
-  int slot = p.slots[t0];
-  if ((unsigned)slot >= (unsigned)p.limit) return;
-  const int id = slot / p.block;
-  int off = slot - id * p.block;
-  if (off > 0) {
-    const long long before = valid_before(p, t0);
-    if (before >= 0 && p.slots[before] == slot - 1) return;
-  }
+// Eight bf16 of a token, as raw words.
+__device__ __forceinline__ uint4 eight(const __nv_bfloat16* x, int vec) {
+  if (vec) return *reinterpret_cast<const uint4*>(x);
+  const unsigned short* e = reinterpret_cast<const unsigned short*>(x);
+  return make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
+}
+// Magnitudes (bf16 pairs) with what is not finite as zero.
+__device__ __forceinline__ uint32_t finite_abs(uint32_t w) {
+  const uint32_t v = w & 0x7fff7fffu;
+  return v & ~__vcmpgeu2(v, 0x7f807f80u);
+}
+__device__ __forceinline__ uint32_t abs_max(uint32_t m, const uint4& w) {
+  return __vmaxu2(m, __vmaxu2(__vmaxu2(finite_abs(w.x), finite_abs(w.y)), __vmaxu2(finite_abs(w.z), finite_abs(w.w))));
+}
+__device__ __forceinline__ uint32_t codes4(uint32_t a, uint32_t b, float inv) {
+  const float x0 = __uint_as_float(a << 16) * inv, x1 = __uint_as_float(a & 0xffff0000u) * inv;
+  const float x2 = __uint_as_float(b << 16) * inv, x3 = __uint_as_float(b & 0xffff0000u) * inv;
+  uint32_t r = e4m3x2(x0, x1) | e4m3x2(x2, x3) << 16;
+  if ((((a & 0x7fff7fffu) + 0x00800080u) | ((b & 0x7fff7fffu) + 0x00800080u)) & 0x80008000u)   // an exponent of all ones
+    r = code_of(x0) | code_of(x1) << 8 | code_of(x2) << 16 | code_of(x3) << 24;
+  return r;
+}
+
+// A run is a stretch of neighbouring tokens and slots inside one block.  A warp takes the runs that begin in a window of `window`
+// tokens, for one head of K or V: D / 8 lanes a token, 16 bytes each, so that a run of up to 32 tokens is read once and stays in
+// registers between the maximum and the codes (longer ones are read again, from the caches).  What continues a run in the same
+// block behind skipped tokens is done by the same warp.  One pass over the input at the copy rate is the bound; windows of one
+// token spread a decode step over the GPU, windows of 32 keep warps with nothing to do few.
+template <int D>
+__global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p) {
+  constexpr int LANES = D / 8, TOKENS = 32 / LANES, HELD = 32 / TOKENS;
+  const int lane = threadIdx.x & 31, sub = lane / LANES, d = lane % LANES * 8;
+  const long long w0 = ((long long)blockIdx.x * 4 + (threadIdx.x >> 5)) * p.window;
+  if (w0 >= p.tokens) return;
+  const int h = blockIdx.y % p.heads, which = blockIdx.y / p.heads, vec = which ? p.v_vec : p.k_vec;
   const long long step = which ? p.v_token : p.k_token;
-  const long long bh = ((long long)which * p.blocks + id) * p.heads + h;
-  uint8_t* codes = p.codes + (long long)which * p.kv_stride + ((long long)id * p.heads + h) * p.block * p.dim;
-  float old = off > 0 ? p.scale[bh] : 0.f;
-  for (;;) {
-    const __nv_bfloat16* x = (const __nv_bfloat16*)(which ? p.v : p.k) + t0 * step + (long long)h * (which ? p.v_head : p.k_head);
-    int n = 1;
-    while (off + n < p.block && t0 + n < p.tokens && p.slots[t0 + n] == slot + n) ++n;
-    float amax = 0.f;
-    for (int i = 0; i < n; ++i)
-      for (int d = lane; d < p.dim; d += 32) {
-        const float v = fabsf(__bfloat162float(x[i * step + d]));
-        if (v <= 3.4028235e38f) amax = fmaxf(amax, v);
-      }
-    amax = warp_max(amax);
-    const float now = fmaxf(old, scale_for(amax));
-    if (off > 0 && now != old) {
-      const float r = old * inv_pow2(now);
-      for (int i = lane; i < off * p.dim; i += 32) codes[i] = (uint8_t)code_of(value_of(codes[i]) * r);
-    }
-    const float inv = inv_pow2(now);
-    for (int i = 0; i < n; ++i)
-      for (int d = lane; d < p.dim; d += 32) codes[(off + i) * p.dim + d] = (uint8_t)code_of(__bfloat162float(x[i * step + d]) * inv);
-    __syncwarp();
-    old = now;
-    off += n;
-    slot += n;
-    if (off == p.block) break;
-    t0 = valid_from(p, t0 + n);
-    if (t0 >= p.tokens || p.slots[t0] != slot) break;
+  const __nv_bfloat16* input = (const __nv_bfloat16*)(which ? p.v : p.k) + (long long)h * (which ? p.v_head : p.k_head) + d;
+  // where runs begin
+  const bool mine = lane < p.window && w0 + lane < p.tokens;
+  const int my_slot = mine ? p.slots[w0 + lane] : -1;
+  const bool valid = (unsigned)my_slot < (unsigned)p.limit;
+  int prev = __shfl_up_sync(0xffffffffu, my_slot, 1);
+  if (lane == 0) prev = w0 > 0 ? p.slots[w0 - 1] : -1;
+  const bool inside = valid && (my_slot & ((1 << p.block_log) - 1)) != 0;
+  bool start = valid && !(inside && prev == my_slot - 1);
+  unsigned ask = __ballot_sync(0xffffffffu, start && inside && (unsigned)prev >= (unsigned)p.limit);
+  while (ask) {                        // behind skipped tokens: does the last one that counts precede this one?
+    const int j = __ffs(ask) - 1;
+    ask &= ask - 1;
+    const long long before = valid_before(p, w0 + j);
+    const int last = before >= 0 ? p.slots[before] : -1;
+    if (lane == j && last == my_slot - 1) start = false;
   }
-  if (lane == 0) p.scale[bh] = old;
+  unsigned runs = __ballot_sync(0xffffffffu, start);
+  while (runs) {
+    const int j = __ffs(runs) - 1;
+    runs &= runs - 1;
+    long long t0 = w0 + j;
+    int slot = __shfl_sync(0xffffffffu, my_slot, j);
+    const int id = slot >> p.block_log;
+    int off = slot - (id << p.block_log);
+    const long long bh = ((long long)which * p.blocks + id) * p.heads + h;
+    uint8_t* codes = p.codes + (long long)which * p.kv_stride + (((long long)id * p.heads + h) << p.block_log) * D;
+    float old = off > 0 ? p.scale[bh] : 0.f;
+    for (;;) {
+      int n = 0;
+      for (;;) {                       // length
+        const int i = n + lane;
+        const bool on = off + i < (1 << p.block_log) && t0 + i < p.tokens && p.slots[t0 + i] == slot + i;
+        const unsigned same = __ballot_sync(0xffffffffu, on);
+        n += same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+        if (same != 0xffffffffu) break;
+      }
+      const __nv_bfloat16* x = input + t0 * step;
+      uint4 held[HELD];
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) {
+        const int tok = i * TOKENS + sub;
+        held[i] = tok < n ? eight(x + tok * step, vec) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) top = abs_max(top, held[i]);
+      for (int tok = 32 + sub; tok < n; tok += TOKENS) top = abs_max(top, eight(x + tok * step, vec));
+      const uint32_t most = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+      const float now = fmaxf(old, scale_for(__uint_as_float(most << 16)));
+      if (off > 0 && now != old) {     // the codes of earlier tokens go to the new scale
+        const float r = old * inv_pow2(now);
+        for (int i = lane; i < off * D / 4; i += 32) {
+          const uint32_t c = reinterpret_cast<const uint32_t*>(codes)[i];
+          uint32_t m = 0;
+#pragma unroll
+          for (int b = 0; b < 32; b += 8) m |= code_of(value_of((c >> b) & 0xffu) * r) << b;
+          reinterpret_cast<uint32_t*>(codes)[i] = m;
+        }
+      }
+      const float inv = inv_pow2(now);
+      uint8_t* to = codes + off * D + d;
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) {
+        const int tok = i * TOKENS + sub;
+        if (tok < n) *reinterpret_cast<uint2*>(to + tok * D) = make_uint2(codes4(held[i].x, held[i].y, inv), codes4(held[i].z, held[i].w, inv));
+      }
+      for (int tok = 32 + sub; tok < n; tok += TOKENS) {
+        const uint4 w = eight(x + tok * step, vec);
+        *reinterpret_cast<uint2*>(to + tok * D) = make_uint2(codes4(w.x, w.y, inv), codes4(w.z, w.w, inv));
+      }
+      __syncwarp();
+      old = now;
+      off += n;
+      slot += n;
+      if (off == 1 << p.block_log) break;
+      t0 = valid_from(p, t0 + n);
+      if (t0 >= p.tokens || p.slots[t0] != slot) break;
+    }
+    if (lane == 0) p.scale[bh] = old;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ reorder
@@ -253,34 +339,47 @@ __global__ void __launch_bounds__(128) kv_reorder_kernel(KvReorder p) {
 
 extern "C" {
 
-// Block tables and slot maps.  rows <= 8192; `tables` int32 [rows, width] is completed in place, `free_count_out` may not be
-// `free_count` (callers that keep one counter copy it back).
+// Block tables and slot maps.  rows <= 8192; `tables` int32 [rows, width] is completed in place; `free_count_out` may be
+// `free_count`; `own`: one word of work space.
 int nb_kv_plan(const int* lengths, const int* new_lens, int* tables, const int* free_ids, const int* free_count, int* free_count_out,
-               int* starts, int* ends, int* row_of, int* positions, int* slots, int rows, int width, int block, int free_size,
+               int* starts, int* ends, int* row_of, int* positions, int* slots, int* own, int rows, int width, int block, int free_size,
                int tokens, unsigned int* status, void* stream) {
   if (rows <= 0 || rows > 8192 || width <= 0 || block <= 0 || tokens < 0 || free_size < 0) return NB_ERR_BAD_ARG;
-  if (free_count == free_count_out || (long long)width * block > 0x7fffffffLL) return NB_ERR_BAD_ARG;
-  KvPlan p{lengths, new_lens, tables, free_ids, free_count, free_count_out, starts, ends, row_of, positions, slots, rows, width, block, free_size, tokens, status};
+  if ((block & (block - 1)) || (long long)width * block > 0x7fffff00LL || tokens > 0x7fffff00) return NB_ERR_BAD_ARG;
+  const int grid = max(1, min(148 * 4, ceil_div(tokens, 1024)));
+  // every block reads the count when it begins, so only a single block may write it back in place
+  const bool later = grid > 1 && free_count == free_count_out;
+  KvPlan p{lengths, new_lens, tables, free_ids, free_count, later ? own : free_count_out, starts, ends, row_of, positions, slots, rows, width, 0, free_size, tokens, 0, status};
+  while ((1 << p.block_log) < block) ++p.block_log;
+  p.vec = !((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(row_of)) & 15);
   static bool configured[64] = {};
   int dev = 0;
   NB_CUDA(cudaGetDevice(&dev));
   if (dev >= 64) return NB_ERR_BAD_ARG;
   if (!configured[dev]) {
-    NB_CUDA(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * 8192 + 1) * 4));
+    NB_CUDA(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * 8192 + 1) * 4));
     configured[dev] = true;
   }
-  const int grid = max(1, min(296, ceil_div(tokens, 1024)));
-  kv_plan_kernel<<<grid, 256, (2 * rows + 1) * 4, (cudaStream_t)stream>>>(p);
+  kv_plan_kernel<<<grid, 256, (3 * rows + 1) * 4, (cudaStream_t)stream>>>(p);
   NB_LAUNCH_CHECK();
+  if (later) NB_CUDA(cudaMemcpyAsync(free_count_out, own, 4, cudaMemcpyDeviceToDevice, (cudaStream_t)stream));
   return NB_OK;
 }
 
 int nb_kv_append(const void* k, const void* v, void* codes, float* scale, const int* slots, int tokens, int heads, int dim, int block,
                  int blocks, long long k_token, long long k_head, long long v_token, long long v_head, long long kv_stride, void* stream) {
-  if (tokens < 0 || heads <= 0 || (dim != 64 && dim != 128) || block <= 0 || blocks <= 0 || (long long)blocks * block > 0x7fffffffLL) return NB_ERR_BAD_ARG;
+  if (tokens < 0 || heads <= 0 || heads > 32767 || (dim != 64 && dim != 128) || block < 16 || (block & (block - 1)) || blocks <= 0) return NB_ERR_BAD_ARG;
+  if ((long long)blocks * block > 0x7fffffffLL) return NB_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(codes) & 15) || (kv_stride & 15)) return NB_ERR_UNALIGNED;
   if (tokens == 0) return NB_OK;
-  KvAppend p{k, v, (uint8_t*)codes, scale, slots, tokens, heads, dim, block, blocks, blocks * block, k_token, k_head, v_token, v_head, kv_stride};
-  kv_append_kernel<<<dim3(ceil_div(tokens, 4), 2 * heads), 128, 0, (cudaStream_t)stream>>>(p);
+  KvAppend p{k, v, (uint8_t*)codes, scale, slots, tokens, heads, 0, blocks, blocks * block, 0, 0, 0, k_token, k_head, v_token, v_head, kv_stride};
+  while ((1 << p.block_log) < block) ++p.block_log;
+  p.k_vec = !((reinterpret_cast<uintptr_t>(k) & 15) || (k_token & 7) || (k_head & 7));
+  p.v_vec = !((reinterpret_cast<uintptr_t>(v) & 15) || (v_token & 7) || (v_head & 7));
+  p.window = tokens <= 2048 ? 1 : 32;
+  const dim3 grid(ceil_div(tokens, 4 * p.window), 2 * heads);
+  if (dim == 64) kv_append_kernel<64><<<grid, 128, 0, (cudaStream_t)stream>>>(p);
+  else kv_append_kernel<128><<<grid, 128, 0, (cudaStream_t)stream>>>(p);
   NB_LAUNCH_CHECK();
   return NB_OK;
 }

@@ -11,7 +11,7 @@ struct KvPlan {
   int* tables;
   const int *free_ids, *free_count;
   int *free_count_out, *starts, *ends, *row_of, *positions, *slots;
-  int rows, width, block, free_size, tokens;
+  int rows, width, block_log, free_size, tokens, vec;
   unsigned int* status;
 };
 
@@ -20,7 +20,7 @@ struct KvAppend {
   uint8_t* codes;
   float* scale;
   const int* slots;
-  int tokens, heads, dim, block, blocks, limit;
+  int tokens, heads, block_log, blocks, limit, window, k_vec, v_vec;
   long long k_token, k_head, v_token, v_head;   // element strides of the inputs
   long long kv_stride;                          // bytes from the keys' codes to the values'
 };

@@ -57,15 +57,14 @@ def beam_select(logits, scores, finished=None, eos=None):
     if guard is not None:
         with guard:
             return beam_select(logits, scores, finished, eos)
-    out = torch.empty((3, requests, beams), dtype=torch.int32, device=logits.device)
-    done = torch.empty((requests, beams), dtype=torch.bool, device=logits.device)
+    like = torch.empty_like
+    new_scores, parents, tokens, done = like(scores), like(scores, dtype=torch.int32), like(scores, dtype=torch.int32), like(scores, dtype=torch.bool)
     nbytes = _work_bytes(requests, beams, vocab)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)      # of this call alone
-    new_scores, parents, tokens = out.unbind(0)
-    at, step = out.data_ptr(), 4 * requests * beams
-    check(cuda_lib().nb_beam_select(logits.data_ptr(), scores.data_ptr(), None if finished is None else finished.data_ptr(), at, at + step, at + 2 * step, done.data_ptr(),
-                                    requests, beams, vocab, -1 if eos is None else eos, int(fp32), pitch, work.data_ptr(), nbytes, raw_stream()), "beam_select")
-    return new_scores.view(torch.float32), parents, tokens, done
+    work = scores.new_empty((nbytes + 3) // 4)               # of this call alone
+    check(cuda_lib().nb_beam_select(logits.data_ptr(), scores.data_ptr(), None if finished is None else finished.data_ptr(), new_scores.data_ptr(), parents.data_ptr(),
+                                    tokens.data_ptr(), done.data_ptr(), requests, beams, vocab, -1 if eos is None else eos, int(fp32), pitch, work.data_ptr(), nbytes,
+                                    raw_stream()), "beam_select")
+    return new_scores, parents, tokens, done
 
 
 @functools.lru_cache(maxsize=256)

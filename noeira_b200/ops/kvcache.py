@@ -77,30 +77,27 @@ def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free
     _ints("free_count", free_count, dev, 1)
     if free_count_out is not None:
         _ints("free_count_out", free_count_out, dev, 1)
-    if block <= 0 or tokens < 0 or width * block >= 1 << 31:
-        raise ValueError(f"block {block}, tokens {tokens}, width {width}: out of range")
+    if block not in BLOCKS or not 0 <= tokens <= 0x7fffff00 or width * block > 0x7fffff00:
+        raise ValueError(f"block {block}, tokens {tokens}, width {width}: blocks of {BLOCKS} tokens, fewer than 2^31 tokens")
     if dev < 0:
         return _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out)
     guard = _on(tables)
     if guard is not None:
         with guard:
             return plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out)
-    in_place = free_count_out is None or free_count_out.data_ptr() == free_count.data_ptr()
-    # one allocation: starts | ends | left | rows | positions | slots, each on a 16-byte boundary
+    if free_count_out is None:
+        free_count_out = free_count
+    # one allocation, each output on a 16-byte boundary; its last four words are the kernel's own
     pr, pt = (rows + 4) & ~3, (tokens + 3) & ~3
-    buf = torch.empty(2 * pr + 4 + 3 * pt, dtype=torch.int32, device=tables.device)
-    starts, ends, left = buf[: rows + 1], buf[pr: pr + rows], buf[2 * pr: 2 * pr + 1]
-    at = 2 * pr + 4
-    row_of, positions, slots = buf[at: at + tokens], buf[at + pt: at + pt + tokens], buf[at + 2 * pt: at + 2 * pt + tokens]
-    out = left if in_place else free_count_out
-    base = buf.data_ptr()
+    buf = torch.empty(2 * pr + 3 * pt + 4, dtype=torch.int32, device=tables.device)
+    starts, _, ends, _, row_of, _, positions, _, slots, _ = buf.split_with_sizes(
+        (rows + 1, pr - rows - 1, rows, pr - rows, tokens, pt - tokens, tokens, pt - tokens, tokens, pt - tokens + 4))
+    at = buf.data_ptr()
+    to = at + 8 * pr
     check(cuda_lib().nb_kv_plan(
-        lengths.data_ptr(), new_lens.data_ptr(), tables.data_ptr(), free.data_ptr(), free_count.data_ptr(), out.data_ptr(), base, base + 4 * pr,
-        base + 4 * at, base + 4 * (at + pt), base + 4 * (at + 2 * pt), rows, width, block, free.numel(), tokens, status_ptr(dev), raw_stream()), "kv_plan")
-    if in_place:
-        free_count.copy_(left)
-        out = free_count
-    return TokenPlan(starts, ends, row_of, positions, slots, out)
+        lengths.data_ptr(), new_lens.data_ptr(), tables.data_ptr(), free.data_ptr(), free_count.data_ptr(), free_count_out.data_ptr(), at, at + 4 * pr, to, to + 4 * pt,
+        to + 8 * pt, to + 12 * pt, rows, width, block, free.numel(), tokens, status_ptr(dev), raw_stream()), "kv_plan")
+    return TokenPlan(starts, ends, row_of, positions, slots, free_count_out)
 
 
 def _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out):
@@ -260,7 +257,7 @@ def paged_attention(q, kv, scale, tables, starts, ends, max_new=None, softmax_sc
             return paged_attention(q, kv, scale, tables, starts, ends, max_new, softmax_scale, out)
     # partial results of this call alone: calls on two streams, or in two graphs, share nothing
     floats = _work_floats(dim)
-    work = torch.empty(floats, dtype=torch.float32, device=q.device)
+    work = scale.new_empty(floats)
     check(cuda_lib().nb_kv_attention(
         q.data_ptr(), out.data_ptr(), kv.data_ptr(), scale.data_ptr(), tables.data_ptr(), starts.data_ptr(), ends.data_ptr(), rows, tokens, max_new, hq, hk, dim,
         block, blocks, width, qs[0], qs[1], os_[0], os_[1], kv.stride(0), scale.stride(0), softmax_scale, work.data_ptr(), floats, status_ptr(dev), raw_stream()), "kv_attention")
