@@ -1,6 +1,8 @@
 """Character-level GPT on a text file (CPU or CUDA): AutoregressiveTrainer with warm-up + cosine schedule.
 
-    python examples/gpt_char.py corpus.txt [--device cuda] [--steps 500]
+    python examples/gpt_char.py corpus.txt [--device cuda] [--steps 500] [--answer "Once" --tokens 64 --beams 4]
+
+``--answer`` continues a prompt with the trained model: beam search (greedy with one beam) over the paged 8-bit cache.
 """
 import argparse
 import os
@@ -18,6 +20,9 @@ def main():
     ap.add_argument("--steps", type=int, default=500)
     ap.add_argument("--seq", type=int, default=128)
     ap.add_argument("--batch", type=int, default=32)
+    ap.add_argument("--answer", default="")
+    ap.add_argument("--tokens", type=int, default=32)
+    ap.add_argument("--beams", type=int, default=4)
     args = ap.parse_args()
     from noeira_b200.data.datasets import CharCorpus
     from noeira_b200.models.gpt import GPT
@@ -32,6 +37,11 @@ def main():
         tr.train_step()
         if (s + 1) % 50 == 0:
             print(s + 1, "loss", round(tr.mean_loss() / 50, 4))
+    if args.answer:
+        prompt = [int(t) for t in corpus.encode(args.answer)]
+        texts, scores = model.eval().beam_search([prompt], beams=args.beams, max_new=min(args.tokens, args.seq - len(prompt)))
+        for text, score in zip(texts[0], scores[0].tolist()):
+            print(round(score, 3), repr(args.answer + corpus.decode([t for t in text if t < corpus.vocab])))
 
 
 if __name__ == "__main__":

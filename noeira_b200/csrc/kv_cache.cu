@@ -57,7 +57,8 @@ __device__ __forceinline__ long long block_scan(long long v, long long* sh, long
   return v + before;
 }
 
-__global__ void __launch_bounds__(256) kv_plan_kernel(KvPlan p) {
+template <int EACH>
+__global__ void __launch_bounds__(256) kv_plan_kernel(const KvPlan p) {
   extern __shared__ int sm[];
   int* s_start = sm;                 // [rows + 1]
   int* s_off = sm + p.rows + 1;      // [rows] first block of the row among the new ones, -1: refused
@@ -66,17 +67,22 @@ __global__ void __launch_bounds__(256) kv_plan_kernel(KvPlan p) {
   const int tid = threadIdx.x, per = ceil_div(p.rows, 256);
   const int lo = min(p.rows, tid * per), hi = min(p.rows, lo + per);
   const int free_count = max(0, min(*p.free_count, p.free_size));
+#pragma unroll 4
+  for (int i = tid; i < p.rows; i += 256) {
+    s_len[i] = p.lengths[i];
+    s_off[i] = p.new_lens[i];
+  }
+  __syncthreads();
   long long sum = 0, total;
-  for (int i = lo; i < hi; ++i) sum += max(0, p.new_lens[i]);
+  for (int i = lo; i < hi; ++i) sum += max(0, s_off[i]);
   long long at = block_scan(sum, sh, total) - sum;      // 64 bits: lengths are the caller's, their sum may be anything
   if (tid == 0) s_start[p.rows] = (int)min(total, 0x7fffffffLL);
   sum = 0;
   for (int i = lo; i < hi; ++i) {
-    const int len = p.lengths[i], add = max(0, p.new_lens[i]);
+    const int len = s_len[i], given = s_off[i], add = max(0, given);
     s_start[i] = (int)min(at, 0x7fffffffLL);
-    s_len[i] = len;
     at += add;
-    const bool fits = len >= 0 && p.new_lens[i] >= 0 && (long long)len + add <= ((long long)p.width << p.block_log) && at <= p.tokens;
+    const bool fits = len >= 0 && given >= 0 && (long long)len + add <= ((long long)p.width << p.block_log) && at <= p.tokens;
     s_off[i] = fits ? ((len + add + (1 << p.block_log) - 1) >> p.block_log) - ((len + (1 << p.block_log) - 1) >> p.block_log) : -1;
     sum += max(0, s_off[i]);
   }
@@ -91,11 +97,13 @@ __global__ void __launch_bounds__(256) kv_plan_kernel(KvPlan p) {
       if (need > 0) taken = off + need;
     }
     if (need > 0) off += need;
-    if (blockIdx.x == 0) p.ends[i] = p.lengths[i] + (s_off[i] < 0 ? 0 : p.new_lens[i]);
   }
   __syncthreads();
   if (blockIdx.x == 0) {
-    for (int i = tid; i <= p.rows; i += 256) p.starts[i] = s_start[i];
+    for (int i = tid; i <= p.rows; i += 256) {
+      p.starts[i] = s_start[i];
+      if (i < p.rows) p.ends[i] = s_len[i] + (s_off[i] < 0 ? 0 : s_start[i + 1] - s_start[i]);
+    }
     taken = (long long)__reduce_max_sync(0xffffffffu, (unsigned)taken);   // at most free_count
     if ((tid & 31) == 0) sh[tid >> 5] = taken;
     __syncthreads();
@@ -104,16 +112,17 @@ __global__ void __launch_bounds__(256) kv_plan_kernel(KvPlan p) {
       *p.free_count_out = free_count - (int)taken;
     }
   }
-  // four neighbouring tokens a thread: one search, one look into the table per page, 16-byte stores
-  for (long long t0 = ((long long)blockIdx.x * 256 + tid) * 4; t0 < p.tokens; t0 += (long long)gridDim.x * 1024) {
+  // Neighbouring tokens of a thread share one search, and one look into the table per page; four of them are stored at once.  In a
+  // decode step neighbours belong to different rows, and a thread with four would wait for four tables in turn: one a thread.
+  for (long long t0 = ((long long)blockIdx.x * 256 + tid) * EACH; t0 < p.tokens; t0 += (long long)gridDim.x * 256 * EACH) {
     int a = 0, b = p.rows;             // last row with start <= t0
     while (b - a > 1) {
       const int m = (a + b) >> 1;
       if (s_start[m] <= (int)t0) a = m; else b = m;
     }
-    int slot[4], pos[4], row[4], page = -1, id = -1;
+    int slot[EACH], pos[EACH], row[EACH], page = -1, id = -1;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < EACH; ++e) {
       const int t = (int)t0 + e;       // may pass the last token by three: below 2^31 by the launcher's limit
       while (a + 1 < p.rows && s_start[a + 1] <= t) {
         ++a;
@@ -135,16 +144,18 @@ __global__ void __launch_bounds__(256) kv_plan_kernel(KvPlan p) {
         if (id >= 0) slot[e] = (id << p.block_log) + in;
       }
     }
-    if (p.vec && t0 + 4 <= p.tokens) {
-      *reinterpret_cast<int4*>(p.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
-      *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
-      *reinterpret_cast<int4*>(p.row_of + t0) = make_int4(row[0], row[1], row[2], row[3]);
+    if (EACH == 4 && p.vec && t0 + 4 <= p.tokens) {
+      *reinterpret_cast<int4*>(p.slots + t0) = make_int4(slot[0], slot[1 % EACH], slot[2 % EACH], slot[3 % EACH]);
+      *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1 % EACH], pos[2 % EACH], pos[3 % EACH]);
+      *reinterpret_cast<int4*>(p.row_of + t0) = make_int4(row[0], row[1 % EACH], row[2 % EACH], row[3 % EACH]);
     } else {
-      for (int e = 0; e < 4 && t0 + e < p.tokens; ++e) {
-        p.slots[t0 + e] = slot[e];
-        p.positions[t0 + e] = pos[e];
-        p.row_of[t0 + e] = row[e];
-      }
+#pragma unroll
+      for (int e = 0; e < EACH; ++e)
+        if (t0 + e < p.tokens) {
+          p.slots[t0 + e] = slot[e];
+          p.positions[t0 + e] = pos[e];
+          p.row_of[t0 + e] = row[e];
+        }
     }
   }
 }
@@ -176,22 +187,15 @@ __device__ __forceinline__ uint4 eight(const __nv_bfloat16* x, int vec) {
   const unsigned short* e = reinterpret_cast<const unsigned short*>(x);
   return make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
 }
-// Magnitudes (bf16 pairs) with what is not finite as zero.
-__device__ __forceinline__ uint32_t finite_abs(uint32_t w) {
-  const uint32_t v = w & 0x7fff7fffu;
-  return v & ~__vcmpgeu2(v, 0x7f807f80u);
-}
-__device__ __forceinline__ uint32_t abs_max(uint32_t m, const uint4& w) {
-  return __vmaxu2(m, __vmaxu2(__vmaxu2(finite_abs(w.x), finite_abs(w.y)), __vmaxu2(finite_abs(w.z), finite_abs(w.w))));
+__device__ __forceinline__ uint32_t abs_max(uint32_t m, const uint4& w) {   // of bf16 pairs, by their bits
+  constexpr uint32_t A = 0x7fff7fffu;
+  return __vmaxu2(m, __vmaxu2(__vmaxu2(w.x & A, w.y & A), __vmaxu2(w.z & A, w.w & A)));
 }
 __device__ __forceinline__ uint32_t codes4(uint32_t a, uint32_t b, float inv) {
-  const float x0 = __uint_as_float(a << 16) * inv, x1 = __uint_as_float(a & 0xffff0000u) * inv;
-  const float x2 = __uint_as_float(b << 16) * inv, x3 = __uint_as_float(b & 0xffff0000u) * inv;
-  uint32_t r = e4m3x2(x0, x1) | e4m3x2(x2, x3) << 16;
-  if ((((a & 0x7fff7fffu) + 0x00800080u) | ((b & 0x7fff7fffu) + 0x00800080u)) & 0x80008000u)   // an exponent of all ones
-    r = code_of(x0) | code_of(x1) << 8 | code_of(x2) << 16 | code_of(x3) << 24;
-  return r;
+  return e4m3x2(__uint_as_float(a << 16) * inv, __uint_as_float(a & 0xffff0000u) * inv) |
+         e4m3x2(__uint_as_float(b << 16) * inv, __uint_as_float(b & 0xffff0000u) * inv) << 16;
 }
+constexpr uint32_t BF16_INF = 0x7f80;
 
 // A run is a stretch of neighbouring tokens and slots inside one block.  A warp takes the runs that begin in a window of `window`
 // tokens, for one head of K or V: D / 8 lanes a token, 16 bytes each, so that a run of up to 32 tokens is read once and stays in
@@ -254,7 +258,17 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p) {
 #pragma unroll
       for (int i = 0; i < HELD; ++i) top = abs_max(top, held[i]);
       for (int tok = 32 + sub; tok < n; tok += TOKENS) top = abs_max(top, eight(x + tok * step, vec));
-      const uint32_t most = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+      uint32_t most = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+      const bool odd = most >= BF16_INF;       // something is not finite: the maximum over what is, element by element
+      if (odd) {
+        most = 0;
+        for (int tok = sub; tok < n; tok += TOKENS)
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t v = reinterpret_cast<const unsigned short*>(x + tok * step)[e] & 0x7fffu;
+            if (v < BF16_INF) most = max(most, v);
+          }
+        most = __reduce_max_sync(0xffffffffu, most);
+      }
       const float now = fmaxf(old, scale_for(__uint_as_float(most << 16)));
       if (off > 0 && now != old) {     // the codes of earlier tokens go to the new scale
         const float r = old * inv_pow2(now);
@@ -268,14 +282,19 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p) {
       }
       const float inv = inv_pow2(now);
       uint8_t* to = codes + off * D + d;
+      if (odd) {
+        for (int tok = sub; tok < n; tok += TOKENS)
+          for (int e = 0; e < 8; ++e) to[tok * D + e] = (uint8_t)code_of(__bfloat162float(x[tok * step + e]) * inv);
+      } else {
 #pragma unroll
-      for (int i = 0; i < HELD; ++i) {
-        const int tok = i * TOKENS + sub;
-        if (tok < n) *reinterpret_cast<uint2*>(to + tok * D) = make_uint2(codes4(held[i].x, held[i].y, inv), codes4(held[i].z, held[i].w, inv));
-      }
-      for (int tok = 32 + sub; tok < n; tok += TOKENS) {
-        const uint4 w = eight(x + tok * step, vec);
-        *reinterpret_cast<uint2*>(to + tok * D) = make_uint2(codes4(w.x, w.y, inv), codes4(w.z, w.w, inv));
+        for (int i = 0; i < HELD; ++i) {
+          const int tok = i * TOKENS + sub;
+          if (tok < n) *reinterpret_cast<uint2*>(to + tok * D) = make_uint2(codes4(held[i].x, held[i].y, inv), codes4(held[i].z, held[i].w, inv));
+        }
+        for (int tok = 32 + sub; tok < n; tok += TOKENS) {
+          const uint4 w = eight(x + tok * step, vec);
+          *reinterpret_cast<uint2*>(to + tok * D) = make_uint2(codes4(w.x, w.y, inv), codes4(w.z, w.w, inv));
+        }
       }
       __syncwarp();
       old = now;
@@ -346,7 +365,7 @@ int nb_kv_plan(const int* lengths, const int* new_lens, int* tables, const int* 
                int tokens, unsigned int* status, void* stream) {
   if (rows <= 0 || rows > 8192 || width <= 0 || block <= 0 || tokens < 0 || free_size < 0) return NB_ERR_BAD_ARG;
   if ((block & (block - 1)) || (long long)width * block > 0x7fffff00LL || tokens > 0x7fffff00) return NB_ERR_BAD_ARG;
-  const int grid = max(1, min(148 * 4, ceil_div(tokens, 1024)));
+  const int each = tokens < 8LL * rows ? 1 : 4, grid = max(1, min(148 * 4, ceil_div(tokens, 256 * each)));
   // every block reads the count when it begins, so only a single block may write it back in place
   const bool later = grid > 1 && free_count == free_count_out;
   KvPlan p{lengths, new_lens, tables, free_ids, free_count, later ? own : free_count_out, starts, ends, row_of, positions, slots, rows, width, 0, free_size, tokens, 0, status};
@@ -357,10 +376,12 @@ int nb_kv_plan(const int* lengths, const int* new_lens, int* tables, const int* 
   NB_CUDA(cudaGetDevice(&dev));
   if (dev >= 64) return NB_ERR_BAD_ARG;
   if (!configured[dev]) {
-    NB_CUDA(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * 8192 + 1) * 4));
+    NB_CUDA(cudaFuncSetAttribute(kv_plan_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * 8192 + 1) * 4));
+    NB_CUDA(cudaFuncSetAttribute(kv_plan_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * 8192 + 1) * 4));
     configured[dev] = true;
   }
-  kv_plan_kernel<<<grid, 256, (3 * rows + 1) * 4, (cudaStream_t)stream>>>(p);
+  if (each == 1) kv_plan_kernel<1><<<grid, 256, (3 * rows + 1) * 4, (cudaStream_t)stream>>>(p);
+  else kv_plan_kernel<4><<<grid, 256, (3 * rows + 1) * 4, (cudaStream_t)stream>>>(p);
   NB_LAUNCH_CHECK();
   if (later) NB_CUDA(cudaMemcpyAsync(free_count_out, own, 4, cudaMemcpyDeviceToDevice, (cudaStream_t)stream));
   return NB_OK;

@@ -5,7 +5,8 @@
 counter-hash dropout after the embeddings and inside every block residual branch (GPTDrop); ``tie=True`` shares the
 embedding matrix with the head (GPTDropTied).  Residual output projections are initialised with std 0.02/sqrt(2L)
 (``gpt_scale_residual_proj``).  Parameter names follow the child paths: ``wte.weight``, ``wpe.weight``,
-``blocks.<i>.norm1.gamma`` …, ``ln_f.gamma``, ``head.weight``.
+``blocks.<i>.norm1.gamma`` …, ``ln_f.gamma``, ``head.weight``.  ``generate`` and ``beam_search`` answer prompts over a paged 8-bit
+key / value cache (``ops.kvcache``, ``ops.beam``); ``new_cache`` and ``forward_cached`` are their parts for servers of their own.
 Reference: noeira/nn/models/gpt.mojo:75,159,193,267,316; ViT / PatchEmbed noeira/nn/models/vit.mojo:25,41.
 """
 from __future__ import annotations
@@ -16,6 +17,8 @@ import torch
 
 from .. import nn
 from ..nn.module import Module
+from ..ops.beam import beam_select
+from ..ops.kvcache import PagedKVCache
 
 
 class GPT(Module):
@@ -85,6 +88,83 @@ class GPT(Module):
         self.wte.vjp(dx)
         self.wpe.vjp(dx)
         return None
+
+    # ---------------------------------------------------------------------------------------- answering
+    def new_cache(self, rows: int, max_len: int, block: int = 16, blocks: int = None, spares: bool = False):
+        """An empty ``PagedKVCache`` for ``rows`` sequences of up to ``max_len`` tokens (at most ``seq``: positions are learned).
+        ``spares``: for beam search, a block more per row; the default number of blocks lets every row grow to ``max_len``."""
+        if not 0 < max_len <= self.seq:
+            raise ValueError(f"max_len: up to {self.seq} positions, got {max_len}")
+        attn = self.blocks[0].attn
+        blocks = rows * (-(-max_len // block) + (3 if spares else 0)) if blocks is None else blocks
+        return PagedKVCache(len(self.blocks), attn.hkv, attn.hd, blocks, rows, max_len, block, self.wte.weight.data.device, spares)
+
+    @torch.no_grad()
+    def forward_cached(self, ids: torch.Tensor, cache, plan, max_new: int = None):
+        """New tokens ``ids [tokens]`` of the cache's rows (``plan = cache.plan(new_lens, tokens)``) → logits ``[rows, vocab]`` of each
+        row's last new token.  Rows without new tokens get those of a neighbour, which mean nothing."""
+        x = self.wte.forward(ids) + self.wpe.forward(plan.positions)
+        for layer, b in enumerate(self.blocks):
+            x = b.forward_cached(x, cache, layer, plan, max_new=max_new)
+        h = self.ln_f.forward(x.index_select(0, (plan.starts[1:] - 1).clamp_min(0)))
+        if not self.tie:
+            return self.head.forward(h)
+        if h.is_cuda:
+            from ..ops.gemm import gemm
+            return gemm(h, self.wte.weight.shadow[:, : self.dim])[:, : self.vocab]
+        return h.float() @ self.wte.weight.data.t()
+
+    @torch.no_grad()
+    def beam_search(self, prompts, beams: int = 4, max_new: int = 32, eos: int = None, block: int = 16):
+        """The ``beams`` likeliest continuations of up to ``max_new`` tokens of each prompt (lists of token ids), best first:
+        ``(sequences, scores)`` with ``sequences[r][j]`` a list that ends behind ``eos`` and ``scores [requests, beams]`` the summed
+        log-probabilities.  Keys and values live in a paged 8-bit cache that the beams of a request share."""
+        lens = [len(p) for p in prompts]
+        if not lens or min(lens) == 0 or beams < 1 or max_new < 1:
+            raise ValueError("beam_search: prompts of at least one token, at least one beam and one new token")
+        R, rows, dev = len(lens), len(lens) * beams, self.wte.weight.data.device
+        cache = self.new_cache(rows, max(lens) + max_new, block, spares=beams > 1)
+        new = torch.zeros(R, beams, dtype=torch.int32)
+        new[:, 0] = torch.tensor(lens)
+        ids = torch.tensor([t for p in prompts for t in p], dtype=torch.int64).to(dev)
+        plan = cache.plan(new.reshape(-1).to(dev), ids.numel())
+        logits = self.forward_cached(ids, cache, plan, max_new=max(lens)).unflatten(0, (R, beams))[:, :1]
+        logits = logits.expand(R, beams, -1).contiguous()            # the beams of a request begin as one
+        scores = torch.full((R, beams), -math.inf, device=dev)
+        scores[:, 0] = 0
+        one = torch.ones(rows, dtype=torch.int32, device=dev)
+        done, steps = None, []
+        for n in range(max_new):
+            scores, parents, tokens, done = beam_select(logits, scores, finished=done if eos is not None else None, eos=eos)
+            steps.append((parents, tokens))
+            if n == max_new - 1 or (eos is not None and n % 8 == 7 and bool(done.all())):
+                break
+            if beams > 1:
+                cache.reorder(parents)
+                if n == 0:
+                    cache.refill_spares()                            # a beam's first own block came from its spare
+            plan = cache.plan(one, rows)
+            logits = self.forward_cached(tokens.reshape(-1), cache, plan, max_new=1).unflatten(0, (R, beams))
+        at, back = torch.arange(beams, device=dev).expand(R, beams), []
+        for parents, tokens in reversed(steps):
+            back.append(torch.gather(tokens, 1, at))
+            at = torch.gather(parents, 1, at).to(torch.int64)
+        check_status_of(dev)
+        out = torch.stack(back[::-1], -1).tolist()
+        if eos is not None:
+            out = [[s[: s.index(eos) + 1] if eos in s else s for s in beam] for beam in out]
+        return out, scores
+
+    def generate(self, prompts, max_new: int = 32, eos: int = None, block: int = 16):
+        """The likeliest next token, ``max_new`` times (or up to ``eos``), after each prompt: a list of lists of token ids."""
+        return [s[0] for s in self.beam_search(prompts, 1, max_new, eos, block)[0]]
+
+
+def check_status_of(device):
+    """Raises what a kernel reported about the cache (no room, a bad block); CPU calls raise by themselves."""
+    if device.type == "cuda":
+        from ..ops import check_status
+        check_status(device)
 
 
 class PatchEmbed(Module):

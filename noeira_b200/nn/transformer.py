@@ -200,6 +200,18 @@ class SelfAttention(Module):
         o = self.core.forward(q, k, v, key_valid=key_valid, bias=bias)
         return self.out.forward(o.reshape(B, S, self.h * self.hd), residual=residual)
 
+    def forward_cached(self, x, cache, layer, plan, max_new=None, residual=None):
+        """New tokens ``x [tokens, dim]`` of the rows of a ``PagedKVCache``: their keys and values go into cache layer ``layer``,
+        and each token attends to its row up to itself.  Inference only (nothing is kept for ``vjp``); causal blocks without
+        rotary embedding, whose positions the cache does not know."""
+        if self.core.mask != "causal" or self.rope_theta:
+            raise ValueError("forward_cached: causal attention without rotary embedding")
+        T = x.shape[0]
+        qkv = self.qkv.forward(x).reshape(T, self.h + 2 * self.hkv, self.hd)
+        cache.append(layer, qkv[:, self.h: self.h + self.hkv], qkv[:, self.h + self.hkv:], plan)
+        o = cache.attend(layer, qkv[:, : self.h], plan, max_new=max_new, softmax_scale=self.core.scale)
+        return self.out.forward(o.reshape(T, self.h * self.hd), residual=residual)
+
     def vjp(self, dy):
         B, S, _ = dy.shape
         do = self.out.vjp(dy).reshape(B, S, self.h, self.hd)
@@ -334,6 +346,11 @@ class TransformerBlock(Module):
 
     def forward(self, x, key_valid=None, bias=None):
         x = self.attn.forward(self.n1.forward(x), key_valid=key_valid, bias=bias, residual=x)
+        return self.ffn.forward(self.n2.forward(x), residual=x)
+
+    def forward_cached(self, x, cache, layer, plan, max_new=None):
+        """``forward`` for new tokens ``[tokens, dim]`` over a ``PagedKVCache`` (see ``SelfAttention.forward_cached``)."""
+        x = self.attn.forward_cached(self.n1.forward(x), cache, layer, plan, max_new=max_new, residual=x)
         return self.ffn.forward(self.n2.forward(x), residual=x)
 
     def vjp(self, dy):

@@ -87,16 +87,14 @@ def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free
             return plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out)
     if free_count_out is None:
         free_count_out = free_count
-    # one allocation, each output on a 16-byte boundary; its last four words are the kernel's own
-    pr, pt = (rows + 4) & ~3, (tokens + 3) & ~3
-    buf = torch.empty(2 * pr + 3 * pt + 4, dtype=torch.int32, device=tables.device)
-    starts, _, ends, _, row_of, _, positions, _, slots, _ = buf.split_with_sizes(
-        (rows + 1, pr - rows - 1, rows, pr - rows, tokens, pt - tokens, tokens, pt - tokens, tokens, pt - tokens + 4))
+    # one allocation; its last word is the kernel's own
+    buf = torch.empty(3 * tokens + 2 * rows + 2, dtype=torch.int32, device=tables.device)
+    slots, positions, row_of, starts, ends, _ = buf.split_with_sizes((tokens, tokens, tokens, rows + 1, rows, 1))
     at = buf.data_ptr()
-    to = at + 8 * pr
+    to = at + 12 * tokens
     check(cuda_lib().nb_kv_plan(
-        lengths.data_ptr(), new_lens.data_ptr(), tables.data_ptr(), free.data_ptr(), free_count.data_ptr(), free_count_out.data_ptr(), at, at + 4 * pr, to, to + 4 * pt,
-        to + 8 * pt, to + 12 * pt, rows, width, block, free.numel(), tokens, status_ptr(dev), raw_stream()), "kv_plan")
+        lengths.data_ptr(), new_lens.data_ptr(), tables.data_ptr(), free.data_ptr(), free_count.data_ptr(), free_count_out.data_ptr(), to, to + 4 * rows + 4,
+        at + 8 * tokens, at + 4 * tokens, at, to + 8 * rows + 4, rows, width, block, free.numel(), tokens, status_ptr(dev), raw_stream()), "kv_plan")
     return TokenPlan(starts, ends, row_of, positions, slots, free_count_out)
 
 
