@@ -25,6 +25,7 @@ namespace {
 using namespace nb;
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
+constexpr int FEW = 64;                // query rows of a row of the batch and head, up to which this kernel does it in any case
 constexpr int STAGES = 4;              // steps in flight: three ahead of the one in work
 constexpr int LEAD = 2;                // steps that starting a tile costs, in the measure by which the batch is cut
 constexpr int LEAST = 2;               // a piece has at least so many steps
@@ -672,29 +673,6 @@ __global__ void __launch_bounds__(THREADS) kv_attn_join_kernel(const KvAttn p) {
   }
 }
 
-typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeFn encode_fn() {
-  static EncodeFn fn = nullptr;
-  if (!fn) {
-    void* sym = nullptr;
-    cudaDriverEntryPointQueryResult res;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &res) == cudaSuccess && res == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeFn>(sym);
-  }
-  return fn;
-}
-// The codes as [2][blocks * heads * block rows][dim bytes], boxes of 16 rows.
-int make_map(CUtensorMap* m, const KvAttn& p, int dim) {
-  EncodeFn enc = encode_fn();
-  if (!enc) return NB_ERR_NO_DRIVER_SYMBOL;
-  cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)p.kv_rows, 2}, strides[2] = {(cuuint64_t)dim, (cuuint64_t)p.kv_stride};
-  cuuint32_t box[3] = {(cuuint32_t)dim, 16, 1}, one[3] = {1, 1, 1};
-  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(p.codes), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? NB_OK : NB_ERR_TENSORMAP;
-}
-
 template <int D, int NB>
 int launch_few(KvAttn p, cudaStream_t stream) {
   constexpr int fixed = 1024 + WARPS * STAGES * (STAGE + (int)sizeof(Head) + 8);
@@ -708,7 +686,7 @@ int launch_few(KvAttn p, cudaStream_t stream) {
     configured[dev] = true;
   }
   CUtensorMap map;
-  const int rc = make_map(&map, p, D);
+  const int rc = kv_code_map(&map, p, D, 1);
   if (rc) return rc;
   p.tile = 8 * NB;
   p.solo = ((long long)p.width << p.block_log) <= SOLO * Shape<D>::KEYS;
@@ -730,7 +708,39 @@ int launch_few(KvAttn p, cudaStream_t stream) {
 
 }  // namespace
 
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeFn encode_fn() {
+  static EncodeFn fn = nullptr;
+  if (!fn) {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult res;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &res) == cudaSuccess && res == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(sym);
+  }
+  return fn;
+}
+int kv_code_map(CUtensorMap* m, const KvAttn& p, int dim, int swizzled) {
+  EncodeFn enc = encode_fn();
+  if (!enc) return NB_ERR_NO_DRIVER_SYMBOL;
+  cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)p.kv_rows, 2}, strides[2] = {(cuuint64_t)dim, (cuuint64_t)p.kv_stride};
+  cuuint32_t box[3] = {(cuuint32_t)dim, 16, 1}, one[3] = {1, 1, 1};
+  const CUtensorMapSwizzle sw = !swizzled ? CU_TENSOR_MAP_SWIZZLE_NONE : dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(p.codes), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? NB_OK : NB_ERR_TENSORMAP;
+}
+
 extern "C" {
+
+// Selects the kernel of rows with many query rows (tests compare the two): 0 by the rule below, 1 the one that reads codes into
+// the fragments, 2 the tensor cores' one.  Returns the previous setting.
+static int g_mode = 0;
+int nb_kv_attention_mode(int mode) {
+  const int old = g_mode;
+  if (mode >= 0 && mode <= 2) g_mode = mode;
+  return old;
+}
 
 // Pieces that the batch is cut into, and floats of work space that nb_kv_attention needs.
 int nb_kv_attention_pieces(int) { return 148 * WARPS * 3; }
@@ -755,6 +765,7 @@ int nb_kv_attention(const void* q, void* out, const void* codes, const float* sc
   p.q_token = q_token; p.q_head = q_head; p.o_token = o_token; p.o_head = o_head; p.kv_stride = kv_stride; p.s_stride = s_stride;
   p.q_vec = !((reinterpret_cast<uintptr_t>(q) & 15) || (q_token & 7) || (q_head & 7));
   p.o_vec = !((reinterpret_cast<uintptr_t>(out) & 7) || (o_token & 3) || (o_head & 3));
+  p.o_vec16 = !((reinterpret_cast<uintptr_t>(out) & 15) || (o_token & 7) || (o_head & 7));
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.pieces = nb_kv_attention_pieces(dim);
   p.part_o = work;
@@ -763,8 +774,17 @@ int nb_kv_attention(const void* q, void* out, const void* codes, const float* sc
   p.few = 0x7fffffff;
   p.status = status;
   const cudaStream_t s = (cudaStream_t)stream;
+  const int most = max(1, min(max_new, tokens));
+  // Rows with many query rows go to the tensor cores when there are tiles enough to fill the GPU: a tile of 256 query rows walks
+  // its keys alone, while the other kernel spreads the keys of few tiles over all SMs.
+  const long long units = (long long)tokens * p.group / 256 + min(rows, tokens);
+  if (g_mode != 1 && (long long)most * p.group > FEW && (g_mode == 2 || (long long)tokens * p.group / 256 * hk >= 96) && units * hk <= 0x7fffffffLL) {
+    p.few = FEW;
+    const int rc = kv_launch_prompts(p, dim, (int)units, s);
+    if (rc) return rc;
+  }
   // one group of eight query rows where no row of the batch has more; with more, two groups share every conversion of a code
-  const bool one = (long long)min(max_new, tokens) * p.group <= 8;
+  const bool one = min((long long)most * p.group, (long long)p.few) <= 8;
   if (dim == 64) return one ? launch_few<64, 1>(p, s) : launch_few<64, 2>(p, s);
   return one ? launch_few<128, 1>(p, s) : launch_few<128, 2>(p, s);
 }

@@ -1,5 +1,6 @@
 // Parameter blocks of the paged 8-bit cache kernels (kv_cache.cu) and of the attention over it (kv_attention.cu).
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -43,7 +44,7 @@ struct KvAttn {
   const int *tables, *starts, *ends;
   int rows, tokens, hq, hk, group, block_log, blocks, width;
   int kv_rows;                                  // blocks * hk * block
-  int q_vec, o_vec;                             // 16-byte loads of q and 8-byte stores of out are aligned
+  int q_vec, o_vec, o_vec16;                    // 16-byte loads of q, 8- and 16-byte stores of out are aligned
   int few;                                      // rows of the batch with at most this many query rows per head are done here
   int tile;                                     // query rows of a tile
   int pieces, solo;                             // warps; every tile is one warp's
@@ -54,3 +55,8 @@ struct KvAttn {
   int4* part_job;                               // of each piece: the job that it begins and does not end
   unsigned int* status;
 };
+
+// Codes as [2][blocks * heads * block rows][dim bytes], boxes of 16 rows, with the operand swizzle of the row's width or none.
+int kv_code_map(CUtensorMap* map, const KvAttn& p, int dim, int swizzled);
+// Rows of the batch with more than p.few query rows, on the tensor cores (kv_attention_prompt_tcgen05.cu).
+int kv_launch_prompts(const KvAttn& p, int dim, int units, cudaStream_t s);

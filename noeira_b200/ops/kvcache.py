@@ -262,6 +262,13 @@ def paged_attention(q, kv, scale, tables, starts, ends, max_new=None, softmax_sc
     return out
 
 
+def set_attention_mode(mode: int) -> int:
+    """Kernel of rows with more than 64 query rows per head: by problem size (0, default), the one that reads codes straight into the
+    fragments of the matrix instructions and spreads a row's keys over the GPU (1), or the one on 256-row tiles of the tensor
+    cores (2).  Returns the previous setting."""
+    return int(cuda_lib().nb_kv_attention_mode(ctypes.c_int(mode)))
+
+
 _WORK = {}
 
 

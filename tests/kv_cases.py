@@ -47,6 +47,15 @@ ATTENTION = [
     ([3000, 1, 4100], [1, 1, 2], 8, 8, 128, 16),
 ]
 
+# enough query rows for the tensor cores' kernel: tiles of 256 query rows, several of them, ends inside tiles and key blocks
+PROMPTS = [
+    ([0], [513], 8, 8, 64, 16),                                       # exactly one token past two tiles
+    ([0, 40, 0], [256, 255, 900], 12, 12, 64, 16),
+    ([500, 1000], [300, 1], 32, 4, 128, 64),                          # eight heads to one, a single token beside it
+    ([0, 127, 128, 3000], [700, 65, 1, 64], 16, 8, 128, 32),
+    ([129, 0, 7, 900], [900, 0, 16, 33], 24, 8, 64, 128),
+]
+
 
 def attention_inputs(case, seed=0):
     held, new, hq, hk, dim, block = case

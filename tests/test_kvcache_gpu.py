@@ -174,6 +174,100 @@ def test_attention(case):
     assert torch.equal(run_attention(d).view(torch.int16), out.view(torch.int16))
 
 
+def reference(d, q, c):
+    """The definition in 64 bits on the GPU, a row at a time: for cases whose loops in Python would take minutes."""
+    codes, scale = d["codes"].cuda().double(), d["scale"].cuda().double()
+    o, A = torch.zeros(d["T"], d["hq"], d["dim"], dtype=torch.float64, device="cuda"), torch.zeros(d["T"], d["hq"], d["dim"], dtype=torch.float64, device="cuda")
+    st, en, G = d["starts"].tolist(), d["ends"].tolist(), d["hq"] // d["hk"]
+    for i, end in enumerate(en):
+        a, b = st[i], st[i + 1]
+        ids = d["tables"][i, : -(-end // d["block"])].long().cuda()
+        k, v = ((codes[w, ids] * scale[w, ids][..., None, None]).transpose(0, 1).reshape(d["hk"], -1, d["dim"])[:, :end].repeat_interleave(G, 0) for w in (0, 1))
+        see = torch.arange(end, device="cuda")[None] <= (end - (b - torch.arange(a, b, device="cuda")))[:, None]
+        p = torch.softmax((q[a:b].cuda().double().transpose(0, 1) @ k.transpose(1, 2) * c).masked_fill(~see, -math.inf), -1)
+        o[a:b], A[a:b] = (p @ v).transpose(0, 1), (p @ v.abs()).transpose(0, 1)
+    return o.cpu().numpy(), A.cpu().numpy()
+
+
+@pytest.fixture(params=[0, 1, 2], ids=["by_size", "fragments", "tiles"])
+def mode(request):
+    """Runs a test once per kernel that rows with many query rows may get."""
+    from noeira_b200.ops.kvcache import set_attention_mode
+    old = set_attention_mode(request.param)
+    yield request.param
+    set_attention_mode(old)
+
+
+@pytest.mark.parametrize("case", C.PROMPTS + C.ATTENTION[7:])
+def test_attention_prompts(case, mode):
+    d = C.attention_inputs(case)
+    q = d["q"][: d["T"], 1: 1 + d["hq"]]
+    c = d["dim"] ** -0.5
+    want, A = reference(d, q, c)
+    out = run_attention(d)
+    clean()
+    err, most = np.abs(out[: d["T"]].cpu().double().numpy() - want), bound(q, d, want, A, c)
+    assert np.all(err <= most), (err / most).max()
+    assert bool((out[d["T"]:] == 7).all())
+    assert torch.equal(run_attention(d).view(torch.int16), out.view(torch.int16))
+
+
+def test_attention_prompts_scales_padding_and_a_strided_output(mode):
+    """Blocks of very different scales, padded tokens behind the last row, an output whose rows are not 16-byte aligned."""
+    from noeira_b200.ops import kvcache
+    d = C.attention_inputs(([100, 3], [800, 300], 32, 8, 128, 16), seed=4)
+    g = torch.Generator().manual_seed(1)
+    d["scale"] = torch.stack([torch.exp2(torch.randint(-9, -5, d["scale"].shape[1:], generator=g).float()), torch.exp2(torch.randint(-14, 6, d["scale"].shape[1:], generator=g).float())])
+    T = d["T"] + 77
+    q = torch.zeros(T, 32, 128).bfloat16()
+    q[: d["T"]] = d["q"][: d["T"], 1:33]
+    wide = torch.full((T, 32 * 128 + 2), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = wide[:, 1: 1 + 32 * 128].unflatten(1, (32, 128))
+    kvcache.paged_attention(q.cuda(), d["codes"].cuda(), d["scale"].cuda(), d["tables"].cuda(), d["starts"].cuda(), d["ends"].cuda(), max_new=800, softmax_scale=0.11, out=out)
+    clean()
+    assert bool((out[d["T"]:] == 7).all()) and bool((wide[:, 0] == 7).all()) and bool((wide[:, -1] == 7).all())
+    want, A = reference(d, q, 0.11)
+    assert np.all(np.abs(out[: d["T"]].cpu().double().numpy() - want) <= bound(q, d, want, A, 0.11))
+
+
+def test_attention_prompts_nan_reaches_only_who_sees_it(mode):
+    d = C.attention_inputs(([10, 200], [1300, 700], 16, 16, 64, 32))
+    codes = d["codes"].cuda()
+    codes.view(torch.uint8)[1, d["tables"][1, 20].item(), 3, 11, 40] = 0xFF      # a value: row 1, place 651, head 3
+    codes.view(torch.uint8)[1, d["tables"][1, 3].item(), 3, 11, 41] = 0x7F       # another: place 107, all of the row's tokens see it
+    codes.view(torch.uint8)[0, d["tables"][0, 30].item(), 5, 2, 9] = 0x7F        # a key: row 0, place 962, head 5
+    d["codes"] = codes
+    o = run_attention(d)[: d["T"]]
+    clean()
+    bad = torch.zeros_like(o, dtype=torch.bool)
+    bad[1300 + 651 - 200:, 3, 40] = True
+    bad[1300:, 3, 41] = True
+    bad[962 - 10: 1300, 5] = True
+    assert torch.equal(torch.isnan(o), bad)
+
+
+def test_attention_prompts_without_keys_and_with_bad_blocks(mode):
+    from noeira_b200.ops import check_status
+    from noeira_b200.ops.status import DeviceStatusError
+    d = C.attention_inputs(([0, 300], [1500, 700], 12, 12, 64, 16))
+    d["ends"][0] = 1400                              # the first hundred tokens see nothing
+    q = d["q"][: d["T"], 1: 1 + d["hq"]]
+    out = run_attention(d)
+    clean()
+    assert bool((out[:100] == 0).all())
+    tail = dict(d, starts=d["starts"].clone(), ends=d["ends"].clone())
+    want, A = reference(tail, q, 0.125)
+    keep = slice(100, d["T"])
+    assert np.all(np.abs(out[keep].cpu().double().numpy() - want[keep]) <= bound(q, d, want[keep], A[keep], 0.125))
+    for bad in (-1, 1 << 30):
+        e = dict(d, tables=d["tables"].clone())
+        e["tables"][0, 40] = bad
+        again = run_attention(e)
+        with pytest.raises(DeviceStatusError, match="bounds"):
+            check_status()
+        assert torch.equal(again[1500: d["T"]], out[1500: d["T"]])
+
+
 @pytest.mark.parametrize("case", [C.ATTENTION[3], C.ATTENTION[8], C.ATTENTION[10]])
 def test_attention_scales_of_any_size(case):
     """Blocks whose scales differ by 2^20, scores far from zero, another softmax scale."""
