@@ -3,16 +3,23 @@
 // Bound by the matrix products (4 D operations per query row and key), so they run on the tcgen05 tensor cores in bf16.  A CTA owns
 // 256 query rows of one cache head as two 128-row tiles; the query heads that share a cache head are neighbours among the rows
 // (row = token * group + head), so that with grouped heads a tile still fills up, and one K / V tile serves all of them.
-// e4m3 codes times a power-of-two scale are exact in bf16, so a key block is turned into bf16 once per CTA:
+// A code is exact in f16, and turning one into f16 is one instruction for two, so a key block is turned into f16 once per CTA
+// without its scales:
+//   * keys: the scale of each 16 keys multiplies their scores, which the exponent's multiply-add does at no cost;
+//   * queries: bf16 is exact in f16 down to 2^-38 of a row's largest element after a power-of-two scaling of the row;
+//   * values: the weights P carry the scale relative to the largest that the CTA sees, 2^lr, as an addition to the exponent, and
+//     the sum of the weights takes it out again, 16 keys at a time.  f16 weights lose bits below 2^-14; where scales differ by
+//     more than 2^20 the CTA takes values times their scale and P in bf16, which has the exponents.
 //
 //   warp 0       MMA issuer: S_t = Q_t K^T, O_t += P_t V, P from tensor memory (the schedule of attention_fwd2_tcgen05.cu)
 //   warp 1       TMA producer: looks up the blocks of 128 keys a step ahead and brings their codes, 16 rows a copy, into one buffer
 //                for keys and one for values, with the scale of each 16 rows; a block that is none arrives as zeros
-//   warps 4-7    copy Q into the swizzled operand layout, then turn codes into bf16 operand tiles (two stages each), 16 codes a
-//                thread and turn; values behind the last key that any row sees become zeros.  A NaN value would reach rows that do
-//                not see it (0 * NaN), so it becomes zero too, and the first key with a NaN is noted per dimension: a row sees a
-//                prefix of the keys, so its output is NaN exactly where that key is in its prefix
-//   warps 8-15   softmax, a thread per query row, 128 scores in registers, running maximum and sum
+//   warps 2, 3   turn codes into operand tiles (two stages each), 16 codes a thread and turn; values behind the last key that any
+//                row sees become zeros.  A NaN value would reach rows that do not
+//                see it (0 * NaN), so in blocks that some row sees in part it becomes zero too, and the first key with a NaN is
+//                noted per dimension: a row sees a prefix of the keys, so its output is NaN where that key is in its prefix
+//   warps 4-11   copy Q into the swizzled operand layout, then softmax: a thread per query row, 128 scores in registers, running
+//                maximum and sum
 #include <cuda.h>
 
 #include <type_traits>
@@ -33,37 +40,50 @@ using nbattn::pack2;
 using nbattn::umma_commit_a;
 using nbattn::unpack2;
 
-constexpr int BQ = 128, BKV = 128, KS = 2, THREADS = 512;
+constexpr int BQ = 128, BKV = 128, KS = 2, THREADS = 384, CONV = 64;   // CONV: threads that turn codes
 // The registers of the launch, moved between the warpgroups; an increase waits until the block's own share has them.
-static_assert(128 * 56 + 128 * 72 + 256 * 192 <= THREADS * 128, "register split");
+static_assert(128 * 88 + 256 * 208 <= THREADS * 168, "register split");
 
-// P = 2^(s * mult - m) of half a row as packed bf16 into tensor memory; returns the half's sum.
+// P = 2^(s f_c - m + lr_c) of half a row, f_c and lr_c of the 16 keys of group c, packed into tensor memory; returns the half's sum
+// of 2^(s f_c - m).
 template <int HALF>
-__device__ __forceinline__ float exp_store(const float (&s)[128], float mult, float m_use, uint32_t s_addr) {
-  uint64_t sum = pack2(0.f, 0.f);
-  const uint64_t mult2 = pack2(mult, mult), negm2 = pack2(-m_use, -m_use);
+__device__ __forceinline__ float exp_store(const float (&s)[128], float row, float m_use, bool bf, const float* group, uint32_t s_addr) {
+  float total = 0.f;
 #pragma unroll
   for (int c = HALF * 4; c < HALF * 4 + 4; ++c) {
+    const float mult = fmaxf(row * group[c], 1.2e-38f), lr = bf ? 0.f : group[8 + c];   // not zero, which would make a masked -inf a NaN
+    const uint64_t mult2 = pack2(mult, mult), add = pack2(lr - m_use, lr - m_use);
+    uint64_t sum = pack2(0.f, 0.f);
+    float e[16];
     uint32_t pk[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      float e0, e1;
-      unpack2(fma2(pack2(s[c * 16 + 2 * u], s[c * 16 + 2 * u + 1]), mult2, negm2), e0, e1);
-      e0 = exp2_fast(e0);
-      e1 = exp2_fast(e1);
-      sum = add2(sum, pack2(e0, e1));
-      const __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
-      pk[u] = *reinterpret_cast<const uint32_t*>(&h);
+      unpack2(fma2(pack2(s[c * 16 + 2 * u], s[c * 16 + 2 * u + 1]), mult2, add), e[2 * u], e[2 * u + 1]);
+      e[2 * u] = exp2_fast(e[2 * u]);
+      e[2 * u + 1] = exp2_fast(e[2 * u + 1]);
+      sum = add2(sum, pack2(e[2 * u], e[2 * u + 1]));
     }
+    if (bf) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(pk[u]) : "f"(e[2 * u + 1]), "f"(e[2 * u]));
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[u]) : "f"(e[2 * u + 1]), "f"(e[2 * u]));
+    }
+    float a, b;
+    unpack2(sum, a, b);
+    total = fmaf(a + b, bf ? 1.f : group[16 + c], total);
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(s_addr + c * 8), "r"(pk[0]), "r"(pk[1]), "r"(pk[2]),
                  "r"(pk[3]), "r"(pk[4]), "r"(pk[5]), "r"(pk[6]), "r"(pk[7])
                  : "memory");
   }
-  float a, b;
-  unpack2(sum, a, b);
-  return a + b;
+  return total;
 }
 
+// four codes as two f16 pairs
+__device__ __forceinline__ void f16_of_codes(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
 // two codes (bits 0..15) times a scale, as bf16 pair
 __device__ __forceinline__ uint32_t bf16_of_codes(uint32_t two, float scale) {
   uint32_t h2;
@@ -84,7 +104,7 @@ template <int HD>
 struct Smem {
   static constexpr int Q = BQ * HD * 2, KV = BKV * HD * 2, RAW = BKV * HD;
   static constexpr int OFF_K = 2 * Q, OFF_V = OFF_K + KS * KV, OFF_RAW = OFF_V + KS * KV, OFF_SC = OFF_RAW + 2 * RAW;
-  static constexpr int OFF_NAN = OFF_SC + 64, OFF_BAR = OFF_NAN + HD * 4, BARS = 1 + 4 + 4 * KS + 8, OFF_MISC = OFF_BAR + BARS * 8;
+  static constexpr int OFF_QF = OFF_SC + 4 * 32 * 4, OFF_NAN = OFF_QF + 2 * BQ, OFF_BAR = OFF_NAN + HD * 4, BARS = 1 + 4 + 4 * KS + 8, OFF_MISC = OFF_BAR + BARS * 8;
   static constexpr int TOTAL = OFF_MISC + 160 + 1024;
   static_assert(TOTAL <= 232448, "shared memory");
 };
@@ -92,11 +112,12 @@ struct Smem {
 template <int HD>
 __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid_constant__ CUtensorMap map, const KvAttn p) {
   using S = Smem<HD>;
-  constexpr int NSUB = HD / 64;
-  constexpr float RESCALE_THRESHOLD = 8.f;
+  constexpr float RESCALE_THRESHOLD = 4.f, LIFT = 11.f;   // weights are at most 2^15, below f16's largest
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* s_scale = reinterpret_cast<float*>(smem + S::OFF_SC);      // [2][8] of 16 key rows each
+  // of the last four key blocks, for each 16 keys: scale of the keys [8], lr [8], 2^-lr [8], scale of the values [8]
+  float* s_group = reinterpret_cast<float*>(smem + S::OFF_SC);
+  signed char* s_qe = reinterpret_cast<signed char*>(smem + S::OFF_QF);   // [2 BQ] exponent by which a query row was scaled down
   int* s_nan = reinterpret_cast<int*>(smem + S::OFF_NAN);           // [HD] first key with a NaN value
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
   int* misc = reinterpret_cast<int*>(smem + S::OFF_MISC);           // [0] tensor memory, [1] abort, [2] any NaN, [3..5] the CTA's tile, [8..23] sums
@@ -122,6 +143,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
   if (threadIdx.x == 0) {
     misc[1] = misc[2] = 0;
     misc[3] = -1;
+    misc[6] = 0;                       // largest scale of the values (its bits), smallest that is not zero
+    misc[7] = 0x7f800000;
   }
   if (threadIdx.x < HD) s_nan[threadIdx.x] = 0x7fffffff;
   __syncthreads();
@@ -157,15 +180,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
   auto p_full = [&](int t) { return aB + 8u * (9 + 4 * KS + t); };
   auto o_done = [&](int t) { return aB + 8u * (11 + 4 * KS + t); };
   if (threadIdx.x == 0) {
-    mbar_init(&bars[0], 4);
+    mbar_init(&bars[0], 8);
     for (int w = 0; w < 2; ++w) {
       mbar_init(&bars[1 + w], 1);
-      mbar_init(&bars[3 + w], 4);
+      mbar_init(&bars[3 + w], CONV / 32);
     }
     for (int i = 0; i < KS; ++i) {
-      mbar_init(&bars[5 + i], 4);
+      mbar_init(&bars[5 + i], CONV / 32);
       mbar_init(&bars[5 + KS + i], 1);
-      mbar_init(&bars[5 + 2 * KS + i], 4);
+      mbar_init(&bars[5 + 2 * KS + i], CONV / 32);
       mbar_init(&bars[5 + 3 * KS + i], 1);
     }
     for (int t = 0; t < 2; ++t) {
@@ -195,13 +218,26 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
 #pragma unroll
   for (int t = 0; t < 2; ++t) nkb[t] = tile0 + t * BQ < qrows ? ceil_div(sees(min(tile0 + (t + 1) * BQ, qrows) - 1), BKV) : 0;
   const int nmax = max(nkb[0], nkb[1]);
-  const int seen = sees(min(tile0 + 2 * BQ, qrows) - 1);            // the most that a row of this CTA sees
+  const int seen = sees(min(tile0 + 2 * BQ, qrows) - 1), sure = sees(tile0);   // the most that a row of this CTA sees, and the fewest
+
+  // scales of the values that this CTA will see
+  for (int pg = threadIdx.x; (long long)pg << p.block_log < seen; pg += THREADS) {
+    const int b = p.tables[(long long)row * p.width + pg];
+    const float v = (unsigned)b < (unsigned)p.blocks ? p.scale[p.s_stride + b * p.hk + head] : 0.f;
+    if (v > 0.f) {
+      atomicMax(&misc[6], __float_as_int(v));
+      atomicMin(&misc[7], __float_as_int(v));
+    }
+  }
+  __syncthreads();
+  const float vref = __int_as_float(misc[6]) > 0.f ? __int_as_float(misc[6]) : 1.f;
+  const bool bf = __int_as_float(misc[7]) * 1048576.f < vref;
 
   if (warp == 0) {
     // ---------------------------------------------------------------- MMA issuer
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (elect_one()) {
-      const uint32_t idesc_s = make_idesc(1u, BQ, BKV, 0u, 0u), idesc_o = make_idesc(1u, BQ, HD, 0u, 1u);
+      const uint32_t idesc_s = make_idesc(0u, BQ, BKV, 0u, 0u), idesc_o = make_idesc(bf ? 1u : 0u, BQ, HD, 0u, 1u);
       bool ok = nmax == 0 || mbar_wait_a(q_full, 0u, p.status, 410);
       auto issue_s = [&](int t, int j) -> bool {
         const int st = j % KS;
@@ -249,7 +285,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- codes: lane l < 8 brings key rows 16 l .. of each step
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     const int* table = p.tables + (long long)row * p.width;
     int src = p.kv_rows;
     float ks = 0.f, vs = 0.f;
@@ -280,7 +316,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
       for (int w = 0; w < 2; ++w) {
         ok = ok && __all_sync(0xffffffffu, !*abort_flag && mbar_wait_a(raw_empty(w), ((uint32_t)j & 1u) ^ 1u, p.status, 420 + w));
         if (!ok) break;
-        if (lane < 8) s_scale[w * 8 + lane] = sc[w];
+        if (w == 0 && lane < 8) {      // block j - 4 is done: its successor's keys wait for its softmax
+          float* g = s_group + (j & 3) * 32 + lane;
+          const float lr = sc[1] > 0.f ? fmaxf(log2f(sc[1] / vref), -40.f) : -40.f;
+          g[0] = sc[0];
+          g[8] = lr;
+          g[16] = exp2f(-lr);
+          g[24] = sc[1];
+        }
         __syncwarp();
         if (lane == 0) mbar_expect_tx_a(raw_full(w), S::RAW);
         __syncwarp();
@@ -296,72 +339,78 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
     for (int w = 0; w < 2; ++w)
       if (issued[w] > 0) mbar_wait_a(raw_full(w), (uint32_t)(issued[w] - 1) & 1u, p.status, 422);
   } else if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-  } else if (warp < 8) {
     // ---------------------------------------------------------------- operands
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    const int tid = threadIdx.x - 128;
-    for (int i = tid; i < 2 * BQ * (HD / 8); i += 128) {
-      const int r = i / (HD / 8), ch = i % (HD / 8), q = tile0 + r;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (q < qrows) {
-        const int tok = q / p.group;
-        const __nv_bfloat16* a = (const __nv_bfloat16*)p.q + (long long)(first + tok) * p.q_token + (long long)(head * p.group + q - tok * p.group) * p.q_head + ch * 8;
-        if (p.q_vec) {
-          w = *reinterpret_cast<const uint4*>(a);
-        } else {
-          const unsigned short* e = reinterpret_cast<const unsigned short*>(a);
-          w = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
-        }
-      }
-      *reinterpret_cast<uint4*>(smem + (r / BQ) * S::Q + (ch / 8) * (BQ * 128) + (r % BQ) * 128 + (((ch & 7) ^ (r & 7)) << 4)) = w;
-    }
-    fence_proxy_async();
-    __syncwarp();
-    if (lane == 0) mbar_arrive_a(q_full);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    const int tid = threadIdx.x - 64;
     constexpr int CH = HD / 16;        // 16-code chunks of a key row
     for (int j = 0; j < nmax; ++j) {
       const int st = j % KS;
       bool ok = true;
-#pragma unroll
+#pragma unroll 1
       for (int w = 0; w < 2; ++w) {
         ok = ok && __all_sync(0xffffffffu, !*abort_flag && mbar_wait_a(raw_full(w), (uint32_t)j & 1u, p.status, 430 + w) &&
                                                mbar_wait_a(w ? v_empty(st) : k_empty(st), ((uint32_t)(j / KS) & 1u) ^ 1u, p.status, 432 + w));
         if (!ok) break;
         const uint8_t* raw = smem + S::OFF_RAW + w * S::RAW;
         uint8_t* to = smem + (w ? S::OFF_V : S::OFF_K) + st * S::KV;
-#pragma unroll 2
-        for (int i = tid; i < BKV * CH; i += 128) {
-          const int r = i / CH, c = i % CH;
-          const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 16);
-          uint32_t cw[4] = {x.x, x.y, x.z, x.w};
-          if (w == 1) {
-            if (j * BKV + r >= seen) cw[0] = cw[1] = cw[2] = cw[3] = 0;
-            if (nan_code(cw[0]) | nan_code(cw[1]) | nan_code(cw[2]) | nan_code(cw[3])) {
-              misc[2] = 1;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t bad = nan_code(cw[e]) >> 7;
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
-                  if ((bad >> (8 * b)) & 1u) atomicMin(&s_nan[c * 16 + e * 4 + b], j * BKV + r);
-                cw[e] &= ~(bad * 0xffu);
-              }
-            }
-          }
-          const float sc = s_scale[w * 8 + (r >> 4)];
-          uint32_t o[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            o[2 * e] = bf16_of_codes(cw[e] & 0xffffu, sc);
-            o[2 * e + 1] = bf16_of_codes(cw[e] >> 16, sc);
-          }
-          // 32 bytes as two chunks; the halves of a 128-wide row in opposite order, so that eight lanes write eight different chunks
+        const bool part = w == 1 && (j + 1) * BKV > sure;           // some row sees only some of the keys
+        // 32 bytes of a chunk as two; the halves of a 128-wide row in opposite order, so that eight lanes write eight different places
+        auto put = [&](int r, int c, const uint32_t (&o)[8]) {
           uint8_t* line = to + (c / 4) * (BKV * 128) + r * 128;
           const int ch = (c & 3) * 2, flip = c / 4;
           const uint4 lo4 = make_uint4(o[0], o[1], o[2], o[3]), hi4 = make_uint4(o[4], o[5], o[6], o[7]);
           *reinterpret_cast<uint4*>(line + (((ch + flip) ^ (r & 7)) << 4)) = flip ? hi4 : lo4;
           *reinterpret_cast<uint4*>(line + (((ch + (flip ^ 1)) ^ (r & 7)) << 4)) = flip ? lo4 : hi4;
+        };
+        if (!part && !(w == 1 && bf)) {
+          // rows of this thread are CONV / CH apart, its chunk is always the same
+#pragma unroll 1
+          for (int i0 = 0; i0 < BKV * CH / CONV; i0 += 4) {
+            uint4 x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const uint4*>(raw + ((i0 + e) * CONV + tid) * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t o[8];
+              f16_of_codes(x[e].x, o[0], o[1]);
+              f16_of_codes(x[e].y, o[2], o[3]);
+              f16_of_codes(x[e].z, o[4], o[5]);
+              f16_of_codes(x[e].w, o[6], o[7]);
+              put((i0 + e) * (CONV / CH) + tid / CH, tid % CH, o);
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int i = tid; i < BKV * CH; i += CONV) {
+            const int r = i / CH, c = i % CH;
+            const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 16);
+            uint32_t cw[4] = {x.x, x.y, x.z, x.w}, o[8];
+            if (part) {
+              if (j * BKV + r >= seen) cw[0] = cw[1] = cw[2] = cw[3] = 0;
+              if (nan_code(cw[0]) | nan_code(cw[1]) | nan_code(cw[2]) | nan_code(cw[3])) {
+                misc[2] = 1;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t bad = nan_code(cw[e]) >> 7;
+#pragma unroll
+                  for (int b = 0; b < 4; ++b)
+                    if ((bad >> (8 * b)) & 1u) atomicMin(&s_nan[c * 16 + e * 4 + b], j * BKV + r);
+                  cw[e] &= ~(bad * 0xffu);
+                }
+              }
+            }
+            const float sc = s_group[(j & 3) * 32 + 24 + (r >> 4)];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (w == 1 && bf) {
+                o[2 * e] = bf16_of_codes(cw[e] & 0xffffu, sc);
+                o[2 * e + 1] = bf16_of_codes(cw[e] >> 16, sc);
+              } else {
+                f16_of_codes(cw[e], o[2 * e], o[2 * e + 1]);
+              }
+            }
+            put(r, c, o);
+          }
         }
         fence_proxy_async();
         __syncwarp();
@@ -377,47 +426,83 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
     }
   } else {
     // ---------------------------------------------------------------- softmax and output: one thread per query row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-    const int t = (warp - 8) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int t = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+#pragma unroll 4
+    for (int i = threadIdx.x - 128 - t * 128; i < BQ * (HD / 8); i += 128) {
+      const int qr = i / (HD / 8), ch = i % (HD / 8), q = tile0 + t * BQ + qr;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (q < qrows) {
+        const int tok = q / p.group;
+        const __nv_bfloat16* a = (const __nv_bfloat16*)p.q + (long long)(first + tok) * p.q_token + (long long)(head * p.group + q - tok * p.group) * p.q_head + ch * 8;
+        if (p.q_vec) {
+          w = *reinterpret_cast<const uint4*>(a);
+        } else {
+          const unsigned short* e = reinterpret_cast<const unsigned short*>(a);
+          w = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
+        }
+      }
+      // power of two that takes the row's largest element to [2^14, 2^15)
+      uint32_t x[4] = {w.x, w.y, w.z, w.w};
+      float top = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(x[e] << 16)), fabsf(__uint_as_float(x[e] & 0xffff0000u))));
+#pragma unroll
+      for (int o = HD / 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      int e2 = (int)(__float_as_uint(top) >> 23) - 127;
+      e2 = top > 0.f && e2 < 128 ? max(-100, min(112, e2 - 14)) : 0;
+      const float by = __uint_as_float((uint32_t)(127 - e2) << 23);
+      if (ch == 0) s_qe[t * BQ + qr] = (signed char)e2;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = __uint_as_float(x[e] << 16) * by, b = __uint_as_float(x[e] & 0xffff0000u) * by;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(x[e]) : "f"(b), "f"(a));
+      }
+      *reinterpret_cast<uint4*>(smem + t * S::Q + (ch / 8) * (BQ * 128) + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive_a(q_full);
     const int q = tile0 + t * BQ + r, n = nkb[t];
     const int lim = q < qrows ? sees(q) : 0;
     const uint32_t s_addr = tmem + ((uint32_t)(quarter * 32) << 16) + t * 128, o_addr = s_addr - t * 128 + 256 + t * 128;
     float m_ref = -INFINITY, l = 0.f;
     bool ok = true;
-    // MODE 0: every real row of the tile sees the whole block; MODE 1: a row sees a prefix of it
-    auto block = [&](int j, auto mode_tag) -> bool {
-      constexpr int MODE = decltype(mode_tag)::value;
+    float qf = 0.f;
+    // One key block, in one place: a variant per kind of mask or of P would not fit the instruction cache beside the others.
+    auto block = [&](int j, bool whole) -> bool {
       if (!__all_sync(0xffffffffu, !*abort_flag && mbar_wait_a(s_full(t), (uint32_t)j & 1u, p.status, 440))) return false;
       tc_fence_after();
       float s[128];
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32_nowait(s_addr + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
       tmem_ld_wait();
-      if (MODE == 1) {
+      if (!whole) {                    // a row sees a prefix of the block
         const int see = lim - j * BKV;
 #pragma unroll
         for (int i = 0; i < 128; ++i) s[i] = i < see ? s[i] : -INFINITY;
       }
-      float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+      const float* group = s_group + (j & 3) * 32;
+      float mx = -INFINITY;
 #pragma unroll
-      for (int i = 4; i < 124; i += 8) {
-        m0 = max3(m0, s[i], s[i + 1]);
-        m1 = max3(m1, s[i + 2], s[i + 3]);
-        m2 = max3(m2, s[i + 4], s[i + 5]);
-        m3 = max3(m3, s[i + 6], s[i + 7]);
+      for (int c = 0; c < 8; ++c) {
+        float m0 = max3(s[c * 16], s[c * 16 + 1], s[c * 16 + 2]), m1 = max3(s[c * 16 + 3], s[c * 16 + 4], s[c * 16 + 5]);
+        m0 = max3(m0, s[c * 16 + 6], s[c * 16 + 7]);
+        m1 = max3(m1, s[c * 16 + 8], s[c * 16 + 9]);
+        m0 = max3(m0, s[c * 16 + 10], s[c * 16 + 11]);
+        m1 = max3(m1, s[c * 16 + 12], s[c * 16 + 13]);
+        m0 = max3(m0, s[c * 16 + 14], s[c * 16 + 15]);
+        mx = fmaxf(mx, fmaxf(m0, m1) * fmaxf(qf * group[c], 1.2e-38f));
       }
-      m0 = max3(m0, s[124], s[125]);
-      m1 = max3(m1, s[126], s[127]);
-      const float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * p.scale_log2;
       float alpha = 1.f;
       const bool grow = mx > m_ref + RESCALE_THRESHOLD || (m_ref == -INFINITY && mx > -INFINITY);
       if (grow) {
         alpha = exp2_fast(m_ref - mx);
         m_ref = mx;
       }
-      const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+      const float m_use = (m_ref == -INFINITY ? 0.f : m_ref) - LIFT;
       if (j > 0 && __any_sync(0xffffffffu, grow)) {
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
           uint32_t o[32];
           tmem_ld_32x32b_x32(o_addr + c, o);
@@ -427,12 +512,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
           tmem_st_32x32b_x32(o_addr + c, o);
         }
       }
-      float sum = exp_store<0>(s, p.scale_log2, m_use, s_addr);
+      float sum = exp_store<0>(s, qf, m_use, bf, group, s_addr);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_a(p_lo(t));
-      sum += exp_store<1>(s, p.scale_log2, m_use, s_addr);
+      sum += exp_store<1>(s, qf, m_use, bf, group, s_addr);
       l = l * alpha + sum;
       tmem_st_wait();
       tc_fence_before();
@@ -441,20 +526,21 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
       return true;
     };
     const int whole = n > 0 ? min(n, sees(tile0 + t * BQ) / BKV) : 0;
-    int j = 0;
+    if (n > 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait_a(q_full, 0u, p.status, 442));
+      qf = p.scale_log2 * __uint_as_float((uint32_t)(127 + s_qe[t * BQ + r]) << 23);   // what a raw score is multiplied by
+    }
 #pragma unroll 1
-    for (; j < whole && ok; ++j) ok = block(j, std::integral_constant<int, 0>{});
-#pragma unroll 1
-    for (; j < n && ok; ++j) ok = block(j, std::integral_constant<int, 1>{});
+    for (int j = 0; j < n && ok; ++j) ok = block(j, j < whole);
     if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait_a(o_done(t), 0u, p.status, 441));
     if (!ok) *abort_flag = 1;
     if (ok && tile0 + t * BQ < qrows) {
       tc_fence_after();
-      const float inv = l == 0.f ? 0.f : 1.f / l;                    // NaN stays NaN
+      const float inv = l == 0.f ? 0.f : (bf ? 1.f : vref) / l;      // NaN stays NaN
       const bool any_nan = misc[2] != 0;
       const int qc = min(q, qrows - 1), tok = qc / p.group;
       __nv_bfloat16* orow = (__nv_bfloat16*)p.out + (long long)(first + tok) * p.o_token + (long long)(head * p.group + qc - tok * p.group) * p.o_head;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         uint32_t o[32];
         if (n > 0) {
