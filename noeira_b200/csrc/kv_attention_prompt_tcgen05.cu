@@ -47,12 +47,14 @@ static_assert(128 * 88 + 256 * 208 <= THREADS * 168, "register split");
 // P = 2^(s f_c - m + lr_c) of half a row, f_c and lr_c of the 16 keys of group c, packed into tensor memory; returns the half's sum
 // of 2^(s f_c - m).
 template <int HALF>
-__device__ __forceinline__ float exp_store(const float (&s)[128], float row, float m_use, bool bf, const float* group, uint32_t s_addr) {
+__device__ __forceinline__ float exp_store(const float (&s)[128], const float (&f)[8], float m_use, bool bf, const float4* group, uint32_t s_addr) {
   float total = 0.f;
+  const float4 lr4 = group[2 + HALF], back4 = group[4 + HALF];
+  const float lrs[4] = {lr4.x, lr4.y, lr4.z, lr4.w}, backs[4] = {back4.x, back4.y, back4.z, back4.w};
 #pragma unroll
   for (int c = HALF * 4; c < HALF * 4 + 4; ++c) {
-    const float mult = fmaxf(row * group[c], 1.2e-38f), lr = bf ? 0.f : group[8 + c];   // not zero, which would make a masked -inf a NaN
-    const uint64_t mult2 = pack2(mult, mult), add = pack2(lr - m_use, lr - m_use);
+    const float add1 = (bf ? 0.f : lrs[c % 4]) - m_use;
+    const uint64_t mult2 = pack2(f[c], f[c]), add = pack2(add1, add1);
     uint64_t sum = pack2(0.f, 0.f);
     float e[16];
     uint32_t pk[8];
@@ -72,7 +74,7 @@ __device__ __forceinline__ float exp_store(const float (&s)[128], float row, flo
     }
     float a, b;
     unpack2(sum, a, b);
-    total = fmaf(a + b, bf ? 1.f : group[16 + c], total);
+    total = fmaf(a + b, bf ? 1.f : backs[c % 4], total);
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(s_addr + c * 8), "r"(pk[0]), "r"(pk[1]), "r"(pk[2]),
                  "r"(pk[3]), "r"(pk[4]), "r"(pk[5]), "r"(pk[6]), "r"(pk[7])
                  : "memory");
@@ -428,37 +430,45 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
     // ---------------------------------------------------------------- softmax and output: one thread per query row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int t = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
-#pragma unroll 4
-    for (int i = threadIdx.x - 128 - t * 128; i < BQ * (HD / 8); i += 128) {
-      const int qr = i / (HD / 8), ch = i % (HD / 8), q = tile0 + t * BQ + qr;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (q < qrows) {
-        const int tok = q / p.group;
-        const __nv_bfloat16* a = (const __nv_bfloat16*)p.q + (long long)(first + tok) * p.q_token + (long long)(head * p.group + q - tok * p.group) * p.q_head + ch * 8;
-        if (p.q_vec) {
-          w = *reinterpret_cast<const uint4*>(a);
-        } else {
-          const unsigned short* e = reinterpret_cast<const unsigned short*>(a);
-          w = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
+    {
+      constexpr int LANES = HD / 8, STEP = 128 / LANES, BATCH = 8;   // lanes of a query row, rows of a turn, turns whose loads go out together
+      const int tid = threadIdx.x - 128 - t * 128, ch = tid % LANES;
+#pragma unroll 1
+      for (int r0 = tid / LANES; r0 < BQ; r0 += STEP * BATCH) {
+        uint4 w[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+          const int q = tile0 + t * BQ + r0 + u * STEP, tok = q / p.group;
+          const __nv_bfloat16* a = (const __nv_bfloat16*)p.q + (long long)(first + tok) * p.q_token + (long long)(head * p.group + q - tok * p.group) * p.q_head + ch * 8;
+          w[u] = make_uint4(0, 0, 0, 0);
+          if (q < qrows && p.q_vec) w[u] = *reinterpret_cast<const uint4*>(a);
+          if (q < qrows && !p.q_vec) {
+            const unsigned short* e = reinterpret_cast<const unsigned short*>(a);
+            w[u] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+          // power of two that takes the row's largest element to [2^14, 2^15)
+          const int qr = r0 + u * STEP;
+          uint32_t x[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+          float top = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(x[e] << 16)), fabsf(__uint_as_float(x[e] & 0xffff0000u))));
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          int e2 = (int)(__float_as_uint(top) >> 23) - 127;
+          e2 = top > 0.f && e2 < 128 ? max(-100, min(112, e2 - 14)) : 0;
+          const float by = __uint_as_float((uint32_t)(127 - e2) << 23);
+          if (ch == 0) s_qe[t * BQ + qr] = (signed char)e2;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = __uint_as_float(x[e] << 16) * by, b = __uint_as_float(x[e] & 0xffff0000u) * by;
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(x[e]) : "f"(b), "f"(a));
+          }
+          *reinterpret_cast<uint4*>(smem + t * S::Q + (ch / 8) * (BQ * 128) + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
         }
       }
-      // power of two that takes the row's largest element to [2^14, 2^15)
-      uint32_t x[4] = {w.x, w.y, w.z, w.w};
-      float top = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(x[e] << 16)), fabsf(__uint_as_float(x[e] & 0xffff0000u))));
-#pragma unroll
-      for (int o = HD / 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      int e2 = (int)(__float_as_uint(top) >> 23) - 127;
-      e2 = top > 0.f && e2 < 128 ? max(-100, min(112, e2 - 14)) : 0;
-      const float by = __uint_as_float((uint32_t)(127 - e2) << 23);
-      if (ch == 0) s_qe[t * BQ + qr] = (signed char)e2;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float a = __uint_as_float(x[e] << 16) * by, b = __uint_as_float(x[e] & 0xffff0000u) * by;
-        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(x[e]) : "f"(b), "f"(a));
-      }
-      *reinterpret_cast<uint4*>(smem + t * S::Q + (ch / 8) * (BQ * 128) + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
     }
     fence_proxy_async();
     __syncwarp();
@@ -482,7 +492,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
 #pragma unroll
         for (int i = 0; i < 128; ++i) s[i] = i < see ? s[i] : -INFINITY;
       }
-      const float* group = s_group + (j & 3) * 32;
+      const float4* group = reinterpret_cast<const float4*>(s_group + (j & 3) * 32);
+      const float4 ks0 = group[0], ks1 = group[1];
+      float f[8] = {ks0.x, ks0.y, ks0.z, ks0.w, ks1.x, ks1.y, ks1.z, ks1.w};
       float mx = -INFINITY;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
@@ -492,7 +504,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
         m0 = max3(m0, s[c * 16 + 10], s[c * 16 + 11]);
         m1 = max3(m1, s[c * 16 + 12], s[c * 16 + 13]);
         m0 = max3(m0, s[c * 16 + 14], s[c * 16 + 15]);
-        mx = fmaxf(mx, fmaxf(m0, m1) * fmaxf(qf * group[c], 1.2e-38f));
+        f[c] = fmaxf(qf * f[c], 1.2e-38f);                          // not zero, which would make a masked -inf a NaN
+        mx = fmaxf(mx, fmaxf(m0, m1) * f[c]);
       }
       float alpha = 1.f;
       const bool grow = mx > m_ref + RESCALE_THRESHOLD || (m_ref == -INFINITY && mx > -INFINITY);
@@ -512,12 +525,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
           tmem_st_32x32b_x32(o_addr + c, o);
         }
       }
-      float sum = exp_store<0>(s, qf, m_use, bf, group, s_addr);
+      float sum = exp_store<0>(s, f, m_use, bf, group, s_addr);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_a(p_lo(t));
-      sum += exp_store<1>(s, qf, m_use, bf, group, s_addr);
+      sum += exp_store<1>(s, f, m_use, bf, group, s_addr);
       l = l * alpha + sum;
       tmem_st_wait();
       tc_fence_before();
