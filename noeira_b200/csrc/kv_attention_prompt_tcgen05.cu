@@ -46,14 +46,14 @@ static_assert(128 * 88 + 256 * 208 <= THREADS * 168, "register split");
 
 // P = 2^(s f_c - m + lr_c) of half a row, f_c and lr_c of the 16 keys of group c, packed into tensor memory; returns the half's sum
 // of 2^(s f_c - m).
-template <int HALF>
-__device__ __forceinline__ float exp_store(const float (&s)[128], const float (&f)[8], float m_use, bool bf, const float4* group, uint32_t s_addr) {
+template <int HALF, bool BF>
+__device__ __forceinline__ float exp_store(const float (&s)[128], const float (&f)[8], float m_use, const float4* group, uint32_t s_addr) {
   float total = 0.f;
   const float4 lr4 = group[2 + HALF], back4 = group[4 + HALF];
   const float lrs[4] = {lr4.x, lr4.y, lr4.z, lr4.w}, backs[4] = {back4.x, back4.y, back4.z, back4.w};
 #pragma unroll
   for (int c = HALF * 4; c < HALF * 4 + 4; ++c) {
-    const float add1 = (bf ? 0.f : lrs[c % 4]) - m_use;
+    const float add1 = (BF ? 0.f : lrs[c % 4]) - m_use;
     const uint64_t mult2 = pack2(f[c], f[c]), add = pack2(add1, add1);
     uint64_t sum = pack2(0.f, 0.f);
     float e[16];
@@ -65,7 +65,7 @@ __device__ __forceinline__ float exp_store(const float (&s)[128], const float (&
       e[2 * u + 1] = exp2_fast(e[2 * u + 1]);
       sum = add2(sum, pack2(e[2 * u], e[2 * u + 1]));
     }
-    if (bf) {
+    if (BF) {
 #pragma unroll
       for (int u = 0; u < 8; ++u) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(pk[u]) : "f"(e[2 * u + 1]), "f"(e[2 * u]));
     } else {
@@ -74,7 +74,7 @@ __device__ __forceinline__ float exp_store(const float (&s)[128], const float (&
     }
     float a, b;
     unpack2(sum, a, b);
-    total = fmaf(a + b, bf ? 1.f : backs[c % 4], total);
+    total = BF ? total + (a + b) : fmaf(a + b, backs[c % 4], total);
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(s_addr + c * 8), "r"(pk[0]), "r"(pk[1]), "r"(pk[2]),
                  "r"(pk[3]), "r"(pk[4]), "r"(pk[5]), "r"(pk[6]), "r"(pk[7])
                  : "memory");
@@ -126,22 +126,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
   volatile int* abort_flag = misc + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // ---------------------------------------------------------------- which rows: the batch's tiles in reverse, the long ones of a row first
-  int tiles_mine = 0;
-  const int per = ceil_div(p.rows, THREADS), lo = min(p.rows, (int)threadIdx.x * per), hi = min(p.rows, lo + per);
+  // ---------------------------------------------------------------- which rows: long ones first, and of a row the tiles that see most
   auto tiles_of = [&](int i) {
     const int first = p.starts[i];
     const long long n = first < 0 ? 0 : (long long)min(p.starts[i + 1], p.tokens) - first;
     return n * p.group <= p.few ? 0 : (int)((n * p.group + 2 * BQ - 1) / (2 * BQ));
   };
-  for (int i = lo; i < hi; ++i) tiles_mine += tiles_of(i);
-  int upto = tiles_mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += u;
-  }
-  if (lane == 31) misc[8 + warp] = upto;
+  const int unit = blockIdx.x / p.hk, head = blockIdx.x % p.hk;
   if (threadIdx.x == 0) {
     misc[1] = misc[2] = 0;
     misc[3] = -1;
@@ -149,26 +140,52 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
     misc[7] = 0x7f800000;
   }
   if (threadIdx.x < HD) s_nan[threadIdx.x] = 0x7fffffff;
-  __syncthreads();
-  int total = 0;
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) upto += misc[8 + w];
-    total += misc[8 + w];
-  }
-  const int want = total - 1 - (int)(blockIdx.x / p.hk), head = blockIdx.x % p.hk;
-  if (want < 0) return;                // the grid is an upper bound
-  if (want >= upto - tiles_mine && want < upto) {
-    int at = upto - tiles_mine;
-    for (int i = lo; i < hi; ++i) {
+  if (p.rows <= THREADS) {
+    // a thread per row: the tiles of all rows with more keys come before its own
+    int2* all = reinterpret_cast<int2*>(smem);                      // Q is not there yet
+    const int i = threadIdx.x;
+    int2 me = make_int2(0, 0);
+    if (i < p.rows) all[i] = me = make_int2(p.ends[i], tiles_of(i));
+    __syncthreads();
+    int before = 0;
+    for (int k = 0; k < p.rows; ++k) {
+      const int2 o = all[k];
+      if (o.x > me.x || (o.x == me.x && k < i)) before += o.y;
+    }
+    if (i < p.rows && unit >= before && unit < before + me.y) {
+      misc[3] = i;
+      misc[4] = before + me.y - 1 - unit;
+    }
+  } else {
+    // more rows than threads: in their order, from the last
+    int mine = 0;
+    const int per = ceil_div(p.rows, THREADS), lo = min(p.rows, (int)threadIdx.x * per), hi = min(p.rows, lo + per);
+    for (int i = lo; i < hi; ++i) mine += tiles_of(i);
+    int upto = mine, total = 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += u;
+    }
+    if (lane == 31) misc[8 + warp] = upto;
+    __syncthreads();
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) upto += misc[8 + w];
+      total += misc[8 + w];
+    }
+    const int want = total - 1 - unit;
+    int at = upto - mine;
+    for (int i = lo; i < hi && want >= at; ++i) {
       const int n = tiles_of(i);
       if (want < at + n) {
         misc[3] = i;
         misc[4] = want - at;
-        break;
       }
       at += n;
     }
   }
+  __syncthreads();
+  if (misc[3] < 0) return;             // the grid is an upper bound
   const uint32_t aS = smem_u32(smem), aB = smem_u32(bars);
   auto q_full = aB;
   auto raw_full = [&](int w) { return aB + 8u * (1 + w); };
@@ -525,12 +542,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
           tmem_st_32x32b_x32(o_addr + c, o);
         }
       }
-      float sum = exp_store<0>(s, f, m_use, bf, group, s_addr);
+      float sum = bf ? exp_store<0, true>(s, f, m_use, group, s_addr) : exp_store<0, false>(s, f, m_use, group, s_addr);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_a(p_lo(t));
-      sum += exp_store<1>(s, f, m_use, bf, group, s_addr);
+      sum += bf ? exp_store<1, true>(s, f, m_use, group, s_addr) : exp_store<1, false>(s, f, m_use, group, s_addr);
       l = l * alpha + sum;
       tmem_st_wait();
       tc_fence_before();

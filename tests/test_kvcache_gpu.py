@@ -530,3 +530,17 @@ def test_cache_through_prompts_steps_and_reorders():
     for c in caches:
         c.reset([0, 1, 2])
     assert int(caches[0].free_count) == int(caches[1].free_count)
+
+
+def test_attention_prompts_in_a_batch_of_many_rows():
+    """More rows than a block has threads: single tokens, rows without new ones and a few prompts among them."""
+    n = 500
+    held = [(7 * i) % 23 for i in range(n)]
+    new = [1 if i % 3 else 0 for i in range(n)]
+    new[0], new[250], new[499], held[250] = 700, 900, 1000, 300
+    d = C.attention_inputs((held, new, 12, 12, 64, 16))
+    q = d["q"][: d["T"], 1:13]
+    want, A = reference(d, q, 0.125)
+    out = run_attention(d)
+    clean()
+    assert np.all(np.abs(out[: d["T"]].cpu().double().numpy() - want) <= bound(q, d, want, A, 0.125))
