@@ -26,7 +26,7 @@ using namespace nb;
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int FEW = 64;                // query rows of a row of the batch and head, up to which this kernel does it in any case
-constexpr int STAGES = 4;              // steps in flight: three ahead of the one in work
+constexpr int STAGES = 3;              // steps in flight: two ahead of the one in work
 constexpr int LEAD = 2;                // steps that starting a tile costs, in the measure by which the batch is cut
 constexpr int LEAST = 2;               // a piece has at least so many steps
 constexpr int SOLO = 8;                // tables of at most so many steps: a tile to a warp, nothing to join
@@ -84,6 +84,12 @@ __device__ __forceinline__ uint32_t nan_code(uint32_t w) {         // nonzero wh
   return (m + 0x01010101u) & 0x80808080u;
 }
 
+// n / d for d >= 1 with m = 2^32 / d rounded up (0 for d = 1): exact below 2^16, a division beyond
+__device__ __forceinline__ int quotient(int n, int d, unsigned m) {
+  if ((unsigned)n < 65536u && d < 65536) return m ? (int)__umulhi((unsigned)n, m) : n;
+  return n / d;
+}
+
 // ---------------------------------------------------------------- how the batch is cut
 // A job is a tile of query rows and a cache head.  It costs LEAD + steps (one, where every job is one warp's).  `upto`
 // (shared memory, rows + 1): exclusive sums over the rows; `piece`: what a warp takes.
@@ -102,7 +108,7 @@ __device__ __forceinline__ int row_tiles(const KvAttn& p, int i) {
   const int first = p.starts[i];
   const long long n = first < 0 ? 0 : (long long)min(p.starts[i + 1], p.tokens) - first;
   // rows with more query rows than `few` belong to the kernel of prompts
-  return n <= 0 || n * p.group > p.few ? 0 : (int)((n * p.group + p.tile - 1) / p.tile);
+  return n <= 0 || n * p.group > p.few ? 0 : (int)((n * p.group + p.tile - 1) >> (p.tile == 8 ? 3 : 4));
 }
 // A batch of 2^31 steps (8 TB of codes) is refused: reported, and nothing is done.
 template <int KEYS>
@@ -153,7 +159,7 @@ __device__ __forceinline__ Job job_at(const KvAttn& p, const int* upto, int x) {
   j.row = a;
   j.cost = job_cost<KEYS>(p, a);
   const int n = (x - upto[a]) / j.cost;
-  j.qt = n / p.hk;
+  j.qt = quotient(n, p.hk, p.hk_mul);
   j.head = n - j.qt * p.hk;
   j.begin = upto[a] + n * j.cost;
   return j;
@@ -174,7 +180,7 @@ struct Part {
     count = min(next, p.tokens) - first;
     end = max(0, min(p.ends[j.row], p.width << p.block_log));
     real = min(p.tile, count * p.group - j.qt * p.tile);          // real rows of the tile
-    const int tok0 = j.qt * p.tile / p.group, tok1 = (j.qt * p.tile + real - 1) / p.group;
+    const int tok0 = quotient(j.qt * p.tile, p.group, p.group_mul), tok1 = quotient(j.qt * p.tile + real - 1, p.group, p.group_mul);
     sure = max(0, min(end, end - new_tokens + tok0 + 1));         // the fewest keys that a real row sees
     seen = max(0, min(end, end - new_tokens + tok1 + 1));         // the most
     const int all = ceil_div(seen, KEYS);
@@ -281,7 +287,7 @@ __device__ __forceinline__ void open_tile(const KvAttn& p, const Part<Shape<D>::
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     // 16 dimensions of each 64, of row g
-    const int idx = w.j.qt * p.tile + b * 8 + g, tok = idx / p.group;
+    const int idx = w.j.qt * p.tile + b * 8 + g, tok = quotient(idx, p.group, p.group_mul);
     const __nv_bfloat16* q = (const __nv_bfloat16*)p.q + (long long)(w.first + tok) * p.q_token + (long long)(w.j.head * p.group + idx - tok * p.group) * p.q_head + c * 16;
     uint32_t x[D / 8];
 #pragma unroll
@@ -320,7 +326,7 @@ __device__ __forceinline__ void open_tile(const KvAttn& p, const Part<Shape<D>::
     for (int h = 0; h < 2; ++h) {
       const int row = b * 8 + 2 * c + h;
       t.f[b][h] = __shfl_sync(0xffffffffu, back, (2 * c + h) * 4);
-      t.lim[b][h] = row < w.real ? max(0, min(w.end, w.end - w.new_tokens + (w.j.qt * p.tile + row) / p.group + 1)) : 0;
+      t.lim[b][h] = row < w.real ? max(0, min(w.end, w.end - w.new_tokens + quotient(w.j.qt * p.tile + row, p.group, p.group_mul) + 1)) : 0;
       t.m[b][h] = NONE;
       t.l[b][h] = 0.f;
     }
@@ -534,7 +540,7 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
 
 template <int D>
 __device__ __forceinline__ void store_out(const KvAttn& p, int first, int head, int idx, int d, float a, float b, float c, float e) {
-  const int tok = idx / p.group;
+  const int tok = quotient(idx, p.group, p.group_mul);
   __nv_bfloat16* o = (__nv_bfloat16*)p.out + (long long)(first + tok) * p.o_token + (long long)(head * p.group + idx - tok * p.group) * p.o_head + d;
   const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, e);
   if (p.o_vec) {
@@ -762,6 +768,8 @@ int nb_kv_attention(const void* q, void* out, const void* codes, const float* sc
   p.q = q; p.out = out; p.codes = (const uint8_t*)codes; p.scale = scale; p.tables = tables; p.starts = starts; p.ends = ends;
   p.rows = rows; p.tokens = tokens; p.hq = hq; p.hk = hk; p.group = hq / hk; p.blocks = blocks; p.width = width; p.kv_rows = blocks * hk * block;
   while ((1 << p.block_log) < block) ++p.block_log;
+  p.group_mul = p.group > 1 ? (unsigned)((0x100000000ULL + p.group - 1) / p.group) : 0;
+  p.hk_mul = hk > 1 ? (unsigned)((0x100000000ULL + hk - 1) / hk) : 0;
   p.q_token = q_token; p.q_head = q_head; p.o_token = o_token; p.o_head = o_head; p.kv_stride = kv_stride; p.s_stride = s_stride;
   p.q_vec = !((reinterpret_cast<uintptr_t>(q) & 15) || (q_token & 7) || (q_head & 7));
   p.o_vec = !((reinterpret_cast<uintptr_t>(out) & 7) || (o_token & 3) || (o_head & 3));

@@ -43,6 +43,7 @@ struct KvAttn {
   const float* scale;                           // [2, N, H]
   const int *tables, *starts, *ends;
   int rows, tokens, hq, hk, group, block_log, blocks, width;
+  unsigned group_mul, hk_mul;                   // 2^32 / group and / hk, rounded up
   int kv_rows;                                  // blocks * hk * block
   int q_vec, o_vec, o_vec16;                    // 16-byte loads of q, 8- and 16-byte stores of out are aligned
   int few;                                      // rows of the batch with at most this many query rows per head are done here
