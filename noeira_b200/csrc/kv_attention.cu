@@ -29,7 +29,7 @@ constexpr int FEW = 64;                // query rows of a row of the batch and h
 constexpr int STAGES = 3;              // steps in flight: two ahead of the one in work
 constexpr int LEAD = 2;                // steps that starting a tile costs, in the measure by which the batch is cut
 constexpr int LEAST = 2;               // a piece has at least so many steps
-constexpr int SOLO = 8;                // tables of at most so many steps: a tile to a warp, nothing to join
+constexpr int TEAM = 40;               // tables of at most so many steps: a tile to a block, whose warps take turns and join in shared memory
 constexpr float RAISE = 8.f;           // the running maximum is raised when it falls behind by more than 2^8 ...
 constexpr float LIFT = 7.f;            // ... and weights are at most 2^(8 + 7), below f16's largest, so that small ones stay normal
 constexpr float NONE = -3e38f;         // the running maximum of a row that has seen nothing
@@ -91,7 +91,7 @@ __device__ __forceinline__ int quotient(int n, int d, unsigned m) {
 }
 
 // ---------------------------------------------------------------- how the batch is cut
-// A job is a tile of query rows and a cache head.  It costs LEAD + steps (one, where every job is one warp's).  `upto`
+// A job is a tile of query rows and a cache head.  It costs LEAD + steps (one, where every job is one block's).  `upto`
 // (shared memory, rows + 1): exclusive sums over the rows; `piece`: what a warp takes.
 struct Cut {
   int total, piece;
@@ -101,48 +101,51 @@ struct Job {
 };
 
 template <int KEYS>
-__device__ __forceinline__ int job_cost(const KvAttn& p, int i) {
-  return p.solo ? 1 : LEAD + ceil_div(max(1, min(p.ends[i], p.width << p.block_log)), KEYS);
+__device__ __forceinline__ int job_cost(const KvAttn& p, int end) {
+  return p.team ? 1 : LEAD + ceil_div(max(1, min(end, p.width << p.block_log)), KEYS);
 }
-__device__ __forceinline__ int row_tiles(const KvAttn& p, int i) {
-  const int first = p.starts[i];
-  const long long n = first < 0 ? 0 : (long long)min(p.starts[i + 1], p.tokens) - first;
-  // rows with more query rows than `few` belong to the kernel of prompts
-  return n <= 0 || n * p.group > p.few ? 0 : (int)((n * p.group + p.tile - 1) >> (p.tile == 8 ? 3 : 4));
-}
-// A batch of 2^31 steps (8 TB of codes) is refused: reported, and nothing is done.
 template <int KEYS>
-__device__ __forceinline__ Cut cut_batch(const KvAttn& p, int* upto, long long* sh) {
+__device__ __forceinline__ long long row_cost(const KvAttn& p, int i) {
+  const int first = __ldg(p.starts + i), next = __ldg(p.starts + i + 1), end = __ldg(p.ends + i);
+  const long long n = first < 0 ? 0 : (long long)min(next, p.tokens) - first;
+  // rows with more query rows than `few` belong to the kernel of prompts
+  const long long tiles = n <= 0 || n * p.group > p.few ? 0 : (n * p.group + p.tile - 1) >> (p.tile == 8 ? 3 : 4);
+  return tiles * p.hk * job_cost<KEYS>(p, end);
+}
+// A batch of which one thread's rows have 2^24 steps (64 GB of codes) is refused: reported, and nothing is done.
+template <int KEYS>
+__device__ __forceinline__ Cut cut_batch(const KvAttn& p, int* upto, int* sh) {
   const int tid = threadIdx.x, per = ceil_div(p.rows, THREADS);
   const int lo = min(p.rows, tid * per), hi = min(p.rows, lo + per);
   long long sum = 0;
-  for (int i = lo; i < hi; ++i) sum += (long long)row_tiles(p, i) * p.hk * job_cost<KEYS>(p, i);
-  long long at = sum;
+  for (int i = lo; i < hi; ++i) sum += row_cost<KEYS>(p, i);
+  const bool large = sum > 1 << 24;
+  const int mine = large ? 0 : (int)sum;
+  int at = mine;
   const int lane = tid & 31, w = tid >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, at, o);
+    const int u = __shfl_up_sync(0xffffffffu, at, o);
     if (lane >= o) at += u;
   }
   if (lane == 31) sh[w] = at;
-  __syncthreads();
-  long long total = 0;
+  const bool refused = __syncthreads_or(large);
+  Cut c;
+  c.total = 0;
 #pragma unroll
   for (int i = 0; i < WARPS; ++i) {
     if (i < w) at += sh[i];
-    total += sh[i];
+    c.total += sh[i];
   }
-  if (total > 0x7fff0000LL) {
+  if (refused) {
     if (tid == 0 && blockIdx.x == 0) report(p.status, NB_ST_BOUNDS, 11, 0);
-    total = at = sum = 0;
+    c.total = 0;
   }
-  Cut c;
-  c.total = (int)total;
-  c.piece = p.solo ? 1 : max(LEAST, (c.total + p.pieces - 1) / p.pieces);
-  int begin = (int)(at - sum);
+  c.piece = p.team ? 1 : max(LEAST, (c.total + p.pieces - 1) / p.pieces);
+  int begin = at - mine;
   for (int i = lo; i < hi; ++i) {
     upto[i] = begin;
-    begin += row_tiles(p, i) * p.hk * job_cost<KEYS>(p, i);
+    if (per > 1) begin += (int)row_cost<KEYS>(p, i);
   }
   if (tid == 0) upto[p.rows] = c.total;
   __syncthreads();
@@ -157,7 +160,7 @@ __device__ __forceinline__ Job job_at(const KvAttn& p, const int* upto, int x) {
   }
   Job j;
   j.row = a;
-  j.cost = job_cost<KEYS>(p, a);
+  j.cost = job_cost<KEYS>(p, __ldg(p.ends + a));
   const int n = (x - upto[a]) / j.cost;
   j.qt = quotient(n, p.hk, p.hk_mul);
   j.head = n - j.qt * p.hk;
@@ -171,21 +174,22 @@ struct Part {
   Job j;
   int stop;                            // where it ends, in the measure of the cut
   int first, count, real, end, new_tokens, sure, seen, from, last;
-  __device__ __forceinline__ void set(const KvAttn& p, const int* upto, int x, int x1) {
+  // `skip`: the first of the job's steps that is this warp's (a team's warps take every fourth)
+  __device__ __forceinline__ void set(const KvAttn& p, const int* upto, int x, int x1, int skip) {
     j = job_at<KEYS>(p, upto, x);
     stop = min(x1, j.begin + j.cost);
-    first = p.starts[j.row];
-    const int next = p.starts[j.row + 1];
+    first = __ldg(p.starts + j.row);
+    const int next = __ldg(p.starts + j.row + 1);
     new_tokens = next - first;
     count = min(next, p.tokens) - first;
-    end = max(0, min(p.ends[j.row], p.width << p.block_log));
+    end = max(0, min(__ldg(p.ends + j.row), p.width << p.block_log));
     real = min(p.tile, count * p.group - j.qt * p.tile);          // real rows of the tile
     const int tok0 = quotient(j.qt * p.tile, p.group, p.group_mul), tok1 = quotient(j.qt * p.tile + real - 1, p.group, p.group_mul);
     sure = max(0, min(end, end - new_tokens + tok0 + 1));         // the fewest keys that a real row sees
     seen = max(0, min(end, end - new_tokens + tok1 + 1));         // the most
     const int all = ceil_div(seen, KEYS);
-    from = p.solo ? 0 : max(0, x - j.begin - LEAD);
-    last = p.solo ? all : min(all, max(0, stop - j.begin - LEAD));
+    from = p.team ? skip : max(0, x - j.begin - LEAD);
+    last = p.team ? all : min(all, max(0, stop - j.begin - LEAD));
   }
 };
 
@@ -209,58 +213,67 @@ __device__ __forceinline__ int chunk_at(int r, int ch) {
 template <int D>
 struct Feed {                          // runs over the steps of a warp's piece, ahead of the work
   Part<Shape<D>::KEYS> part;
-  int x, x1, stride;
+  int x, x1, stride, skip, hop;        // skip, hop: this warp's first step of a job, and how far it is to the next
   int step, page0, base;               // lane l: first row of page page0 + l among the tensor's rows, none: behind the last
-  float ks, vs;                        // and its scales
-  __device__ __forceinline__ void begin(int at, int end, int by) {
+  __device__ __forceinline__ void begin(int at, int end, int by, int first, int every) {
     x = at;
     x1 = end;
     stride = by;
+    skip = first;
+    hop = every;
     step = part.last = 0;
   }
   __device__ __forceinline__ void turn(const KvAttn& p, int page) {                  // the next 32 pages
     page0 = page;
     const int pg = page + (int)(threadIdx.x & 31);
     base = p.kv_rows;
-    ks = vs = -1.f;
     if ((long long)pg << p.block_log < part.seen) {
-      const int b = p.tables[(long long)part.j.row * p.width + pg];
-      if ((unsigned)b < (unsigned)p.blocks) {
-        const int page_head = b * p.hk + part.j.head;
-        base = page_head << p.block_log;
-        ks = p.scale[page_head];
-        vs = p.scale[p.s_stride + page_head];
-      } else {
-        report(p.status, NB_ST_BOUNDS, 10, part.j.row);
-      }
+      const int b = __ldg(p.tables + (long long)part.j.row * p.width + pg);
+      if ((unsigned)b < (unsigned)p.blocks) base = (b * p.hk + part.j.head) << p.block_log;
+      else report(p.status, NB_ST_BOUNDS, 10, part.j.row);
     }
   }
+  // The barrier of a stage completes with the bytes of the boxes and with the copies of the scales.
   __device__ __forceinline__ void next(const KvAttn& p, const CUtensorMap& map, const int* upto, uint32_t stage, Head* head, uint32_t bar) {
     constexpr int SUB = Shape<D>::SUB, KEYS = Shape<D>::KEYS;
     while (step >= part.last) {        // the next part that has steps
       if (x >= x1) return;
-      part.set(p, upto, x, x1);
+      part.set(p, upto, x, x1, skip);
       x = stride ? x + stride : part.stop;
       step = part.from;
       page0 = -64;
     }
-    const int lane = threadIdx.x & 31;
-    if (lane == 0) mbar_expect_tx_at(bar, STAGE);
+    int row[SUB];
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
       const int k0 = step * KEYS + s * 16, pg = k0 >> p.block_log;
       if (pg - page0 >= 32) turn(p, pg);
-      const int row = __shfl_sync(0xffffffffu, base, pg - page0) + (k0 & ((1 << p.block_log) - 1));
-      if (lane == pg - page0) {
-        head->ks[s] = ks;
-        head->vs[s] = vs;
-      }
-      if (lane == 0) {
-        copy_box(stage + s * 1024, map, bar, row, 0);
-        copy_box(stage + 2048 + s * 1024, map, bar, row, 1);
-      }
+      row[s] = __shfl_sync(0xffffffffu, base, pg - page0);
     }
-    ++step;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+        if (row[s] < p.kv_rows) {
+          const float* from = p.scale + (row[s] >> p.block_log);
+          copy4(smem_u32(&head->ks[s]), from);
+          copy4(smem_u32(&head->vs[s]), from + p.s_stride);
+        } else {
+          head->ks[s] = head->vs[s] = -1.f;
+        }
+      }
+      mbar_expect_tx_at(bar, STAGE);
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+        const int y = row[s] + ((step * KEYS + s * 16) & ((1 << p.block_log) - 1));
+        copy_box(stage + s * 1024, map, bar, y, 0);
+        copy_box(stage + 2048 + s * 1024, map, bar, y, 1);
+      }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+    }
+    step += hop;
+  }
+  static __device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
   }
   static __device__ __forceinline__ void mbar_expect_tx_at(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -281,15 +294,15 @@ struct Tile {                          // what a warp keeps of a tile of 8 NB qu
   float vref, vinv;                    // the largest scale of the values so far, and its inverse
 };
 
+// The query rows of a tile as they are in memory: 16 dimensions of each 64, of row g of each 8.
 template <int D, int NB>
-__device__ __forceinline__ void open_tile(const KvAttn& p, const Part<Shape<D>::KEYS>& w, Tile<D, NB>& t) {
+__device__ __forceinline__ void fetch_q(const KvAttn& p, const Part<Shape<D>::KEYS>& w, uint32_t (&raw)[NB][D / 8]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    // 16 dimensions of each 64, of row g
     const int idx = w.j.qt * p.tile + b * 8 + g, tok = quotient(idx, p.group, p.group_mul);
     const __nv_bfloat16* q = (const __nv_bfloat16*)p.q + (long long)(w.first + tok) * p.q_token + (long long)(w.j.head * p.group + idx - tok * p.group) * p.q_head + c * 16;
-    uint32_t x[D / 8];
+    uint32_t (&x)[D / 8] = raw[b];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) x[i] = 0;
     if (tok < w.count) {
@@ -309,6 +322,14 @@ __device__ __forceinline__ void open_tile(const KvAttn& p, const Part<Shape<D>::
         }
       }
     }
+  }
+}
+template <int D, int NB>
+__device__ __forceinline__ void open_tile(const KvAttn& p, const Part<Shape<D>::KEYS>& w, const uint32_t (&raw)[NB][D / 8], Tile<D, NB>& t) {
+  const int c = threadIdx.x & 3;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const uint32_t (&x)[D / 8] = raw[b];
     // power of two that takes the row's largest element to [2^14, 2^15); the row's scores are scaled back by its inverse
     float top = 0.f;
 #pragma unroll
@@ -553,6 +574,47 @@ __device__ __forceinline__ void store_out(const KvAttn& p, int first, int head, 
   }
 }
 
+// Joins what the warps of a block have of a tile, relative to the largest maximum of each row.
+template <int D, int NB>
+__device__ __forceinline__ void join_team(const KvAttn& p, const Part<Shape<D>::KEYS>& w, const Tile<D, NB>& t, float* team_o, float2* team_ml) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = b * 8 + 2 * c + h;
+      const float l = column_sum(t.l[b][h]);
+      if (row >= w.real) continue;
+      float* o = team_o + (warp * 8 * NB + row) * D + g * (D / 8);
+#pragma unroll
+      for (int k = 0; k < D / 16; k += 2)
+        *reinterpret_cast<float4*>(o + 2 * k) = make_float4(t.o[b][k][h] * t.vref, t.o[b][k][2 + h] * t.vref, t.o[b][k + 1][h] * t.vref, t.o[b][k + 1][2 + h] * t.vref);
+      if (g == 0) team_ml[warp * 8 * NB + row] = make_float2(t.m[b][h], l);
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < w.real * (D / 4); i += THREADS) {
+    const int row = i / (D / 4), d = i % (D / 4) * 4;
+    float top = NONE, l = 0.f;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) top = fmaxf(top, team_ml[k * 8 * NB + row].x);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) {
+      const float2 ml = team_ml[k * 8 * NB + row];
+      const float f = ml.x == NONE ? 1.f : ex2(ml.x - top);          // without a maximum all is zero, or NaN
+      const float4 v = *reinterpret_cast<const float4*>(team_o + (k * 8 * NB + row) * D + d);
+      l += ml.y * f;
+      o.x += v.x * f;
+      o.y += v.y * f;
+      o.z += v.z * f;
+      o.w += v.w * f;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    store_out<D>(p, w.first, w.j.head, w.j.qt * p.tile + row, d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  }
+  __syncthreads();                     // before the next tile's
+}
+
 // Partial results of a warp: slot 1 for the job that begins in its piece and runs on, slot 0 for the one that came from before.
 __device__ __forceinline__ long long slot_at(long long piece, int slot) { return (piece * 2 + slot) * 16; }
 
@@ -565,50 +627,65 @@ __global__ void __launch_bounds__(THREADS, 3) kv_attn_kernel(const __grid_consta
   const uint8_t* ring = smem + warp * STAGES * STAGE;
   Head* heads = reinterpret_cast<Head*>(smem + WARPS * STAGES * STAGE) + warp * STAGES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WARPS * STAGES * (STAGE + sizeof(Head))) + warp * STAGES;
-  long long* sh = reinterpret_cast<long long*>(smem + WARPS * STAGES * (STAGE + sizeof(Head) + 8));
-  int* upto = reinterpret_cast<int*>(sh + WARPS);
+  int* sh = reinterpret_cast<int*>(smem + WARPS * STAGES * (STAGE + sizeof(Head) + 8));
+  float* team_o = reinterpret_cast<float*>(sh + WARPS);           // [WARPS][8 NB][D], a team's only
+  float2* team_ml = reinterpret_cast<float2*>(team_o + (p.team ? WARPS * 8 * NB * D : 0));
+  int* upto = reinterpret_cast<int*>(team_ml + (p.team ? WARPS * 8 * NB : 0));
   if (lane == 0) {
     prefetch_tensormap(&map);
-    for (int i = 0; i < STAGES; ++i) mbar_init(&bars[i], 1);
+    for (int i = 0; i < STAGES; ++i) mbar_init(&bars[i], 2);
     fence_barrier_init();
   }
   const Cut cut = cut_batch<KEYS>(p, upto, sh);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int piece = blockIdx.x * WARPS + warp;
-  int x = (int)min((long long)cut.total, (long long)piece * cut.piece);
-  const int x1 = p.solo ? cut.total : (int)min((long long)cut.total, (long long)x + cut.piece), stride = p.solo ? p.pieces : 0;
-  if (!p.solo && lane == 0) p.part_job[piece].w = 0;
+  const int piece = blockIdx.x * WARPS + warp, hop = p.team ? WARPS : 1;
+  int x = p.team ? blockIdx.x : (int)min((long long)cut.total, (long long)piece * cut.piece);
+  const int x1 = p.team ? cut.total : (int)min((long long)cut.total, (long long)x + cut.piece), stride = p.team ? gridDim.x : 0;
+  if (!p.team && lane == 0) p.part_job[piece].w = 0;
   const uint32_t ring_a = smem_u32(ring), bars_a = smem_u32(bars);
   Feed<D> feed;
-  feed.begin(x, x1, stride);
-#pragma unroll 1
-  for (int i = 0; i < STAGES - 1; ++i) feed.next(p, map, upto, ring_a + i * STAGE, heads + i, bars_a + 8 * i);
+  feed.begin(x, x1, stride, p.team ? warp : 0, hop);
   int at = 0;                          // stage of the next step
   uint32_t phase = 0;
+  bool ok = true, primed = false;
   while (x < x1) {
     Part<KEYS> w;
-    w.set(p, upto, x, x1);
-    Tile<D, NB> t;
-    open_tile<D, NB>(p, w, t);
+    w.set(p, upto, x, x1, p.team ? warp : 0);
+    uint32_t raw[NB][D / 8];
+    fetch_q<D, NB>(p, w, raw);
+    if (!primed) {                     // the first copies go out while the queries are on their way
 #pragma unroll 1
-    for (int st = w.from; st < w.last; ++st) {
+      for (int i = 0; i < STAGES - 1; ++i) feed.next(p, map, upto, ring_a + i * STAGE, heads + i, bars_a + 8 * i);
+      primed = true;
+    }
+    Tile<D, NB> t;
+    open_tile<D, NB>(p, w, raw, t);
+#pragma unroll 1
+    for (int st = w.from; st < w.last && ok; st += hop) {
       __syncwarp();                    // all lanes are done with the step before, whose stage is filled anew
       const int ahead = (at + STAGES - 1) % STAGES;
       feed.next(p, map, upto, ring_a + ahead * STAGE, heads + ahead, bars_a + 8 * ahead);
-      if (!__all_sync(0xffffffffu, mbar_wait(&bars[at], phase, p.status, 401))) {
-        // Copies that do not come: give the others in flight their time, so that none writes into memory that is no longer
-        // this block's, and leave.
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars[at], phase, p.status, 401));
+      if (!ok) {
+        // Copies that do not come: give the others in flight their time, so that none writes into memory that is no longer this
+        // block's, and do nothing more but take part in the block's barriers.
         for (int i = 1; i < STAGES; ++i) {
           const int b = (at + i) % STAGES;
           mbar_wait(&bars[b], phase ^ (b < at ? 1u : 0u), p.status, 402);
         }
-        return;
+        break;
       }
       step_tile<D, NB>(p, t, ring + at * STAGE, heads + at, st, w.seen, w.sure);
       at = (at + 1) % STAGES;
       phase ^= at == 0 ? 1u : 0u;
     }
-    const bool alone = p.solo || (x == w.j.begin && w.stop == w.j.begin + w.j.cost);
+    if (p.team) {
+      join_team<D, NB>(p, w, t, team_o, team_ml);
+      x += stride;
+      continue;
+    }
+    if (!ok) return;
+    const bool alone = x == w.j.begin && w.stop == w.j.begin + w.j.cost;
     const long long slot = slot_at(piece, x == w.j.begin);
     if (!alone && x == w.j.begin && lane == 0)   // this piece's warp of the join kernel does this job, of so many pieces
       p.part_job[piece] = make_int4(w.first, w.j.head, w.j.qt, ((w.j.begin + w.j.cost - 1) / cut.piece - piece + 1) | w.real << 16);
@@ -629,7 +706,7 @@ __global__ void __launch_bounds__(THREADS, 3) kv_attn_kernel(const __grid_consta
         }
         if (!alone && g == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + row) * 2) = make_float2(t.m[b][h], l);
       }
-    x = stride ? x + stride : w.stop;
+    x = w.stop;
   }
 }
 
@@ -641,11 +718,12 @@ __global__ void __launch_bounds__(THREADS) kv_attn_join_kernel(const KvAttn p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = lane % COLS, share = lane / COLS;
   // every block waits, also one with nothing to join: what follows in the stream may start when this kernel is done
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 all = p.part_job[blockIdx.x * WARPS + (lane & (WARPS - 1))];
 #pragma unroll 1
   for (int i = 0; i < WARPS; ++i) {
-    const int piece = blockIdx.x * WARPS + i;
-    const int4 job = p.part_job[piece];
-    const int n = job.w & 0xffff, real = job.w >> 16, qt = job.z;
+    const int piece = blockIdx.x * WARPS + i, size = __shfl_sync(0xffffffffu, all.w, i);
+    const int first = __shfl_sync(0xffffffffu, all.x, i), head = __shfl_sync(0xffffffffu, all.y, i), qt = __shfl_sync(0xffffffffu, all.z, i);
+    const int n = size & 0xffff, real = size >> 16;
     if (n == 0) continue;
 #pragma unroll 1
     for (int row = warp; row < real; row += WARPS) {
@@ -674,7 +752,7 @@ __global__ void __launch_bounds__(THREADS) kv_attn_join_kernel(const KvAttn p) {
         l += __shfl_xor_sync(0xffffffffu, l, 16);
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      if (share == 0) store_out<D>(p, job.x, job.y, qt * p.tile + row, col * 4, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+      if (share == 0) store_out<D>(p, first, head, qt * p.tile + row, col * 4, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     }
   }
 }
@@ -682,23 +760,23 @@ __global__ void __launch_bounds__(THREADS) kv_attn_join_kernel(const KvAttn p) {
 template <int D, int NB>
 int launch_few(KvAttn p, cudaStream_t stream) {
   constexpr int fixed = 1024 + WARPS * STAGES * (STAGE + (int)sizeof(Head) + 8);
-  const int scan = WARPS * 8 + (p.rows + 1) * 4;
+  p.tile = 8 * NB;
+  p.team = ((long long)p.width << p.block_log) <= TEAM * Shape<D>::KEYS;
+  const int scan = WARPS * 4 + (p.rows + 1) * 4 + (p.team ? WARPS * 8 * NB * (D * 4 + 8) : 0);
   static bool configured[64] = {};
   int dev = 0;
   NB_CUDA(cudaGetDevice(&dev));
   if (dev >= 64) return NB_ERR_BAD_ARG;
   if (!configured[dev]) {
-    NB_CUDA(cudaFuncSetAttribute(kv_attn_kernel<D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + WARPS * 8 + 8193 * 4));
+    NB_CUDA(cudaFuncSetAttribute(kv_attn_kernel<D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + WARPS * 4 + 8193 * 4 + WARPS * 8 * NB * (D * 4 + 8)));
     configured[dev] = true;
   }
   CUtensorMap map;
   const int rc = kv_code_map(&map, p, D, 1);
   if (rc) return rc;
-  p.tile = 8 * NB;
-  p.solo = ((long long)p.width << p.block_log) <= SOLO * Shape<D>::KEYS;
   kv_attn_kernel<D, NB><<<p.pieces / WARPS, THREADS, fixed + scan, stream>>>(map, p);
   NB_LAUNCH_CHECK();
-  if (p.solo) return NB_OK;
+  if (p.team) return NB_OK;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.pieces / WARPS);
   cfg.blockDim = dim3(THREADS);

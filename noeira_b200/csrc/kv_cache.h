@@ -48,7 +48,7 @@ struct KvAttn {
   int q_vec, o_vec, o_vec16;                    // 16-byte loads of q, 8- and 16-byte stores of out are aligned
   int few;                                      // rows of the batch with at most this many query rows per head are done here
   int tile;                                     // query rows of a tile
-  int pieces, solo;                             // warps; every tile is one warp's
+  int pieces, team;                             // warps; every tile is one block's
   long long q_token, q_head, o_token, o_head;
   long long kv_stride, s_stride;                // from the keys' codes / scales to the values'
   float scale_log2;
