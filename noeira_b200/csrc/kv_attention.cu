@@ -828,7 +828,11 @@ int nb_kv_attention_mode(int mode) {
 
 // Pieces that the batch is cut into, and floats of work space that nb_kv_attention needs.
 int nb_kv_attention_pieces(int) { return 148 * WARPS * 3; }
-long long nb_kv_attention_work(int dim) { return (long long)nb_kv_attention_pieces(dim) * (2 * 16 * (dim + 2) + 4); }
+// None where tables are so short that a block does a tile.
+long long nb_kv_attention_work(int dim, long long keys) {
+  if (keys <= TEAM * 16 * (128 / dim)) return 0;
+  return (long long)nb_kv_attention_pieces(dim) * (2 * 16 * (dim + 2) + 4);
+}
 
 int nb_kv_attention(const void* q, void* out, const void* codes, const float* scale, const int* tables, const int* starts,
                     const int* ends, int rows, int tokens, int max_new, int hq, int hk, int dim, int block, int blocks, int width,
@@ -841,7 +845,8 @@ int nb_kv_attention(const void* q, void* out, const void* codes, const float* sc
   if ((long long)blocks * hk * block > 0x7fffffffLL - 256) return NB_ERR_TOO_LARGE;   // rows of the copies' tensor
   if (tokens == 0) return NB_OK;
   if ((reinterpret_cast<uintptr_t>(codes) & 15) || (kv_stride & 15)) return NB_ERR_UNALIGNED;
-  if (!work || work_floats < nb_kv_attention_work(dim) || (reinterpret_cast<uintptr_t>(work) & 15)) return NB_ERR_BAD_ARG;
+  const long long floats = nb_kv_attention_work(dim, (long long)width * block);
+  if (floats > 0 && (!work || work_floats < floats || (reinterpret_cast<uintptr_t>(work) & 15))) return NB_ERR_BAD_ARG;
   KvAttn p{};
   p.q = q; p.out = out; p.codes = (const uint8_t*)codes; p.scale = scale; p.tables = tables; p.starts = starts; p.ends = ends;
   p.rows = rows; p.tokens = tokens; p.hq = hq; p.hk = hk; p.group = hq / hk; p.blocks = blocks; p.width = width; p.kv_rows = blocks * hk * block;

@@ -309,7 +309,10 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p) {
 }
 
 // ------------------------------------------------------------------------------------------------ reorder
-__global__ void __launch_bounds__(128) kv_reorder_kernel(KvReorder p) {
+// A block per row and four planes (a plane: one layer's keys or values): what a row copies is found out once for them, and their
+// loads go out together.  The table is the first plane's business.
+constexpr int PLANES = 4;
+__global__ void __launch_bounds__(128) kv_reorder_kernel(const KvReorder p) {
   const int j = blockIdx.x, g = j / p.beams * p.beams;
   int parent = p.parents[j];
   if (parent < 0 || parent >= p.beams) {
@@ -341,17 +344,32 @@ __global__ void __launch_bounds__(128) kv_reorder_kernel(KvReorder p) {
     }
   }
   if (!move) return;
+  // The copied places of a head lie together (fill * dim bytes); over the heads they are a head's whole size apart.
   const long long page = (long long)p.heads * p.block * p.dim;
-  uint8_t* base = p.codes + (long long)blockIdx.y * p.plane;
-  const uint4* s = reinterpret_cast<const uint4*>(base + (long long)from * page);
-  uint4* d = reinterpret_cast<uint4*>(base + (long long)to * page);
-  const int head16 = p.block * p.dim / 16, fill16 = fill * p.dim / 16;
-  for (int i = threadIdx.x; i < p.heads * fill16; i += blockDim.x) {
-    const int h = i / fill16, o = h * head16 + i - h * fill16;
-    d[o] = s[o];
+  const int head16 = p.block * p.dim / 16, fill16 = fill * p.dim / 16, n = p.heads * fill16;
+  const int last = min(p.planes, (int)(blockIdx.y + 1) * PLANES);
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int h = i / fill16;
+    const long long o = (long long)h * head16 + (i - h * fill16);
+    uint4 v[PLANES];
+#pragma unroll
+    for (int k = 0; k < PLANES; ++k) {
+      const int plane = blockIdx.y * PLANES + k;
+      if (plane < last) v[k] = __ldcs(reinterpret_cast<const uint4*>(p.codes + plane * p.plane + from * page) + o);
+    }
+#pragma unroll
+    for (int k = 0; k < PLANES; ++k) {
+      const int plane = blockIdx.y * PLANES + k;
+      if (plane < last) __stcs(reinterpret_cast<uint4*>(p.codes + plane * p.plane + to * page) + o, v[k]);
+    }
   }
-  float* sc = p.scale + (long long)blockIdx.y * p.blocks * p.heads;
-  for (int i = threadIdx.x; i < p.heads; i += blockDim.x) sc[(long long)to * p.heads + i] = sc[(long long)from * p.heads + i];
+  for (int i = threadIdx.x; i < p.heads * PLANES; i += blockDim.x) {
+    const int plane = blockIdx.y * PLANES + i / p.heads, h = i % p.heads;
+    if (plane < last) {
+      float* sc = p.scale + (long long)plane * p.blocks * p.heads + h;
+      sc[(long long)to * p.heads] = sc[(long long)from * p.heads];
+    }
+  }
 }
 
 }  // namespace
@@ -410,9 +428,9 @@ int nb_kv_reorder(void* codes, float* scale, const int* tables, const int* lengt
                   unsigned int* status, void* stream) {
   if (planes <= 0 || planes > 65535 || blocks <= 0 || heads <= 0 || block <= 0 || dim % 16 || rows <= 0 || beams <= 0 || rows % beams || width <= 0) return NB_ERR_BAD_ARG;
   if (reinterpret_cast<uintptr_t>(codes) & 15) return NB_ERR_UNALIGNED;
-  KvReorder p{(uint8_t*)codes, scale, tables, lengths, parents, spare, tables_out, lengths_out, spare_out, blocks, heads, block, dim, rows, beams, width,
+  KvReorder p{(uint8_t*)codes, scale, tables, lengths, parents, spare, tables_out, lengths_out, spare_out, blocks, heads, block, dim, rows, beams, width, planes,
               (long long)blocks * heads * block * dim, status};
-  kv_reorder_kernel<<<dim3(rows, planes), 128, 0, (cudaStream_t)stream>>>(p);
+  kv_reorder_kernel<<<dim3(rows, ceil_div(planes, PLANES)), 128, 0, (cudaStream_t)stream>>>(p);
   NB_LAUNCH_CHECK();
   return NB_OK;
 }

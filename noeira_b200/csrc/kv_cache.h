@@ -31,7 +31,7 @@ struct KvReorder {
   float* scale;
   const int *tables, *lengths, *parents, *spare;
   int *tables_out, *lengths_out, *spare_out;
-  int blocks, heads, block, dim, rows, beams, width;
+  int blocks, heads, block, dim, rows, beams, width, planes;
   long long plane;                              // bytes of one layer's keys or values
   unsigned int* status;
 };
