@@ -57,43 +57,47 @@ __device__ __forceinline__ long long block_scan(long long v, long long* sh, long
   return v + before;
 }
 
+// Place of row i in shared memory: a thread's rows are neighbours, and without a gap every 32 the threads of a warp would meet in the
+// same banks.
+__host__ __device__ inline int spread(int i) { return i + (i >> 5); }
+
 template <int EACH>
 __global__ void __launch_bounds__(256) kv_plan_kernel(const KvPlan p) {
   extern __shared__ int sm[];
   int* s_start = sm;                 // [rows + 1]
-  int* s_off = sm + p.rows + 1;      // [rows] first block of the row among the new ones, -1: refused
-  int* s_len = s_off + p.rows;       // [rows]
+  int* s_off = sm + spread(p.rows) + 1;   // [rows] first block of the row among the new ones, -1: refused
+  int* s_len = s_off + spread(p.rows) + 1;   // [rows]
   __shared__ long long sh[8];
   const int tid = threadIdx.x, per = ceil_div(p.rows, 256);
   const int lo = min(p.rows, tid * per), hi = min(p.rows, lo + per);
   const int free_count = max(0, min(*p.free_count, p.free_size));
 #pragma unroll 4
   for (int i = tid; i < p.rows; i += 256) {
-    s_len[i] = p.lengths[i];
-    s_off[i] = p.new_lens[i];
+    s_len[spread(i)] = p.lengths[i];
+    s_off[spread(i)] = p.new_lens[i];
   }
   __syncthreads();
   long long sum = 0, total;
-  for (int i = lo; i < hi; ++i) sum += max(0, s_off[i]);
+  for (int i = lo; i < hi; ++i) sum += max(0, s_off[spread(i)]);
   long long at = block_scan(sum, sh, total) - sum;      // 64 bits: lengths are the caller's, their sum may be anything
-  if (tid == 0) s_start[p.rows] = (int)min(total, 0x7fffffffLL);
+  if (tid == 0) s_start[spread(p.rows)] = (int)min(total, 0x7fffffffLL);
   sum = 0;
   for (int i = lo; i < hi; ++i) {
-    const int len = s_len[i], given = s_off[i], add = max(0, given);
-    s_start[i] = (int)min(at, 0x7fffffffLL);
+    const int len = s_len[spread(i)], given = s_off[spread(i)], add = max(0, given);
+    s_start[spread(i)] = (int)min(at, 0x7fffffffLL);
     at += add;
     const bool fits = len >= 0 && given >= 0 && (long long)len + add <= ((long long)p.width << p.block_log) && at <= p.tokens;
-    s_off[i] = fits ? ((len + add + (1 << p.block_log) - 1) >> p.block_log) - ((len + (1 << p.block_log) - 1) >> p.block_log) : -1;
-    sum += max(0, s_off[i]);
+    s_off[spread(i)] = fits ? ((len + add + (1 << p.block_log) - 1) >> p.block_log) - ((len + (1 << p.block_log) - 1) >> p.block_log) : -1;
+    sum += max(0, s_off[spread(i)]);
   }
   long long off = block_scan(sum, sh, total) - sum, taken = 0;
   for (int i = lo; i < hi; ++i) {
-    const int need = s_off[i];
+    const int need = s_off[spread(i)];
     if (need < 0 || (need > 0 && off + need > free_count)) {
-      s_off[i] = -1;
+      s_off[spread(i)] = -1;
       if (blockIdx.x == 0) report(p.status, NB_ST_CACHE_FULL, 1, i);
     } else {
-      s_off[i] = (int)min(off, 0x7fffffffLL);           // with need = 0 any offset will do
+      s_off[spread(i)] = (int)min(off, 0x7fffffffLL);           // with need = 0 any offset will do
       if (need > 0) taken = off + need;
     }
     if (need > 0) off += need;
@@ -101,8 +105,8 @@ __global__ void __launch_bounds__(256) kv_plan_kernel(const KvPlan p) {
   __syncthreads();
   if (blockIdx.x == 0) {
     for (int i = tid; i <= p.rows; i += 256) {
-      p.starts[i] = s_start[i];
-      if (i < p.rows) p.ends[i] = s_len[i] + (s_off[i] < 0 ? 0 : s_start[i + 1] - s_start[i]);
+      p.starts[i] = s_start[spread(i)];
+      if (i < p.rows) p.ends[i] = s_len[spread(i)] + (s_off[spread(i)] < 0 ? 0 : s_start[spread(i + 1)] - s_start[spread(i)]);
     }
     taken = (long long)__reduce_max_sync(0xffffffffu, (unsigned)taken);   // at most free_count
     if ((tid & 31) == 0) sh[tid >> 5] = taken;
@@ -118,26 +122,26 @@ __global__ void __launch_bounds__(256) kv_plan_kernel(const KvPlan p) {
     int a = 0, b = p.rows;             // last row with start <= t0
     while (b - a > 1) {
       const int m = (a + b) >> 1;
-      if (s_start[m] <= (int)t0) a = m; else b = m;
+      if (s_start[spread(m)] <= (int)t0) a = m; else b = m;
     }
     int slot[EACH], pos[EACH], row[EACH], page = -1, id = -1;
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
       const int t = (int)t0 + e;       // may pass the last token by three: below 2^31 by the launcher's limit
-      while (a + 1 < p.rows && s_start[a + 1] <= t) {
+      while (a + 1 < p.rows && s_start[spread(a + 1)] <= t) {
         ++a;
         page = -1;
       }
-      const bool real = t < s_start[p.rows] && t < p.tokens;
-      const int len = s_len[a], at_pos = len + t - s_start[a];
+      const bool real = t < s_start[spread(p.rows)] && t < p.tokens;
+      const int len = s_len[spread(a)], at_pos = len + t - s_start[spread(a)];
       slot[e] = -1;
       pos[e] = real ? at_pos : 0;
       row[e] = real ? a : -1;
-      if (real && s_off[a] >= 0) {
+      if (real && s_off[spread(a)] >= 0) {
         const int pg = at_pos >> p.block_log, in = at_pos - (pg << p.block_log);
         if (pg != page) {
           const int have = (int)(((long long)len + (1 << p.block_log) - 1) >> p.block_log);
-          id = pg < have ? p.tables[(long long)a * p.width + pg] : p.free_ids[free_count - 1 - (s_off[a] + pg - have)];
+          id = pg < have ? p.tables[(long long)a * p.width + pg] : p.free_ids[free_count - 1 - (s_off[spread(a)] + pg - have)];
           page = pg;
         }
         if (in == 0) p.tables[(long long)a * p.width + pg] = id;   // the first token of a block: the block is new
@@ -394,12 +398,12 @@ int nb_kv_plan(const int* lengths, const int* new_lens, int* tables, const int* 
   NB_CUDA(cudaGetDevice(&dev));
   if (dev >= 64) return NB_ERR_BAD_ARG;
   if (!configured[dev]) {
-    NB_CUDA(cudaFuncSetAttribute(kv_plan_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * 8192 + 1) * 4));
-    NB_CUDA(cudaFuncSetAttribute(kv_plan_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * 8192 + 1) * 4));
+    NB_CUDA(cudaFuncSetAttribute(kv_plan_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * (8192 + 256 + 1) * 4));
+    NB_CUDA(cudaFuncSetAttribute(kv_plan_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * (8192 + 256 + 1) * 4));
     configured[dev] = true;
   }
-  if (each == 1) kv_plan_kernel<1><<<grid, 256, (3 * rows + 1) * 4, (cudaStream_t)stream>>>(p);
-  else kv_plan_kernel<4><<<grid, 256, (3 * rows + 1) * 4, (cudaStream_t)stream>>>(p);
+  if (each == 1) kv_plan_kernel<1><<<grid, 256, 3 * (spread(rows) + 1) * 4, (cudaStream_t)stream>>>(p);
+  else kv_plan_kernel<4><<<grid, 256, 3 * (spread(rows) + 1) * 4, (cudaStream_t)stream>>>(p);
   NB_LAUNCH_CHECK();
   if (later) NB_CUDA(cudaMemcpyAsync(free_count_out, own, 4, cudaMemcpyDeviceToDevice, (cudaStream_t)stream));
   return NB_OK;
