@@ -41,7 +41,6 @@ __device__ __forceinline__ float value_of(Key k) {
   u ^= (u >> 31) ? 0x80000000u : 0xffffffffu;
   return __uint_as_float(u);
 }
-__device__ __forceinline__ float fit(float x) { return x != x ? -INFINITY : fminf(x, TOP); }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

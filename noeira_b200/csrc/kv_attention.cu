@@ -29,7 +29,6 @@ constexpr int FEW = 64;                // query rows of a row of the batch and h
 constexpr int STAGES = 3;              // steps in flight: two ahead of the one in work
 constexpr int LEAD = 2;                // steps that starting a tile costs, in the measure by which the batch is cut
 constexpr int LEAST = 2;               // a piece has at least so many steps
-constexpr int TEAM = 40;               // tables of at most so many steps: a tile to a block, whose warps take turns and join in shared memory
 constexpr float RAISE = 8.f;           // the running maximum is raised when it falls behind by more than 2^8 ...
 constexpr float LIFT = 7.f;            // ... and weights are at most 2^(8 + 7), below f16's largest, so that small ones stay normal
 constexpr float NONE = -3e38f;         // the running maximum of a row that has seen nothing
@@ -761,7 +760,13 @@ template <int D, int NB>
 int launch_few(KvAttn p, cudaStream_t stream) {
   constexpr int fixed = 1024 + WARPS * STAGES * (STAGE + (int)sizeof(Head) + 8);
   p.tile = 8 * NB;
-  p.team = ((long long)p.width << p.block_log) <= TEAM * Shape<D>::KEYS;
+  // Short tables: a block to a tile, its warps taking turns at the steps and joining in shared memory, which saves the second
+  // kernel; where there are many such tiles, pieces spread them better.  Measured, block / pieces: one row of 300 keys 7.8 / 10.5
+  // us, of 640 11.2 / 11.9, of 1200 15.4 / 11.3 (D = 64); 128 rows of 300 keys 15.3 / 18.7, 1024 rows 98 / 64.  Tiles of 16 rows
+  // come several to a row and share its keys: 4 rows of 64 tokens over 560 keys (D = 128) 37 / 53, 64 rows of 17 over 520 50 / 68.
+  const long long steps = (((long long)p.width << p.block_log) + Shape<D>::KEYS - 1) / Shape<D>::KEYS;
+  const long long jobs = ((long long)p.tokens * p.group / p.tile + min(p.rows, p.tokens)) * p.hk;
+  p.team = NB == 1 ? steps <= 24 && jobs <= 1024 : steps <= 40 && jobs <= 4096;
   const int scan = WARPS * 4 + (p.rows + 1) * 4 + (p.team ? WARPS * 8 * NB * (D * 4 + 8) : 0);
   static bool configured[64] = {};
   int dev = 0;
@@ -828,9 +833,7 @@ int nb_kv_attention_mode(int mode) {
 
 // Pieces that the batch is cut into, and floats of work space that nb_kv_attention needs.
 int nb_kv_attention_pieces(int) { return 148 * WARPS * 3; }
-// None where tables are so short that a block does a tile.
-long long nb_kv_attention_work(int dim, long long keys) {
-  if (keys <= TEAM * 16 * (128 / dim)) return 0;
+long long nb_kv_attention_work(int dim) {
   return (long long)nb_kv_attention_pieces(dim) * (2 * 16 * (dim + 2) + 4);
 }
 
@@ -845,8 +848,7 @@ int nb_kv_attention(const void* q, void* out, const void* codes, const float* sc
   if ((long long)blocks * hk * block > 0x7fffffffLL - 256) return NB_ERR_TOO_LARGE;   // rows of the copies' tensor
   if (tokens == 0) return NB_OK;
   if ((reinterpret_cast<uintptr_t>(codes) & 15) || (kv_stride & 15)) return NB_ERR_UNALIGNED;
-  const long long floats = nb_kv_attention_work(dim, (long long)width * block);
-  if (floats > 0 && (!work || work_floats < floats || (reinterpret_cast<uintptr_t>(work) & 15))) return NB_ERR_BAD_ARG;
+  if (!work || work_floats < nb_kv_attention_work(dim) || (reinterpret_cast<uintptr_t>(work) & 15)) return NB_ERR_BAD_ARG;
   KvAttn p{};
   p.q = q; p.out = out; p.codes = (const uint8_t*)codes; p.scale = scale; p.tables = tables; p.starts = starts; p.ends = ends;
   p.rows = rows; p.tokens = tokens; p.hq = hq; p.hk = hk; p.group = hq / hk; p.blocks = blocks; p.width = width; p.kv_rows = blocks * hk * block;
@@ -866,16 +868,21 @@ int nb_kv_attention(const void* q, void* out, const void* codes, const float* sc
   p.status = status;
   const cudaStream_t s = (cudaStream_t)stream;
   const int most = max(1, min(max_new, tokens));
-  // Rows with many query rows go to the tensor cores when there are tiles enough to fill the GPU: a tile of 256 query rows walks
-  // its keys alone, while the other kernel spreads the keys of few tiles over all SMs.
+  // Rows with many query rows go to the tensor cores when there are tiles enough: a tile of 256 query rows walks its keys alone,
+  // while the other kernel spreads the keys of few tiles over all SMs.  Measured, other kernel / tiles, 2000 keys behind: one row of
+  // 256 query rows 34 / 52 us, of 512 47 / 56, of 1024 90 / 64 (12 heads of 64: 12, 24, 48 tiles); 256 x 8 heads of 128 44 / 60,
+  // 1024 x 8 (32 tiles) 90 / 62.  Below 64 query rows a row fills a quarter of its tile: 64 rows of 64 100 / 114, of 68 144 / 107.
   const long long units = (long long)tokens * p.group / 256 + min(rows, tokens);
-  if (g_mode != 1 && (long long)most * p.group > FEW && (g_mode == 2 || (long long)tokens * p.group / 256 * hk >= 96) && units * hk <= 0x7fffffffLL) {
+  if (g_mode != 1 && (long long)most * p.group > FEW && (g_mode == 2 || (long long)tokens * p.group / 256 * hk >= 32) && units * hk <= 0x7fffffffLL) {
     p.few = FEW;
     const int rc = kv_launch_prompts(p, dim, (int)units, s);
     if (rc) return rc;
   }
-  // one group of eight query rows where no row of the batch has more; with more, two groups share every conversion of a code
-  const bool one = min((long long)most * p.group, (long long)p.few) <= 8;
+  // Tiles of 16 query rows share every conversion of a code; tiles of 8 are twice as many and spread little work better.  Measured,
+  // 8 / 16 rows: one row of 64 tokens over 2000 keys, 12 heads of 64 (48 tiles of 16) 18 / 28 us, of 256 (192 tiles) 34 / 34, 16 rows
+  // of 32 over 500 (384 tiles) 22 / 16; 32 rows of one token, 16 heads to one (32 tiles), up to 9000 keys 42 / 80; 256 tokens x 32/8
+  // heads of 128 (512 tiles) 107 / 90.
+  const bool one = min((long long)most * p.group, (long long)p.few) <= 8 || (long long)tokens * p.group / 16 * hk < 256;
   if (dim == 64) return one ? launch_few<64, 1>(p, s) : launch_few<64, 2>(p, s);
   return one ? launch_few<128, 1>(p, s) : launch_few<128, 2>(p, s);
 }

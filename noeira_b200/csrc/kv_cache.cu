@@ -61,7 +61,6 @@ __device__ __forceinline__ long long block_scan(long long v, long long* sh, long
 // same banks.
 __host__ __device__ inline int spread(int i) { return i + (i >> 5); }
 
-template <int EACH>
 __global__ void __launch_bounds__(256) kv_plan_kernel(const KvPlan p) {
   extern __shared__ int sm[];
   int* s_start = sm;                 // [rows + 1]
@@ -116,51 +115,32 @@ __global__ void __launch_bounds__(256) kv_plan_kernel(const KvPlan p) {
       *p.free_count_out = free_count - (int)taken;
     }
   }
-  // Neighbouring tokens of a thread share one search, and one look into the table per page; four of them are stored at once.  In a
-  // decode step neighbours belong to different rows, and a thread with four would wait for four tables in turn: one a thread.
-  for (long long t0 = ((long long)blockIdx.x * 256 + tid) * EACH; t0 < p.tokens; t0 += (long long)gridDim.x * 256 * EACH) {
-    int a = 0, b = p.rows;             // last row with start <= t0
+  // A token a thread: four neighbours to a thread, sharing a search and 16-byte stores, waited for their tables in turn and took
+  // longer at every size (64 rows of one token 4.7 us instead of 3.4, 2000 rows of 30 tokens 7.7 instead of 7.2).
+  for (long long t0 = (long long)blockIdx.x * 256 + tid; t0 < p.tokens; t0 += (long long)gridDim.x * 256) {
+    const int t = (int)t0;
+    int a = 0, b = p.rows;             // last row with start <= t
     while (b - a > 1) {
       const int m = (a + b) >> 1;
-      if (s_start[spread(m)] <= (int)t0) a = m; else b = m;
+      if (s_start[spread(m)] <= t) a = m; else b = m;
     }
-    int slot[EACH], pos[EACH], row[EACH], page = -1, id = -1;
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      const int t = (int)t0 + e;       // may pass the last token by three: below 2^31 by the launcher's limit
-      while (a + 1 < p.rows && s_start[spread(a + 1)] <= t) {
-        ++a;
-        page = -1;
+    const bool real = t < s_start[spread(p.rows)];
+    const int len = s_len[spread(a)], off0 = s_off[spread(a)], pos = len + t - s_start[spread(a)];
+    int slot = -1;
+    if (real && off0 >= 0) {
+      const int pg = pos >> p.block_log, in = pos - (pg << p.block_log), have = (int)(((long long)len + (1 << p.block_log) - 1) >> p.block_log);
+      int id;
+      if (pg < have) {
+        id = p.tables[(long long)a * p.width + pg];
+      } else {
+        id = p.free_ids[free_count - 1 - (off0 + pg - have)];
+        if (in == 0) p.tables[(long long)a * p.width + pg] = id;    // the first token of a block: the block is new
       }
-      const bool real = t < s_start[spread(p.rows)] && t < p.tokens;
-      const int len = s_len[spread(a)], at_pos = len + t - s_start[spread(a)];
-      slot[e] = -1;
-      pos[e] = real ? at_pos : 0;
-      row[e] = real ? a : -1;
-      if (real && s_off[spread(a)] >= 0) {
-        const int pg = at_pos >> p.block_log, in = at_pos - (pg << p.block_log);
-        if (pg != page) {
-          const int have = (int)(((long long)len + (1 << p.block_log) - 1) >> p.block_log);
-          id = pg < have ? p.tables[(long long)a * p.width + pg] : p.free_ids[free_count - 1 - (s_off[spread(a)] + pg - have)];
-          page = pg;
-        }
-        if (in == 0) p.tables[(long long)a * p.width + pg] = id;   // the first token of a block: the block is new
-        if (id >= 0) slot[e] = (id << p.block_log) + in;
-      }
+      if (id >= 0) slot = (id << p.block_log) + in;
     }
-    if (EACH == 4 && p.vec && t0 + 4 <= p.tokens) {
-      *reinterpret_cast<int4*>(p.slots + t0) = make_int4(slot[0], slot[1 % EACH], slot[2 % EACH], slot[3 % EACH]);
-      *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1 % EACH], pos[2 % EACH], pos[3 % EACH]);
-      *reinterpret_cast<int4*>(p.row_of + t0) = make_int4(row[0], row[1 % EACH], row[2 % EACH], row[3 % EACH]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < EACH; ++e)
-        if (t0 + e < p.tokens) {
-          p.slots[t0 + e] = slot[e];
-          p.positions[t0 + e] = pos[e];
-          p.row_of[t0 + e] = row[e];
-        }
-    }
+    p.slots[t0] = slot;
+    p.positions[t0] = real ? pos : 0;
+    p.row_of[t0] = real ? a : -1;
   }
 }
 
@@ -204,8 +184,8 @@ constexpr uint32_t BF16_INF = 0x7f80;
 // A run is a stretch of neighbouring tokens and slots inside one block.  A warp takes the runs that begin in a window of `window`
 // tokens, for one head of K or V: D / 8 lanes a token, 16 bytes each, so that a run of up to 32 tokens is read once and stays in
 // registers between the maximum and the codes (longer ones are read again, from the caches).  What continues a run in the same
-// block behind skipped tokens is done by the same warp.  One pass over the input at the copy rate is the bound; windows of one
-// token spread a decode step over the GPU, windows of 32 keep warps with nothing to do few.
+// block behind skipped tokens is done by the same warp.  One pass over the input at the copy rate is the bound; windows of eight
+// tokens spread a decode step over the GPU, windows of 32 keep warps with nothing to do few.
 template <int D>
 __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p) {
   constexpr int LANES = D / 8, TOKENS = 32 / LANES, HELD = 32 / TOKENS;
@@ -232,6 +212,58 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p) {
     if (lane == j && last == my_slot - 1) start = false;
   }
   unsigned runs = __ballot_sync(0xffffffffu, start);
+  // Runs of one token, as in a decode step: several at a time, so that their loads go out together.  One that has to move earlier
+  // codes or holds what is not finite is left to the loop below.
+  int next = __shfl_down_sync(0xffffffffu, my_slot, 1);
+  const long long behind = w0 + lane + 1;
+  const bool more = behind < p.tokens;
+  if (lane == 31 || lane + 1 >= p.window) next = more ? p.slots[behind] : -1;
+  const bool room = ((my_slot + 1) & ((1 << p.block_log) - 1)) != 0;
+  const unsigned single = __ballot_sync(0xffffffffu, start && !(room && more && (next == my_slot + 1 || (unsigned)next >= (unsigned)p.limit)));
+  if (__popc(single) > 1) {
+    constexpr int TURNS = 8 / TOKENS;
+    for (int i0 = 0; i0 < p.window; i0 += 8) {
+      uint4 x[TURNS];
+      float old[TURNS];
+      int slot[TURNS];
+#pragma unroll
+      for (int u = 0; u < TURNS; ++u) {
+        const int j = i0 + u * TOKENS + sub;
+        slot[u] = __shfl_sync(0xffffffffu, my_slot, j & 31);
+        x[u] = make_uint4(0, 0, 0, 0);
+        old[u] = 0.f;
+        if (!((single >> (j & 31)) & 1u) || j >= p.window) {
+          slot[u] = -1;
+        } else {
+          x[u] = eight(input + (w0 + j) * step, vec);
+          if (slot[u] & ((1 << p.block_log) - 1)) old[u] = p.scale[((long long)which * p.blocks + (slot[u] >> p.block_log)) * p.heads + h];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < TURNS; ++u) {
+        uint32_t top = abs_max(0, x[u]);
+        top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const bool first = (slot[u] & ((1 << p.block_log) - 1)) == 0;
+        const float now = fmaxf(old[u], scale_for(__uint_as_float(top << 16)));
+        const bool done = slot[u] >= 0 && top < BF16_INF && (first || now == old[u]);
+        if (done) {
+          const long long bh = ((long long)which * p.blocks + (slot[u] >> p.block_log)) * p.heads + h;
+          const float inv = inv_pow2(now);
+          uint8_t* to = p.codes + (long long)which * p.kv_stride + ((((long long)(slot[u] >> p.block_log)) * p.heads + h) << p.block_log) * D +
+                        (slot[u] & ((1 << p.block_log) - 1)) * D + d;
+          *reinterpret_cast<uint2*>(to) = make_uint2(codes4(x[u].x, x[u].y, inv), codes4(x[u].z, x[u].w, inv));
+          if (first && d == 0) p.scale[bh] = now;
+        }
+        // one lane of each token speaks for it
+        const unsigned said = __ballot_sync(0xffffffffu, done && lane % LANES == 0);
+#pragma unroll
+        for (int k = 0; k < TOKENS; ++k)
+          if ((said >> (k * LANES)) & 1u) runs &= ~(1u << ((i0 + u * TOKENS + k) & 31));
+      }
+    }
+  }
   while (runs) {
     const int j = __ffs(runs) - 1;
     runs &= runs - 1;
@@ -387,23 +419,20 @@ int nb_kv_plan(const int* lengths, const int* new_lens, int* tables, const int* 
                int tokens, unsigned int* status, void* stream) {
   if (rows <= 0 || rows > 8192 || width <= 0 || block <= 0 || tokens < 0 || free_size < 0) return NB_ERR_BAD_ARG;
   if ((block & (block - 1)) || (long long)width * block > 0x7fffff00LL || tokens > 0x7fffff00) return NB_ERR_BAD_ARG;
-  const int each = tokens < 8LL * rows ? 1 : 4, grid = max(1, min(148 * 4, ceil_div(tokens, 256 * each)));
+  const int grid = max(1, min(148 * 4, ceil_div(tokens, 256)));
   // every block reads the count when it begins, so only a single block may write it back in place
   const bool later = grid > 1 && free_count == free_count_out;
-  KvPlan p{lengths, new_lens, tables, free_ids, free_count, later ? own : free_count_out, starts, ends, row_of, positions, slots, rows, width, 0, free_size, tokens, 0, status};
+  KvPlan p{lengths, new_lens, tables, free_ids, free_count, later ? own : free_count_out, starts, ends, row_of, positions, slots, rows, width, 0, free_size, tokens, status};
   while ((1 << p.block_log) < block) ++p.block_log;
-  p.vec = !((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(row_of)) & 15);
   static bool configured[64] = {};
   int dev = 0;
   NB_CUDA(cudaGetDevice(&dev));
   if (dev >= 64) return NB_ERR_BAD_ARG;
   if (!configured[dev]) {
-    NB_CUDA(cudaFuncSetAttribute(kv_plan_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * (8192 + 256 + 1) * 4));
-    NB_CUDA(cudaFuncSetAttribute(kv_plan_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * (8192 + 256 + 1) * 4));
+    NB_CUDA(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * (8192 + 256 + 1) * 4));
     configured[dev] = true;
   }
-  if (each == 1) kv_plan_kernel<1><<<grid, 256, 3 * (spread(rows) + 1) * 4, (cudaStream_t)stream>>>(p);
-  else kv_plan_kernel<4><<<grid, 256, 3 * (spread(rows) + 1) * 4, (cudaStream_t)stream>>>(p);
+  kv_plan_kernel<<<grid, 256, 3 * (spread(rows) + 1) * 4, (cudaStream_t)stream>>>(p);
   NB_LAUNCH_CHECK();
   if (later) NB_CUDA(cudaMemcpyAsync(free_count_out, own, 4, cudaMemcpyDeviceToDevice, (cudaStream_t)stream));
   return NB_OK;
@@ -419,7 +448,7 @@ int nb_kv_append(const void* k, const void* v, void* codes, float* scale, const 
   while ((1 << p.block_log) < block) ++p.block_log;
   p.k_vec = !((reinterpret_cast<uintptr_t>(k) & 15) || (k_token & 7) || (k_head & 7));
   p.v_vec = !((reinterpret_cast<uintptr_t>(v) & 15) || (v_token & 7) || (v_head & 7));
-  p.window = tokens <= 2048 ? 1 : 32;
+  p.window = tokens <= 1024 ? 8 : 32;   // 512 single tokens 3.6 us instead of 7.1; two prompts of 1024 6.5 instead of 8.0
   const dim3 grid(ceil_div(tokens, 4 * p.window), 2 * heads);
   if (dim == 64) kv_append_kernel<64><<<grid, 128, 0, (cudaStream_t)stream>>>(p);
   else kv_append_kernel<128><<<grid, 128, 0, (cudaStream_t)stream>>>(p);

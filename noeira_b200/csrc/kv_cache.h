@@ -12,7 +12,7 @@ struct KvPlan {
   int* tables;
   const int *free_ids, *free_count;
   int *free_count_out, *starts, *ends, *row_of, *positions, *slots;
-  int rows, width, block_log, free_size, tokens, vec;
+  int rows, width, block_log, free_size, tokens;
   unsigned int* status;
 };
 

@@ -255,11 +255,11 @@ def paged_attention(q, kv, scale, tables, starts, ends, max_new=None, softmax_sc
         with guard:
             return paged_attention(q, kv, scale, tables, starts, ends, max_new, softmax_scale, out)
     # partial results of this call alone: calls on two streams, or in two graphs, share nothing
-    floats = _work_floats(dim, width * block)
-    work = scale.new_empty(floats) if floats else None
+    floats = _work_floats(dim)
+    work = scale.new_empty(floats)
     check(cuda_lib().nb_kv_attention(
         q.data_ptr(), out.data_ptr(), kv.data_ptr(), scale.data_ptr(), tables.data_ptr(), starts.data_ptr(), ends.data_ptr(), rows, tokens, max_new, hq, hk, dim,
-        block, blocks, width, qs[0], qs[1], os_[0], os_[1], kv.stride(0), scale.stride(0), softmax_scale, work.data_ptr() if floats else None, floats, status_ptr(dev), raw_stream()), "kv_attention")
+        block, blocks, width, qs[0], qs[1], os_[0], os_[1], kv.stride(0), scale.stride(0), softmax_scale, work.data_ptr(), floats, status_ptr(dev), raw_stream()), "kv_attention")
     return out
 
 
@@ -270,11 +270,11 @@ def set_attention_mode(mode: int) -> int:
     return int(cuda_lib().nb_kv_attention_mode(ctypes.c_int(mode)))
 
 
-@functools.lru_cache(maxsize=256)
-def _work_floats(dim, keys):
+@functools.lru_cache(maxsize=8)
+def _work_floats(dim):
     fn = cuda_lib().nb_kv_attention_work
     fn.restype = ctypes.c_longlong
-    return int(fn(ctypes.c_int(dim), ctypes.c_longlong(keys)))
+    return int(fn(ctypes.c_int(dim)))
 
 
 def _attention_cpu(q, kv, scale, tables, starts, ends, softmax_scale, out):
