@@ -37,6 +37,10 @@ __device__ __forceinline__ float value_of(uint32_t code) {
 }
 
 // ------------------------------------------------------------------------------------------------ plan
+// Sums over the rows (tokens before a row, new blocks before a row), then a search for each token.  Every block does the sums for
+// itself in shared memory: a kernel of its own for them would cost a launch, which is all that a decode step takes (64 rows of one
+// token 3.3 us).  600k tokens of 2048 rows: 12.7 us; the bytes (7.6 MB written) would be 1.2, the sums take half of the rest and the
+// eleven dependent reads of a search the other.
 // Inclusive sum over the block (256 threads); `sh` holds 8 values.
 __device__ __forceinline__ long long block_scan(long long v, long long* sh, long long& total) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -185,7 +189,9 @@ constexpr uint32_t BF16_INF = 0x7f80;
 // tokens, for one head of K or V: D / 8 lanes a token, 16 bytes each, so that a run of up to 32 tokens is read once and stays in
 // registers between the maximum and the codes (longer ones are read again, from the caches).  What continues a run in the same
 // block behind skipped tokens is done by the same warp.  One pass over the input at the copy rate is the bound; windows of eight
-// tokens spread a decode step over the GPU, windows of 32 keep warps with nothing to do few.
+// tokens spread a decode step over the GPU, windows of 32 keep warps with nothing to do few.  26k tokens of 24 prompts, 8 heads of
+// 128 (166 MB): 39 us, 4.3 TB/s; a warp has one run, whose loads, maximum and stores follow one another, and 16 warps fit an SM
+// beside the 64 registers that hold a run.  64 single tokens, 5 heads of 64: 2.6 us.
 template <int D>
 __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p) {
   constexpr int LANES = D / 8, TOKENS = 32 / LANES, HELD = 32 / TOKENS;
@@ -346,7 +352,8 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p) {
 
 // ------------------------------------------------------------------------------------------------ reorder
 // A block per row and four planes (a plane: one layer's keys or values): what a row copies is found out once for them, and their
-// loads go out together.  The table is the first plane's business.
+// loads go out together.  The table is the first plane's business.  384 rows with up to 63 tokens in their last block, 16 layers of 5
+// heads of 64 (112 MB copied): 43 us, 5.1 TB/s read and written (one plane a block: 47); one search of 4 beams, 6 layers: 3.6 us.
 constexpr int PLANES = 4;
 __global__ void __launch_bounds__(128) kv_reorder_kernel(const KvReorder p) {
   const int j = blockIdx.x, g = j / p.beams * p.beams;
