@@ -196,14 +196,14 @@ struct Part {
 };
 
 // ---------------------------------------------------------------- the ring
+constexpr int STAGE = 4096;            // half of it keys, half values
 template <int D>
 struct Shape {
-  static constexpr int SUB = 128 / D;  // sub-tiles of 16 keys in a step
+  static constexpr int SUB = STAGE / 32 / D;   // sub-tiles of 16 keys in a step
   static constexpr int KEYS = 16 * SUB;
 };
-constexpr int STAGE = 4096;            // 2 KB of keys, 2 KB of values
 struct Head {                          // of a stage
-  float ks[2], vs[2];                  // scales of the sub-tiles; a scale below zero: no keys there
+  float ks[STAGE / 2048], vs[STAGE / 2048];   // scales of the sub-tiles; a scale below zero: no keys there
 };
 
 // Byte of 16-byte chunk `ch` of row `r` (0..15) of a sub-tile, as the copy's swizzle leaves it.
@@ -267,8 +267,8 @@ struct Feed {                          // runs over the steps of a warp's piece,
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
         const int y = row[s] + ((step * KEYS + s * 16) & ((1 << p.block_log) - 1));
-        copy_box(stage + s * 1024, map, bar, y, 0);
-        copy_box(stage + 2048 + s * 1024, map, bar, y, 1);
+        copy_box(stage + s * 16 * D, map, bar, y, 0);
+        copy_box(stage + STAGE / 2 + s * 16 * D, map, bar, y, 1);
       }
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
     }
@@ -394,8 +394,8 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
       for (int i = 0; i < 4; ++i) s[u][b][i] = 0.f;
 #pragma unroll
     for (int d = 0; d < D / 64; ++d) {
-      const uint4 x = *reinterpret_cast<const uint4*>(st + u * 1024 + chunk_at<D>(g, d * 4 + c));
-      const uint4 y = *reinterpret_cast<const uint4*>(st + u * 1024 + chunk_at<D>(g + 8, d * 4 + c));
+      const uint4 x = *reinterpret_cast<const uint4*>(st + u * 16 * D + chunk_at<D>(g, d * 4 + c));
+      const uint4 y = *reinterpret_cast<const uint4*>(st + u * 16 * D + chunk_at<D>(g + 8, d * 4 + c));
       const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -472,11 +472,11 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (D == 64) {
-        const uint2 x = *reinterpret_cast<const uint2*>(st + 2048 + u * 1024 + chunk_at<D>(2 * c + (k & 1) + (k >> 1) * 8, g >> 1) + (g & 1) * 8);
+        const uint2 x = *reinterpret_cast<const uint2*>(st + STAGE / 2 + u * 16 * D + chunk_at<D>(2 * c + (k & 1) + (k >> 1) * 8, g >> 1) + (g & 1) * 8);
         v[k][0] = x.x;
         v[k][1] = x.y;
       } else {
-        const uint4 x = *reinterpret_cast<const uint4*>(st + 2048 + u * 1024 + chunk_at<D>(2 * c + (k & 1) + (k >> 1) * 8, g));
+        const uint4 x = *reinterpret_cast<const uint4*>(st + STAGE / 2 + u * 16 * D + chunk_at<D>(2 * c + (k & 1) + (k >> 1) * 8, g));
         v[k][0] = x.x;
         v[k][1] = x.y;
         v[k][D / 32 - 2] = x.z;
@@ -762,14 +762,6 @@ __global__ void __launch_bounds__(THREADS) kv_attn_join_kernel(const KvAttn p) {
 template <int D, int NB>
 int launch_few(KvAttn p, cudaStream_t stream) {
   constexpr int fixed = 1024 + WARPS * STAGES * (STAGE + (int)sizeof(Head) + 8);
-  p.tile = 8 * NB;
-  // Short tables: a block to a tile, its warps taking turns at the steps and joining in shared memory, which saves the second
-  // kernel; where there are many such tiles, pieces spread them better.  Measured, block / pieces: one row of 300 keys 7.8 / 10.5
-  // us, of 640 11.2 / 11.9, of 1200 15.4 / 11.3 (D = 64); 128 rows of 300 keys 15.3 / 18.7, 1024 rows 98 / 64.  Tiles of 16 rows
-  // come several to a row and share its keys: 4 rows of 64 tokens over 560 keys (D = 128) 37 / 53, 64 rows of 17 over 520 50 / 68.
-  const long long steps = (((long long)p.width << p.block_log) + Shape<D>::KEYS - 1) / Shape<D>::KEYS;
-  const long long jobs = ((long long)p.tokens * p.group / p.tile + min(p.rows, p.tokens)) * p.hk;
-  p.team = NB == 1 ? steps <= 24 && jobs <= 1024 : steps <= 40 && jobs <= 4096;
   const int scan = WARPS * 4 + (p.rows + 1) * 4 + (p.team ? WARPS * 8 * NB * (D * 4 + 8) : 0);
   static bool configured[64] = {};
   int dev = 0;
@@ -834,10 +826,51 @@ int nb_kv_attention_mode(int mode) {
   return old;
 }
 
-// Pieces that the batch is cut into, and floats of work space that nb_kv_attention needs.
-int nb_kv_attention_pieces(int) { return 148 * WARPS * 3; }
-long long nb_kv_attention_work(int dim) {
-  return (long long)nb_kv_attention_pieces(dim) * (2 * 16 * (dim + 2) + 4);
+}  // extern "C"
+
+static constexpr int PIECES = 148 * WARPS * 3;                    // the warps that are resident together
+
+// What a call is done by, from its sizes alone.
+struct Plan {
+  bool tiles;                          // rows with more than `few` query rows on the tensor cores
+  int few, units;
+  bool one, team;                      // tiles of 8 query rows, not 16; a block to a tile, not pieces of equal length
+};
+static Plan plan_for(int dim, int rows, int tokens, int max_new, int hq, int hk, long long keys) {
+  Plan r{false, 0x7fffffff, 0, false, false};
+  const int group = hq / hk;
+  const long long most = max(1, min(max_new, tokens));
+  // Rows with many query rows go to the tensor cores when there are tiles enough: a tile of 256 query rows walks its keys alone,
+  // while the other kernel spreads the keys of few tiles over all SMs.  Measured, other kernel / tiles, 2000 keys behind: one row of
+  // 256 query rows 34 / 52 us, of 512 47 / 56, of 1024 90 / 64 (12 heads of 64: 12, 24, 48 tiles); 256 x 8 heads of 128 44 / 60,
+  // 1024 x 8 (32 tiles) 90 / 62.  Below 64 query rows a row fills a quarter of its tile: 64 rows of 64 100 / 114, of 68 144 / 107.
+  const long long units = (long long)tokens * group / 256 + min(rows, tokens);
+  if (g_mode != 1 && most * group > FEW && (g_mode == 2 || (long long)tokens * group / 256 * hk >= 32) && units * hk <= 0x7fffffffLL) {
+    r.tiles = true;
+    r.few = FEW;
+    r.units = (int)units;
+  }
+  // Tiles of 16 query rows share every conversion of a code; tiles of 8 are twice as many and spread little work better.  Measured,
+  // 8 / 16 rows: one row of 64 tokens over 2000 keys, 12 heads of 64 (48 tiles of 16) 18 / 28 us, of 256 (192 tiles) 34 / 34, 16 rows
+  // of 32 over 500 (384 tiles) 22 / 16; 32 rows of one token, 16 heads to one (32 tiles), up to 9000 keys 42 / 80; 256 tokens x 32/8
+  // heads of 128 (512 tiles) 107 / 90.
+  r.one = min(most * group, (long long)r.few) <= 8 || (long long)tokens * group / 16 * hk < 256;
+  // Short tables: a block to a tile, its warps taking turns at the steps and joining in shared memory, which saves the second
+  // kernel; where there are many such tiles, pieces spread them better.  Measured, block / pieces: one row of 300 keys 7.8 / 10.5
+  // us, of 640 11.2 / 11.9, of 1200 15.4 / 11.3 (D = 64); 128 rows of 300 keys 15.3 / 18.7, 1024 rows 98 / 64.  Tiles of 16 rows
+  // come several to a row and share its keys: 4 rows of 64 tokens over 560 keys (D = 128) 37 / 53, 64 rows of 17 over 520 50 / 68.
+  const long long steps = (keys * dim + STAGE / 2 - 1) / (STAGE / 2);
+  const long long jobs = ((long long)tokens * group / (r.one ? 8 : 16) + min(rows, tokens)) * hk;
+  r.team = r.one ? steps <= 24 && jobs <= 1024 : steps <= 40 && jobs <= 4096;
+  return r;
+}
+
+extern "C" {
+
+// Floats of work space that nb_kv_attention needs for these sizes: partial results, where rows are cut into pieces.
+long long nb_kv_attention_work(int dim, int rows, int tokens, int max_new, int hq, int hk, int block, int width) {
+  if (hk <= 0 || hq < hk || tokens <= 0) return 0;
+  return plan_for(dim, rows, tokens, max_new, hq, hk, (long long)width * block).team ? 0 : (long long)PIECES * (2 * 16 * (dim + 2) + 4);
 }
 
 int nb_kv_attention(const void* q, void* out, const void* codes, const float* scale, const int* tables, const int* starts,
@@ -851,7 +884,8 @@ int nb_kv_attention(const void* q, void* out, const void* codes, const float* sc
   if ((long long)blocks * hk * block > 0x7fffffffLL - 256) return NB_ERR_TOO_LARGE;   // rows of the copies' tensor
   if (tokens == 0) return NB_OK;
   if ((reinterpret_cast<uintptr_t>(codes) & 15) || (kv_stride & 15)) return NB_ERR_UNALIGNED;
-  if (!work || work_floats < nb_kv_attention_work(dim) || (reinterpret_cast<uintptr_t>(work) & 15)) return NB_ERR_BAD_ARG;
+  const long long floats = nb_kv_attention_work(dim, rows, tokens, max_new, hq, hk, block, width);
+  if (floats > 0 && (!work || work_floats < floats || (reinterpret_cast<uintptr_t>(work) & 15))) return NB_ERR_BAD_ARG;
   KvAttn p{};
   p.q = q; p.out = out; p.codes = (const uint8_t*)codes; p.scale = scale; p.tables = tables; p.starts = starts; p.ends = ends;
   p.rows = rows; p.tokens = tokens; p.hq = hq; p.hk = hk; p.group = hq / hk; p.blocks = blocks; p.width = width; p.kv_rows = blocks * hk * block;
@@ -863,31 +897,22 @@ int nb_kv_attention(const void* q, void* out, const void* codes, const float* sc
   p.o_vec = !((reinterpret_cast<uintptr_t>(out) & 7) || (o_token & 3) || (o_head & 3));
   p.o_vec16 = !((reinterpret_cast<uintptr_t>(out) & 15) || (o_token & 7) || (o_head & 7));
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  p.pieces = nb_kv_attention_pieces(dim);
+  p.pieces = PIECES;
   p.part_o = work;
   p.part_ml = work + (long long)p.pieces * 2 * 16 * dim;
   p.part_job = (int4*)(p.part_ml + (long long)p.pieces * 2 * 16 * 2);
-  p.few = 0x7fffffff;
   p.status = status;
+  const Plan plan = plan_for(dim, rows, tokens, max_new, hq, hk, (long long)width * block);
   const cudaStream_t s = (cudaStream_t)stream;
-  const int most = max(1, min(max_new, tokens));
-  // Rows with many query rows go to the tensor cores when there are tiles enough: a tile of 256 query rows walks its keys alone,
-  // while the other kernel spreads the keys of few tiles over all SMs.  Measured, other kernel / tiles, 2000 keys behind: one row of
-  // 256 query rows 34 / 52 us, of 512 47 / 56, of 1024 90 / 64 (12 heads of 64: 12, 24, 48 tiles); 256 x 8 heads of 128 44 / 60,
-  // 1024 x 8 (32 tiles) 90 / 62.  Below 64 query rows a row fills a quarter of its tile: 64 rows of 64 100 / 114, of 68 144 / 107.
-  const long long units = (long long)tokens * p.group / 256 + min(rows, tokens);
-  if (g_mode != 1 && (long long)most * p.group > FEW && (g_mode == 2 || (long long)tokens * p.group / 256 * hk >= 32) && units * hk <= 0x7fffffffLL) {
-    p.few = FEW;
-    const int rc = kv_launch_prompts(p, dim, (int)units, s);
+  p.few = plan.few;
+  p.tile = plan.one ? 8 : 16;
+  p.team = plan.team;
+  if (plan.tiles) {
+    const int rc = kv_launch_prompts(p, dim, plan.units, s);
     if (rc) return rc;
   }
-  // Tiles of 16 query rows share every conversion of a code; tiles of 8 are twice as many and spread little work better.  Measured,
-  // 8 / 16 rows: one row of 64 tokens over 2000 keys, 12 heads of 64 (48 tiles of 16) 18 / 28 us, of 256 (192 tiles) 34 / 34, 16 rows
-  // of 32 over 500 (384 tiles) 22 / 16; 32 rows of one token, 16 heads to one (32 tiles), up to 9000 keys 42 / 80; 256 tokens x 32/8
-  // heads of 128 (512 tiles) 107 / 90.
-  const bool one = min((long long)most * p.group, (long long)p.few) <= 8 || (long long)tokens * p.group / 16 * hk < 256;
-  if (dim == 64) return one ? launch_few<64, 1>(p, s) : launch_few<64, 2>(p, s);
-  return one ? launch_few<128, 1>(p, s) : launch_few<128, 2>(p, s);
+  if (dim == 64) return plan.one ? launch_few<64, 1>(p, s) : launch_few<64, 2>(p, s);
+  return plan.one ? launch_few<128, 1>(p, s) : launch_few<128, 2>(p, s);
 }
 
 }  // extern "C"

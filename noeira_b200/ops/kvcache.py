@@ -255,11 +255,11 @@ def paged_attention(q, kv, scale, tables, starts, ends, max_new=None, softmax_sc
         with guard:
             return paged_attention(q, kv, scale, tables, starts, ends, max_new, softmax_scale, out)
     # partial results of this call alone: calls on two streams, or in two graphs, share nothing
-    floats = _work_floats(dim)
-    work = scale.new_empty(floats)
+    floats = _work_floats(dim, rows, tokens, max_new, hq, hk, block, width, _MODE[0])
+    work = scale.new_empty(floats) if floats else None
     check(cuda_lib().nb_kv_attention(
         q.data_ptr(), out.data_ptr(), kv.data_ptr(), scale.data_ptr(), tables.data_ptr(), starts.data_ptr(), ends.data_ptr(), rows, tokens, max_new, hq, hk, dim,
-        block, blocks, width, qs[0], qs[1], os_[0], os_[1], kv.stride(0), scale.stride(0), softmax_scale, work.data_ptr(), floats, status_ptr(dev), raw_stream()), "kv_attention")
+        block, blocks, width, qs[0], qs[1], os_[0], os_[1], kv.stride(0), scale.stride(0), softmax_scale, work.data_ptr() if floats else None, floats, status_ptr(dev), raw_stream()), "kv_attention")
     return out
 
 
@@ -267,14 +267,19 @@ def set_attention_mode(mode: int) -> int:
     """Kernel of rows with more than 64 query rows per head: by problem size (0, default), the one that reads codes straight into the
     fragments of the matrix instructions and spreads a row's keys over the GPU (1), or the one on 256-row tiles of the tensor
     cores (2).  Returns the previous setting."""
-    return int(cuda_lib().nb_kv_attention_mode(ctypes.c_int(mode)))
+    old = int(cuda_lib().nb_kv_attention_mode(ctypes.c_int(mode)))
+    _MODE[0] = mode if 0 <= mode <= 2 else old
+    return old
 
 
-@functools.lru_cache(maxsize=8)
-def _work_floats(dim):
+_MODE = [0]
+
+
+@functools.lru_cache(maxsize=1024)
+def _work_floats(dim, rows, tokens, max_new, hq, hk, block, width, mode):
     fn = cuda_lib().nb_kv_attention_work
     fn.restype = ctypes.c_longlong
-    return int(fn(ctypes.c_int(dim)))
+    return int(fn(*map(ctypes.c_int, (dim, rows, tokens, max_new, hq, hk, block, width))))
 
 
 def _attention_cpu(q, kv, scale, tables, starts, ends, softmax_scale, out):
