@@ -5,8 +5,8 @@
 // 64 bits.  Ties go to the lowest b * vocab + v.  NaN counts as -inf, +inf as the largest finite number.
 //
 // One pass over the logits, which is all that there is to read (R * beams * vocab elements at the copy rate), split over blocks of
-// one part of one beam's row each, the elements in registers.  The block's maximum and sum come first; then the K = beams best of
-// its elements: the K-th largest of a warp's lane maxima is a lower bound of the block's K-th element, and the largest of these
+// one part of one beam's row each, the elements in registers.  The maximum and sum of each warp come first; then the K = beams best
+// of the block's elements: the K-th largest of a warp's lane maxima is a lower bound of the block's K-th element, and the largest of these
 // bounds over the warps leaves few elements above it (about 2 K of 8192 in random order, and never more than K lanes' shares per
 // warp), which are ranked by counting.  A second kernel, a block per request, joins the parts of each beam and ranks the beams.
 // 48 x 8 beams over 32003 fp32 logits (49 MB): 27 us, the pass 19 of them: 15 instructions a logit and 350 a warp for the maxima,
@@ -59,7 +59,7 @@ __device__ __forceinline__ Key warp_best(Key k) {
 template <bool FP32, int EACH, bool WIDE>
 __global__ void __launch_bounds__(THREADS) beam_part_kernel(const BeamSel p) {
   constexpr int VEC = WIDE ? (FP32 ? 4 : 8) : 1, SIZE = FP32 ? 4 : 2;   // neighbouring elements of a thread, bytes of an element
-  __shared__ float sh[32];
+  __shared__ float2 sum_sh[THREADS / 32];            // maximum, sum of exponentials of each warp
   __shared__ Key bound_sh[THREADS / 32];
   __shared__ int found;
   extern __shared__ Key cand[];                      // the elements above the bound
@@ -114,21 +114,25 @@ __global__ void __launch_bounds__(THREADS) beam_part_kernel(const BeamSel p) {
   const int at_best = first + (best / VEC) * THREADS * VEC + best % VEC;
   const Key mine = at_best < p.vocab ? key_of(m, at_best) : 0;   // this thread's best; 0: it has no element
   if (tid == 0) found = 0;
-  const float top = block_max(m, sh);                // its barriers publish `found` too
-  const float from = top == -INFINITY ? 0.f : top;
+  // a warp's sum is relative to its own maximum: nothing waits for the block's
+  const float top = warp_max(m), from = top == -INFINITY ? 0.f : top;
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const float d = x[i] - from;
     s += ex2(fmaf(d, 1.44269502f, d * 1.92596303e-8f));     // log2(e) in two parts: the first alone is off by 2^-26, always the same way
   }
+  s = warp_sum(s);
   Key left = mine, bound = 0;
   for (int k = 0; k < K; ++k) {
     bound = warp_best(left);
     if (left == bound) left = 0;
   }
-  if (lane == 0) bound_sh[warp] = bound;
-  s = block_sum(s, sh);                              // publishes the bounds
+  if (lane == 0) {
+    bound_sh[warp] = bound;
+    sum_sh[warp] = make_float2(top, s);
+  }
+  __syncthreads();
 #pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) bound = max(bound, bound_sh[w]);
   if (mine >= bound && mine != 0) {
@@ -144,11 +148,20 @@ __global__ void __launch_bounds__(THREADS) beam_part_kernel(const BeamSel p) {
   }
   __syncthreads();
   const long long at = row * p.parts + part;
-  if (tid == 0) p.part_ms[at] = make_float2(top, s);
+  if (tid == 0) {
+    float2 all = sum_sh[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 32; ++w) all.x = fmaxf(all.x, sum_sh[w].x);
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) sum += sum_sh[w].x == -INFINITY ? 0.f : sum_sh[w].y * expf(sum_sh[w].x - all.x);
+    p.part_ms[at] = make_float2(all.x, sum);
+  }
   const int n = found;
   for (int i = tid; i < n; i += THREADS) {
     const Key k = cand[i];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) rank += cand[j] > k;
     if (rank < K) p.part_key[at * K + rank] = k;
   }
@@ -159,6 +172,7 @@ __global__ void __launch_bounds__(THREADS) beam_part_kernel(const BeamSel p) {
 __global__ void __launch_bounds__(THREADS) beam_join_kernel(const BeamSel p) {
   __shared__ unsigned long long val[32 * 32];        // order of the value as an unsigned number; 0: no candidate
   __shared__ long long idx[32 * 32];                 // b * vocab + v
+  __shared__ Key key_sh[THREADS / 32][64];
   const int r = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, K = p.beams;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int b = warp; b < K; b += THREADS / 32) {
@@ -185,29 +199,54 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const BeamSel p) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       const double lsum = log(s);
-      // K rounds of the largest key below the last one; each lane looks through its own
       const int m = p.parts * K;
       const Key* keys = p.part_key + row * m;
-      constexpr int HELD = 8;                        // in registers, more are read again
-      Key held[HELD];
-#pragma unroll
-      for (int i = 0; i < HELD; ++i) held[i] = lane + 32 * i < m ? keys[lane + 32 * i] : 0;
-      Key last = ~0ULL;
-      for (int k = 0; k < K; ++k) {
-        Key best = 0;
-#pragma unroll
-        for (int i = 0; i < HELD; ++i) best = held[i] < last && held[i] > best ? held[i] : best;
-        for (int i = lane + 32 * HELD; i < m; i += 32) {
-          const Key y = keys[i];
-          best = y < last && y > best ? y : best;
+      Key mine = 0;                                  // the lane-th best
+      if (m <= 64) {
+        // few: the rank of each among all
+        const Key k0 = lane < m ? keys[lane] : 0, k1 = lane + 32 < m ? keys[lane + 32] : 0;
+        Key* all = key_sh[warp];
+        all[lane] = k0;
+        all[lane + 32] = k1;
+        __syncwarp();
+        int r0 = 0, r1 = 0;
+#pragma unroll 8
+        for (int j = 0; j < m; ++j) {
+          const Key y = all[j];
+          r0 += y > k0;
+          r1 += y > k1;
         }
-        last = warp_best(best);
-        if (lane == k && last) {
-          const float x = value_of(last);
-          at = (long long)b * p.vocab + (int)~(uint32_t)last;
-          if (x > -INFINITY && score > -INFINITY) v = score + ((double)x - (double)from - lsum);
+        __syncwarp();
+        all[lane] = 0;
+        __syncwarp();
+        if (k0 && r0 < K) all[r0] = k0;
+        if (k1 && r1 < K) all[r1] = k1;
+        __syncwarp();
+        mine = all[lane];
+        __syncwarp();
+      } else {
+        // K rounds of the largest key below the last one; each lane looks through its own
+        constexpr int HELD = 8;                      // in registers, more are read again
+        Key held[HELD];
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) held[i] = lane + 32 * i < m ? keys[lane + 32 * i] : 0;
+        Key last = ~0ULL;
+        for (int k = 0; k < K && last; ++k) {        // zero: fewer tokens than beams
+          Key best = 0;
+#pragma unroll
+          for (int i = 0; i < HELD; ++i) best = held[i] < last && held[i] > best ? held[i] : best;
+          for (int i = lane + 32 * HELD; i < m; i += 32) {
+            const Key y = keys[i];
+            best = y < last && y > best ? y : best;
+          }
+          last = warp_best(best);
+          if (lane == k) mine = last;
         }
-        if (last == 0) break;                        // fewer tokens than beams
+      }
+      if (mine && lane < K) {
+        const float x = value_of(mine);
+        at = (long long)b * p.vocab + (int)~(uint32_t)mine;
+        if (x > -INFINITY && score > -INFINITY) v = score + ((double)x - (double)from - lsum);
       }
     }
     if (lane < K) {
@@ -224,6 +263,7 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const BeamSel p) {
     const long long at = idx[i];
     if (u == 0) continue;
     int rank = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) rank += val[j] > u || (val[j] == u && idx[j] < at);
     if (rank < K) {
       const long long o = (long long)r * K + rank;
