@@ -9,8 +9,8 @@
 // of the block's elements: the K-th largest of a warp's lane maxima is a lower bound of the block's K-th element, and the largest of these
 // bounds over the warps leaves few elements above it (about 2 K of 8192 in random order, and never more than K lanes' shares per
 // warp), which are ranked by counting.  A second kernel, a block per request, joins the parts of each beam and ranks the beams.
-// 48 x 8 beams over 32003 fp32 logits (49 MB): 27 us, the pass 19 of them: 15 instructions a logit and 350 a warp for the maxima,
-// bounds and sums of a part.  1 x 4 over 49152 bf16 logits: 7 us, two launches.
+// 48 x 8 beams over 32003 fp32 logits (49 MB): 24 us, the pass about 18 of them: 15 instructions a logit and 300 a warp for the
+// maximum, bound and sum of a part, then the join's chain of reads and ranks.  1 x 4 over 49152 bf16 logits: 7 us, two launches.
 #include "common.cuh"
 
 namespace {
@@ -295,7 +295,8 @@ int launch_parts(const BeamSel& p, cudaStream_t s) {
 }
 
 // Elements of a thread: long parts read with more loads in flight and leave less to join; short ones spread few rows over the GPU.
-// Measured, 8 / 32 (vocabulary 49152): 4 rows 7.4 / 8.2 us, 16 rows 8.6 / 8.8, 32 rows 15.4 / 14.0, 64 rows 19.2 / 15.4.
+// Measured, 8 / 32 (vocabulary 49152): 4 rows 7.4 / 8.2 us, 16 rows 8.6 / 8.8, 32 rows 15.4 / 14.0, 64 rows 19.2 / 15.4 (the pass as
+// it is, the join with rounds where it counts ranks now).
 int elements_each(long long rows, int vocab) { return rows * ceil_div(vocab, THREADS * 32) >= 148 ? 32 : 8; }
 
 }  // namespace

@@ -90,7 +90,7 @@ def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free
         free_count_out = free_count
     # one allocation; its last word is the kernel's own
     buf = torch.empty(3 * tokens + 2 * rows + 2, dtype=torch.int32, device=tables.device)
-    slots, positions, row_of, starts, ends, _ = buf.split_with_sizes((tokens, tokens, tokens, rows + 1, rows, 1))
+    slots, positions, row_of, starts, ends, _ = torch.unsafe_split_with_sizes(buf, (tokens, tokens, tokens, rows + 1, rows, 1))   # integers: no autograd to track views for
     at = buf.data_ptr()
     to = at + 12 * tokens
     check(cuda_lib().nb_kv_plan(
