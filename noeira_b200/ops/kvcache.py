@@ -8,7 +8,8 @@ blocks that its line of ``tables`` int32 ``[rows, width]`` names; token number `
 ``starts[i] .. starts[i + 1]`` of the token dimension.
 
 None of the calls synchronises.  What only the device can see (no free block, a bad block id) is reported through the status
-word (``ops.check_status``) and never touches memory outside the tensors.
+word (``ops.check_status``) and never touches memory outside the tensors; on CPU tensors, whose forms compute in fp32, the same
+raises ``RuntimeError`` or ``ValueError``.
 """
 from __future__ import annotations
 
