@@ -544,3 +544,42 @@ def test_attention_prompts_in_a_batch_of_many_rows():
     out = run_attention(d)
     clean()
     assert np.all(np.abs(out[: d["T"]].cpu().double().numpy() - want) <= bound(q, d, want, A, 0.125))
+
+
+@pytest.mark.parametrize("case", [C.ATTENTION[3], C.ATTENTION[7], C.ATTENTION[12], C.PROMPTS[1], C.PROMPTS[3]])
+def test_attention_queries_on_odd_addresses(case, mode):
+    """Query rows that begin on no 16-byte boundary, as views of a wider matrix, give the bits of aligned ones."""
+    from noeira_b200.ops import kvcache
+    d = C.attention_inputs(case)
+    T, hq, dim = d["T"], d["hq"], d["dim"]
+    q = d["q"][:T, 1: 1 + hq].contiguous().cuda()
+    wide = torch.zeros(T, hq * dim + 3, dtype=torch.bfloat16, device="cuda")
+    odd = wide[:, 1: 1 + hq * dim].unflatten(1, (hq, dim))
+    odd.copy_(q)
+    rest = (d["codes"].cuda(), d["scale"].cuda(), d["tables"].cuda(), d["starts"].cuda(), d["ends"].cuda(), d["max_new"])
+    a, b = kvcache.paged_attention(q, *rest), kvcache.paged_attention(odd, *rest)
+    clean()
+    assert torch.equal(a, b)
+
+
+def test_plan_in_a_captured_graph_counts_down():
+    """A plan of many tokens, captured with its counter in place: each replay takes the next blocks."""
+    from noeira_b200.ops import kvcache
+    rows, new, width = 40, 20, 12
+    tables = torch.full((rows, width), -1, dtype=I32, device="cuda")
+    lengths, free, count = torch.zeros(rows, dtype=I32, device="cuda"), torch.arange(rows * width, dtype=I32, device="cuda"), ints([rows * width])
+    add = torch.full((rows,), new, dtype=I32, device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        p = kvcache.plan_tokens(tables, lengths, add, free, count, 16, rows * new)
+        lengths.copy_(p.ends)
+    left = rows * width
+    for n in range(1, 9):
+        g.replay()
+        torch.cuda.synchronize()
+        left -= rows * (-(-n * new // 16) + -(n - 1) * new // 16)
+        used = tables[tables >= 0]
+        assert int(count) == left and bool((lengths == n * new).all()) and used.numel() == rows * width - left == used.unique().numel()
+    clean()
