@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(256) kv_plan_kernel(const KvPlan p) {
       if (id >= 0) slot = (id << p.block_log) + in;
     }
     p.slots[t0] = slot;
-    p.positions[t0] = real ? pos : 0;
+    p.positions[t0] = slot >= 0 ? pos : 0;   // a place that the row does not have is none to look up: it may lie anywhere
     p.row_of[t0] = real ? a : -1;
   }
 }

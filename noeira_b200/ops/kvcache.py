@@ -35,7 +35,7 @@ class TokenPlan(NamedTuple):
     starts: torch.Tensor       # int32 [rows + 1] first token of each row
     ends: torch.Tensor         # int32 [rows]     tokens that the row holds after the call
     rows: torch.Tensor         # int32 [tokens]   row of each token, -1 behind the last
-    positions: torch.Tensor    # int32 [tokens]   place of each token in its row, 0 behind the last
+    positions: torch.Tensor    # int32 [tokens]   place of each token in its row, 0 where it has no slot
     slots: torch.Tensor        # int32 [tokens]   slot of each token, -1 where there is none
     free_count: torch.Tensor   # int32 [1]        free blocks that are left
 
@@ -124,9 +124,9 @@ def _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_c
         off += need
         for t in range(first, min(at, tokens)):
             p = held + t - first
-            row_of[t], positions[t] = i, p
+            row_of[t] = i
             if ok and int(tables[i, p // block]) >= 0:
-                slots[t] = int(tables[i, p // block]) * block + p % block
+                slots[t], positions[t] = int(tables[i, p // block]) * block + p % block, p
     if refused:
         raise RuntimeError(f"key / value cache: rows {refused} found no room")
     out = free_count if free_count_out is None else free_count_out
