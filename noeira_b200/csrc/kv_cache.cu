@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(256) kv_plan_kernel(const KvPlan p) {
     const int len = s_len[spread(i)], given = s_off[spread(i)], add = max(0, given);
     s_start[spread(i)] = (int)min(at, 0x7fffffffLL);
     at += add;
-    const bool fits = len >= 0 && given >= 0 && (long long)len + add <= ((long long)p.width << p.block_log) && at <= p.tokens;
+    const bool fits = len >= 0 && given >= 0 && (long long)len + add <= p.limit && at <= p.tokens;
     s_off[spread(i)] = fits ? ((len + add + (1 << p.block_log) - 1) >> p.block_log) - ((len + (1 << p.block_log) - 1) >> p.block_log) : -1;
     sum += max(0, s_off[spread(i)]);
   }
@@ -419,17 +419,17 @@ __global__ void __launch_bounds__(128) kv_reorder_kernel(const KvReorder p) {
 
 extern "C" {
 
-// Block tables and slot maps.  rows <= 8192; `tables` int32 [rows, width] is completed in place; `free_count_out` may be
-// `free_count`; `own`: one word of work space.
+// Block tables and slot maps.  rows <= 8192; `tables` int32 [rows, width] is completed in place; a row holds at most `limit` tokens,
+// width * block at most; `free_count_out` may be `free_count`; `own`: one word of work space.
 int nb_kv_plan(const int* lengths, const int* new_lens, int* tables, const int* free_ids, const int* free_count, int* free_count_out,
                int* starts, int* ends, int* row_of, int* positions, int* slots, int* own, int rows, int width, int block, int free_size,
-               int tokens, unsigned int* status, void* stream) {
+               int tokens, int limit, unsigned int* status, void* stream) {
   if (rows <= 0 || rows > 8192 || width <= 0 || block <= 0 || tokens < 0 || free_size < 0) return NB_ERR_BAD_ARG;
-  if ((block & (block - 1)) || (long long)width * block > 0x7fffff00LL || tokens > 0x7fffff00) return NB_ERR_BAD_ARG;
+  if ((block & (block - 1)) || (long long)width * block > 0x7fffff00LL || tokens > 0x7fffff00 || limit < 0 || limit > (long long)width * block) return NB_ERR_BAD_ARG;
   const int grid = max(1, min(148 * 4, ceil_div(tokens, 256)));
   // every block reads the count when it begins, so only a single block may write it back in place
   const bool later = grid > 1 && free_count == free_count_out;
-  KvPlan p{lengths, new_lens, tables, free_ids, free_count, later ? own : free_count_out, starts, ends, row_of, positions, slots, rows, width, 0, free_size, tokens, status};
+  KvPlan p{lengths, new_lens, tables, free_ids, free_count, later ? own : free_count_out, starts, ends, row_of, positions, slots, rows, width, 0, free_size, tokens, limit, status};
   while ((1 << p.block_log) < block) ++p.block_log;
   static bool configured[64] = {};
   int dev = 0;

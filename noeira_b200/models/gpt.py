@@ -102,7 +102,10 @@ class GPT(Module):
     @torch.no_grad()
     def forward_cached(self, ids: torch.Tensor, cache, plan, max_new: int = None):
         """New tokens ``ids [tokens]`` of the cache's rows (``plan = cache.plan(new_lens, tokens)``) → logits ``[rows, vocab]`` of each
-        row's last new token.  Rows without new tokens get those of a neighbour, which mean nothing."""
+        row's last new token.  Rows without new tokens get those of a neighbour, which mean nothing.  The cache's ``max_len`` may
+        not pass ``seq``, behind which there are no positions."""
+        if cache.max_len > self.seq:
+            raise ValueError(f"forward_cached: a cache of rows of up to {cache.max_len} tokens, the model has {self.seq} positions")
         x = self.wte.forward(ids) + self.wpe.forward(plan.positions)
         for layer, b in enumerate(self.blocks):
             x = b.forward_cached(x, cache, layer, plan, max_new=max_new)

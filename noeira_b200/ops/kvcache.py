@@ -57,15 +57,15 @@ def _ints(name, t, device, numel=None):
 
 
 # ------------------------------------------------------------------------------------------------ plan
-def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out=None) -> TokenPlan:
+def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out=None, max_len=None) -> TokenPlan:
     """Gives every row the blocks for ``new_lens[i]`` more tokens and every token its slot.
 
     ``tables`` int32 ``[rows, width]`` is completed in place; ``lengths`` / ``new_lens`` int32 ``[rows]``; ``free`` int32 is a
     stack of free block ids of which the first ``free_count`` (int32 ``[1]``) are there; ``tokens`` is the size of the token
     dimension.  Blocks come off the top of the stack in row order.  A row is refused (slots -1, length unchanged, status word)
-    when the stack has too few blocks left for it, when it outgrows its table or the token dimension, or when a length is
-    negative; behind a row that the stack could not serve, only rows that need no new block are served.  ``free_count`` is
-    updated in place unless ``free_count_out`` is given.
+    when the stack has too few blocks left for it, when it outgrows its table, ``max_len`` tokens (default: what its table has
+    room for) or the token dimension, or when a length is negative; behind a row that the stack could not serve, only rows that
+    need no new block are served.  ``free_count`` is updated in place unless ``free_count_out`` is given.
     """
     dev = tables.get_device()
     shape = tables.shape
@@ -81,12 +81,15 @@ def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free
         _ints("free_count_out", free_count_out, dev, 1)
     if block not in BLOCKS or not 0 <= tokens <= 0x7fffff00 or width * block > 0x7fffff00:
         raise ValueError(f"block {block}, tokens {tokens}, width {width}: blocks of {BLOCKS} tokens, fewer than 2^31 tokens")
+    limit = width * block if max_len is None else min(int(max_len), width * block)
+    if limit < 0:
+        raise ValueError(f"max_len: not negative, got {max_len}")
     if dev < 0:
-        return _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out)
+        return _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out, limit)
     guard = _on(tables)
     if guard is not None:
         with guard:
-            return plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out)
+            return plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out, max_len)
     if free_count_out is None:
         free_count_out = free_count
     # one allocation; its last word is the kernel's own
@@ -96,12 +99,12 @@ def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free
     to = at + 12 * tokens
     check(cuda_lib().nb_kv_plan(
         lengths.data_ptr(), new_lens.data_ptr(), tables.data_ptr(), free.data_ptr(), free_count.data_ptr(), free_count_out.data_ptr(), to, to + 4 * rows + 4,
-        at + 8 * tokens, at + 4 * tokens, at, to + 8 * rows + 4, rows, width, block, free.numel(), tokens, status_ptr(dev), raw_stream()), "kv_plan")
+        at + 8 * tokens, at + 4 * tokens, at, to + 8 * rows + 4, rows, width, block, free.numel(), tokens, limit, status_ptr(dev), raw_stream()), "kv_plan")
     return TokenPlan(starts, ends, row_of, positions, slots, free_count_out)
 
 
-def _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out):
-    rows, width = tables.shape
+def _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out, limit):
+    rows = tables.shape[0]
     count = max(0, min(int(free_count), free.numel()))
     starts, ends = torch.zeros(rows + 1, dtype=torch.int32), lengths.clone()
     row_of, positions, slots = (torch.full((tokens,), v, dtype=torch.int32) for v in (-1, 0, -1))
@@ -110,7 +113,7 @@ def _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_c
         held, new = int(lengths[i]), int(new_lens[i])
         first, at = at, at + max(new, 0)
         starts[i + 1] = min(at, 0x7fffffff)
-        fits = held >= 0 and new >= 0 and held + new <= width * block and at <= tokens
+        fits = held >= 0 and new >= 0 and held + new <= limit and at <= tokens
         need = -(-(held + new) // block) + -held // block if fits else 0
         ok = fits and (need == 0 or off + need <= count)
         if ok:
@@ -356,7 +359,7 @@ class PagedKVCache:
 
     def plan(self, new_lens, tokens) -> TokenPlan:
         """Room for ``new_lens[i]`` more tokens in row ``i``; the rows' lengths count them from here on."""
-        plan = plan_tokens(self.tables, self.lengths, new_lens, self.free, self.free_count, self.block, tokens)
+        plan = plan_tokens(self.tables, self.lengths, new_lens, self.free, self.free_count, self.block, tokens, max_len=self.max_len)
         self.lengths.copy_(plan.ends)
         return plan
 

@@ -1,0 +1,60 @@
+"""Paged 8-bit cache, beam search and GPT's answers on CPU tensors at the borders of what their calls allow."""
+import pytest
+import torch
+
+from noeira_b200.models.gpt import GPT
+from noeira_b200.ops import kvcache
+
+I32 = torch.int32
+
+
+def ints(v):
+    return torch.tensor(v, dtype=I32)
+
+
+# ------------------------------------------------------------------------------------------------ plan
+@pytest.mark.parametrize("block", [16, 32])
+def test_rows_hold_max_len_tokens_and_no_more(block):
+    c = kvcache.PagedKVCache(1, 1, 64, 8, 2, 18, block, device="cpu")
+    p = c.plan(ints([18, 17]), 35)
+    assert p.positions.tolist() == list(range(18)) + list(range(17)) and min(p.slots.tolist()) >= 0
+    assert c.plan(ints([0, 1]), 1).positions.tolist() == [17]
+    for new in ([1, 0], [0, 10]):
+        with pytest.raises(RuntimeError, match="no room"):
+            c.plan(ints(new), sum(new))
+    assert c.lengths.tolist() == [18, 18]
+
+
+def test_plan_tokens_takes_a_limit():
+    ok = dict(tables=torch.full((2, 3), -1, dtype=I32), lengths=ints([0, 0]), new_lens=ints([20, 1]), free=ints([0, 1, 2, 3]), free_count=ints([4]), block=16, tokens=21)
+    kvcache.plan_tokens(**{**ok, "free_count": ints([4]), "max_len": 20})
+    kvcache.plan_tokens(**{**ok, "free_count": ints([4]), "max_len": 1 << 40})        # no more than the table has room for
+    with pytest.raises(RuntimeError, match=r"rows \[0\]"):
+        kvcache.plan_tokens(**ok, max_len=19)
+    with pytest.raises(ValueError, match="max_len"):
+        kvcache.plan_tokens(**ok, max_len=-1)
+
+
+# ------------------------------------------------------------------------------------------------ GPT
+def small(**kw):
+    return GPT(**{**dict(vocab=32, seq=20, dim=64, layers=1, heads=1, seed=3), **kw}).eval()
+
+
+def test_gpt_answers_up_to_its_last_position():
+    """``seq`` is no multiple of the block."""
+    m = small()
+    cache = m.new_cache(1, 20)
+    ids = torch.arange(19)
+    m.forward_cached(ids, cache, cache.plan(ints([19]), 19))
+    assert bool(torch.isfinite(m.forward_cached(ids[:1], cache, cache.plan(ints([1]), 1))).all())
+    with pytest.raises(RuntimeError, match="no room"):
+        cache.plan(ints([1]), 1)
+    assert len(m.generate([[1] * 15], max_new=5)[0]) == 5
+
+
+def test_gpt_refuses_a_cache_of_longer_rows():
+    m = small()
+    cache = kvcache.PagedKVCache(1, 1, 64, 4, 1, 21, device="cpu")
+    plan = cache.plan(ints([2]), 2)
+    with pytest.raises(ValueError, match="20 positions"):
+        m.forward_cached(torch.zeros(2, dtype=torch.int64), cache, plan)

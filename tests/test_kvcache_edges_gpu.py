@@ -50,3 +50,19 @@ def test_tokens_of_refused_rows_have_place_zero(lengths, new, width, free, token
     assert np.array_equal(slots, want["slots"]) and np.array_equal(p.rows.cpu().numpy(), want["rows"])
     assert np.array_equal(positions, np.where(want["slots"] >= 0, want["positions"], 0))
     assert positions.min() >= 0 and positions.max() < width * 16
+
+
+@pytest.mark.parametrize("block", [16, 32])
+def test_rows_hold_max_len_tokens_and_no_more(block):
+    """A length that is no multiple of the block: the last block has places behind it, which belong to no token."""
+    from noeira_b200.ops import kvcache
+    c = kvcache.PagedKVCache(1, 1, 64, 8, 2, 18, block)
+    p = c.plan(ints([18, 17]), 35)
+    clean()
+    assert p.positions.tolist() == list(range(18)) + list(range(17)) and min(p.slots.tolist()) >= 0
+    p = c.plan(ints([1, 1]), 2)
+    reported("no room")
+    assert p.positions.tolist() == [0, 17] and p.slots.tolist()[0] == -1 and c.lengths.tolist() == [18, 18]
+    p = c.plan(ints([0, 10]), 10)
+    reported("no room")
+    assert p.positions.tolist() == [0] * 10 and p.slots.tolist() == [-1] * 10 and c.lengths.tolist() == [18, 18]
