@@ -106,10 +106,14 @@ class GPT(Module):
         not pass ``seq``, behind which there are no positions."""
         if cache.max_len > self.seq:
             raise ValueError(f"forward_cached: a cache of rows of up to {cache.max_len} tokens, the model has {self.seq} positions")
-        x = self.wte.forward(ids) + self.wpe.forward(plan.positions)
+        T = ids.numel()
+        if ids.dim() != 1 or T == 0 or plan.positions.shape != ids.shape:
+            raise ValueError(f"forward_cached: ids of the {plan.positions.numel()} tokens of the plan, one at least, got {tuple(ids.shape)}")
+        # a plan that was refused is known only later: what it names is looked up inside the tables
+        x = self.wte.forward(ids) + self.wpe.forward(plan.positions.clamp(0, self.seq - 1))
         for layer, b in enumerate(self.blocks):
             x = b.forward_cached(x, cache, layer, plan, max_new=max_new)
-        h = self.ln_f.forward(x.index_select(0, (plan.starts[1:] - 1).clamp_min(0)))
+        h = self.ln_f.forward(x.index_select(0, (plan.starts[1:] - 1).clamp(0, T - 1)))
         if not self.tie:
             return self.head.forward(h)
         if h.is_cuda:

@@ -58,3 +58,27 @@ def test_gpt_refuses_a_cache_of_longer_rows():
     plan = cache.plan(ints([2]), 2)
     with pytest.raises(ValueError, match="20 positions"):
         m.forward_cached(torch.zeros(2, dtype=torch.int64), cache, plan)
+
+
+def test_gpt_looks_up_places_inside_its_tables_only():
+    """What a refused plan holds on the GPU, where nothing raises: rows that start behind the tokens, places of any size."""
+    m = small()
+    cache = m.new_cache(3, 20)
+    plan = cache.plan(ints([2, 3, 0]), 5)
+    ids = torch.tensor([1, 2, 3, 4, 5])
+    want = m.forward_cached(ids, cache, plan)
+    got = m.forward_cached(ids, cache, plan._replace(starts=ints([0, 2, 5, 9])))
+    assert torch.equal(got[:2], want[:2]) and bool(torch.isfinite(got).all())
+    got = m.forward_cached(ids, cache, plan._replace(positions=ints([0, 1, 20, -7, 0x7fffffff])))
+    assert torch.equal(got[0], want[0]) and bool(torch.isfinite(got).all())
+
+
+def test_gpt_refuses_ids_that_are_not_the_plans():
+    m = small()
+    cache = m.new_cache(2, 20)
+    plan = cache.plan(ints([2, 1]), 3)
+    for ids in (torch.zeros(1, dtype=torch.int64), torch.zeros(4, dtype=torch.int64), torch.zeros(1, 3, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="3 tokens"):
+            m.forward_cached(ids, cache, plan)
+    with pytest.raises(ValueError, match="one at least"):
+        m.forward_cached(torch.zeros(0, dtype=torch.int64), cache, cache.plan(ints([0, 0]), 0))
