@@ -129,6 +129,8 @@ class GPT(Module):
         lens = [len(p) for p in prompts]
         if not lens or min(lens) == 0 or beams < 1 or max_new < 1:
             raise ValueError("beam_search: prompts of at least one token, at least one beam and one new token")
+        if not all(0 <= t < self.vocab for p in prompts for t in p):
+            raise ValueError(f"beam_search: prompts of the model's {self.vocab} tokens, got {[t for p in prompts for t in p if not 0 <= t < self.vocab][:4]}")
         R, rows, dev = len(lens), len(lens) * beams, self.wte.weight.data.device
         cache = self.new_cache(rows, max(lens) + max_new, block, spares=beams > 1)
         new = torch.zeros(R, beams, dtype=torch.int32)

@@ -82,3 +82,12 @@ def test_gpt_refuses_ids_that_are_not_the_plans():
             m.forward_cached(ids, cache, plan)
     with pytest.raises(ValueError, match="one at least"):
         m.forward_cached(torch.zeros(0, dtype=torch.int64), cache, cache.plan(ints([0, 0]), 0))
+
+
+@pytest.mark.parametrize("bad", [32, -1, 1 << 40])
+def test_gpt_refuses_prompts_of_other_tokens(bad):
+    m = small()
+    for answer in (m.beam_search, m.generate):
+        with pytest.raises(ValueError, match="32 tokens"):
+            answer([[1, 2], [3, bad, 4]], max_new=2)
+    assert len(m.generate([[0, 31]], max_new=2)[0]) == 2
