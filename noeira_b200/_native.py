@@ -178,7 +178,7 @@ _SIGNATURES = {
     "nb_norm_fwd": "pipppip" + "iifip",
     "nb_bn_fwd": "pppppppppp" + "liffiip",
     "nb_act_fwd": "pplip", "nb_act_bwd": "ppplip",
-    "nb_kv_plan": "p" * 12 + "iiiiiipp", "nb_kv_append": "ppppp" + "iiiii" + "lllllp",
+    "nb_kv_plan": "p" * 12 + "iiiiiiipp", "nb_kv_append": "ppppp" + "iiiii" + "lllllp",
     "nb_kv_attention": "p" * 7 + "i" * 9 + "llllll" + "fplpp", "nb_kv_reorder": "p" * 9 + "i" * 8 + "pp",
     "nb_beam_select": "p" * 7 + "iiiiilplp",
 }

@@ -138,9 +138,11 @@ __global__ void __launch_bounds__(256) kv_plan_kernel(const KvPlan p) {
         id = p.tables[(long long)a * p.width + pg];
       } else {
         id = p.free_ids[free_count - 1 - (off0 + pg - have)];
+        if ((unsigned)id >= (unsigned)p.blocks) id = -1;
         if (in == 0) p.tables[(long long)a * p.width + pg] = id;    // the first token of a block: the block is new
       }
-      if (id >= 0) slot = (id << p.block_log) + in;
+      if ((unsigned)id < (unsigned)p.blocks) slot = (id << p.block_log) + in;
+      else report(p.status, NB_ST_BOUNDS, 4, a);
     }
     p.slots[t0] = slot;
     p.positions[t0] = slot >= 0 ? pos : 0;   // a place that the row does not have is none to look up: it may lie anywhere
@@ -420,16 +422,17 @@ __global__ void __launch_bounds__(128) kv_reorder_kernel(const KvReorder p) {
 extern "C" {
 
 // Block tables and slot maps.  rows <= 8192; `tables` int32 [rows, width] is completed in place; a row holds at most `limit` tokens,
-// width * block at most; `free_count_out` may be `free_count`; `own`: one word of work space.
+// width * block at most; ids of `blocks` (blocks * block <= 2^31) and more get no slot and are reported; `free_count_out` may be
+// `free_count`; `own`: one word of work space.
 int nb_kv_plan(const int* lengths, const int* new_lens, int* tables, const int* free_ids, const int* free_count, int* free_count_out,
                int* starts, int* ends, int* row_of, int* positions, int* slots, int* own, int rows, int width, int block, int free_size,
-               int tokens, int limit, unsigned int* status, void* stream) {
+               int tokens, int blocks, int limit, unsigned int* status, void* stream) {
   if (rows <= 0 || rows > 8192 || width <= 0 || block <= 0 || tokens < 0 || free_size < 0) return NB_ERR_BAD_ARG;
-  if ((block & (block - 1)) || (long long)width * block > 0x7fffff00LL || tokens > 0x7fffff00 || limit < 0 || limit > (long long)width * block) return NB_ERR_BAD_ARG;
+  if ((block & (block - 1)) || (long long)width * block > 0x7fffff00LL || tokens > 0x7fffff00 || limit < 0 || limit > (long long)width * block || blocks <= 0 || (long long)blocks * block > 1LL << 31) return NB_ERR_BAD_ARG;
   const int grid = max(1, min(148 * 4, ceil_div(tokens, 256)));
   // every block reads the count when it begins, so only a single block may write it back in place
   const bool later = grid > 1 && free_count == free_count_out;
-  KvPlan p{lengths, new_lens, tables, free_ids, free_count, later ? own : free_count_out, starts, ends, row_of, positions, slots, rows, width, 0, free_size, tokens, limit, status};
+  KvPlan p{lengths, new_lens, tables, free_ids, free_count, later ? own : free_count_out, starts, ends, row_of, positions, slots, rows, width, 0, free_size, tokens, blocks, limit, status};
   while ((1 << p.block_log) < block) ++p.block_log;
   static bool configured[64] = {};
   int dev = 0;

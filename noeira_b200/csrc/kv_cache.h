@@ -13,6 +13,7 @@ struct KvPlan {
   const int *free_ids, *free_count;
   int *free_count_out, *starts, *ends, *row_of, *positions, *slots;
   int rows, width, block_log, free_size, tokens;
+  int blocks;                                   // of the cache: an id from here on is none
   int limit;                                    // tokens that a row may hold: no more than its line of the table has room for
   unsigned int* status;
 };

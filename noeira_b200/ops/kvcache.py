@@ -57,7 +57,7 @@ def _ints(name, t, device, numel=None):
 
 
 # ------------------------------------------------------------------------------------------------ plan
-def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out=None, max_len=None) -> TokenPlan:
+def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out=None, max_len=None, blocks=None) -> TokenPlan:
     """Gives every row the blocks for ``new_lens[i]`` more tokens and every token its slot.
 
     ``tables`` int32 ``[rows, width]`` is completed in place; ``lengths`` / ``new_lens`` int32 ``[rows]``; ``free`` int32 is a
@@ -65,7 +65,9 @@ def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free
     dimension.  Blocks come off the top of the stack in row order.  A row is refused (slots -1, length unchanged, status word)
     when the stack has too few blocks left for it, when it outgrows its table, ``max_len`` tokens (default: what its table has
     room for) or the token dimension, or when a length is negative; behind a row that the stack could not serve, only rows that
-    need no new block are served.  ``free_count`` is updated in place unless ``free_count_out`` is given.
+    need no new block are served.  A token whose block's id, in the table or on the stack, is none of the cache's ``blocks``
+    (default: as many as have slots) gets slot -1 (status word).  ``free_count`` is updated in place unless ``free_count_out`` is
+    given.
     """
     dev = tables.get_device()
     shape = tables.shape
@@ -84,12 +86,16 @@ def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free
     limit = width * block if max_len is None else min(int(max_len), width * block)
     if limit < 0:
         raise ValueError(f"max_len: not negative, got {max_len}")
+    if blocks is None:
+        blocks = (1 << 31) // block
+    elif not 0 < blocks <= (1 << 31) // block:
+        raise ValueError(f"blocks: 1 to 2^31 / {block}, got {blocks}")
     if dev < 0:
-        return _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out, limit)
+        return _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out, limit, blocks)
     guard = _on(tables)
     if guard is not None:
         with guard:
-            return plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out, max_len)
+            return plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out, max_len, blocks)
     if free_count_out is None:
         free_count_out = free_count
     # one allocation; its last word is the kernel's own
@@ -99,16 +105,16 @@ def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free
     to = at + 12 * tokens
     check(cuda_lib().nb_kv_plan(
         lengths.data_ptr(), new_lens.data_ptr(), tables.data_ptr(), free.data_ptr(), free_count.data_ptr(), free_count_out.data_ptr(), to, to + 4 * rows + 4,
-        at + 8 * tokens, at + 4 * tokens, at, to + 8 * rows + 4, rows, width, block, free.numel(), tokens, limit, status_ptr(dev), raw_stream()), "kv_plan")
+        at + 8 * tokens, at + 4 * tokens, at, to + 8 * rows + 4, rows, width, block, free.numel(), tokens, blocks, limit, status_ptr(dev), raw_stream()), "kv_plan")
     return TokenPlan(starts, ends, row_of, positions, slots, free_count_out)
 
 
-def _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out, limit):
+def _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out, limit, blocks):
     rows = tables.shape[0]
     count = max(0, min(int(free_count), free.numel()))
     starts, ends = torch.zeros(rows + 1, dtype=torch.int32), lengths.clone()
     row_of, positions, slots = (torch.full((tokens,), v, dtype=torch.int32) for v in (-1, 0, -1))
-    at, off, taken, refused = 0, 0, 0, []
+    at, off, taken, refused, bad = 0, 0, 0, [], []
     for i in range(rows):
         held, new = int(lengths[i]), int(new_lens[i])
         first, at = at, at + max(new, 0)
@@ -119,7 +125,8 @@ def _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_c
         if ok:
             have = -(-held // block)
             for k in range(need):
-                tables[i, have + k] = free[count - 1 - off - k]
+                new_id = int(free[count - 1 - off - k])
+                tables[i, have + k] = new_id if 0 <= new_id < blocks else -1
             taken = max(taken, off + need) if need else taken
             ends[i] = held + new
         else:
@@ -128,10 +135,16 @@ def _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_c
         for t in range(first, min(at, tokens)):
             p = held + t - first
             row_of[t] = i
-            if ok and int(tables[i, p // block]) >= 0:
-                slots[t], positions[t] = int(tables[i, p // block]) * block + p % block, p
+            if not ok:
+                continue
+            b = int(tables[i, p // block])
+            if 0 <= b < blocks:
+                slots[t], positions[t] = b * block + p % block, p
+            else:
+                bad.append(i)
     if refused:
         raise RuntimeError(f"key / value cache: rows {refused} found no room")
+    _need(not bad, f"tables, free: rows {sorted(set(bad))} were given blocks outside the cache")
     out = free_count if free_count_out is None else free_count_out
     out.fill_(count - taken)
     return TokenPlan(starts, ends, row_of, positions, slots, out)
@@ -359,7 +372,7 @@ class PagedKVCache:
 
     def plan(self, new_lens, tokens) -> TokenPlan:
         """Room for ``new_lens[i]`` more tokens in row ``i``; the rows' lengths count them from here on."""
-        plan = plan_tokens(self.tables, self.lengths, new_lens, self.free, self.free_count, self.block, tokens, max_len=self.max_len)
+        plan = plan_tokens(self.tables, self.lengths, new_lens, self.free, self.free_count, self.block, tokens, max_len=self.max_len, blocks=self.blocks)
         self.lengths.copy_(plan.ends)
         return plan
 

@@ -35,6 +35,22 @@ def test_plan_tokens_takes_a_limit():
         kvcache.plan_tokens(**ok, max_len=-1)
 
 
+@pytest.mark.parametrize("bad", [8, 1 << 27, 1 << 28, -1])
+@pytest.mark.parametrize("place", ["table", "stack"])
+def test_plan_names_blocks_that_are_none(bad, place):
+    c = kvcache.PagedKVCache(1, 1, 64, 8, 2, 64, 16, device="cpu")
+    c.plan(ints([5, 5]), 10)
+    if place == "table":
+        c.tables[0, 0] = bad
+    else:
+        c.free[int(c.free_count) - 1] = bad
+    with pytest.raises(ValueError, match=r"rows \[0\]"):
+        c.plan(ints([13, 3]), 16)
+    for blocks in (0, (1 << 27) + 1):
+        with pytest.raises(ValueError, match="blocks"):
+            kvcache.plan_tokens(c.tables, c.lengths, ints([1, 1]), c.free, c.free_count, 16, 2, blocks=blocks)
+
+
 # ------------------------------------------------------------------------------------------------ GPT
 def small(**kw):
     return GPT(**{**dict(vocab=32, seq=20, dim=64, layers=1, heads=1, seed=3), **kw}).eval()

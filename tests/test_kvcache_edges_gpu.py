@@ -66,3 +66,30 @@ def test_rows_hold_max_len_tokens_and_no_more(block):
     p = c.plan(ints([0, 10]), 10)
     reported("no room")
     assert p.positions.tolist() == [0] * 10 and p.slots.tolist() == [-1] * 10 and c.lengths.tolist() == [18, 18]
+
+
+@pytest.mark.parametrize("bad", [8, 1 << 27, 1 << 28, 0x7fffffff, -1, -(1 << 31)])
+@pytest.mark.parametrize("place", ["table", "stack"])
+def test_plan_reports_blocks_that_are_none(bad, place):
+    """An id shifted past 32 bits would be the slot of another block."""
+    from noeira_b200.ops import kvcache
+    c = kvcache.PagedKVCache(1, 1, 64, 8, 2, 64, 16)
+    c.plan(ints([5, 5]), 10)                                # blocks 0 and 1
+    clean()
+    if place == "table":
+        c.tables[0, 0] = bad
+        want = [-1] * 11 + [32, 33] + [21, 22, 23]          # row 0's tokens 5 to 15 lie in its first block, then block 2
+    else:
+        c.free[int(c.free_count) - 1] = bad
+        want = list(range(5, 16)) + [-1, -1] + [21, 22, 23]
+    p = c.plan(ints([13, 3]), 16)
+    reported("bounds")
+    assert p.slots.tolist() == want
+    assert p.positions.tolist() == [q if s >= 0 else 0 for q, s in zip([*range(5, 18), *range(5, 8)], want)]
+    assert c.tables[0, 1].item() == (2 if place == "table" else -1)
+    k = torch.ones(16, 1, 64, dtype=torch.bfloat16, device="cuda")
+    before = c.kv.clone()
+    c.append(0, k, k, p)
+    clean()
+    changed = (c.kv.view(torch.uint8) != before.view(torch.uint8)).any(-1)[0].any(0)[:, 0].reshape(-1).nonzero().reshape(-1).tolist()
+    assert changed == sorted(s for s in want if s >= 0)
