@@ -1,8 +1,10 @@
 // Beam search: the best continuations over beams and vocabulary.
 //
-// value(b, v) = score_b + x_bv - log sum_u exp x_bu.  Within a beam the order of the values is the order of the logits, so
-// the candidates of a beam are found by its logits alone, exactly; only the winners of the beams are compared by value, in
-// 64 bits.  Ties go to the lowest b * vocab + v.  NaN counts as -inf, +inf as the largest finite number.
+// value(b, v) = score_b + x_bv - log sum_u exp x_bu, in 64 bits.  It never falls while x rises, so the candidates of a beam are
+// found by its logits alone; only the winners of the beams are compared by value.  Ties go to the lowest b * vocab + v.  Where
+// different logits round to one value (beside an infinite one, next to zero, at a score of 1e20) the last candidate's value is
+// looked for from the row's begin; a beam that does not exist (-inf) offers its first tokens.  NaN counts as -inf, +inf as the
+// largest finite number.
 //
 // One pass over the logits, which is all that there is to read (R * beams * vocab elements at the copy rate), split over blocks of
 // one part of one beam's row each, the elements in registers.  The maximum and sum of each warp come first; then the K = beams best
@@ -27,7 +29,7 @@ struct BeamSel {
   float* scores_out;
   int *parents, *tokens;
   unsigned char* done;
-  int requests, beams, vocab, eos, parts;
+  int requests, beams, vocab, eos, parts, fp32;
   long long pitch;                 // elements between beams' rows
   float2* part_ms;                 // [R * beams, parts] maximum, sum of exponentials
   Key* part_key;                   // [R * beams, parts, beams] best first
@@ -181,7 +183,9 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const BeamSel p) {
     const double score = s0 != s0 ? -INFINITY : (double)s0;
     long long at = 0x7fffffffffffffffLL;
     double v = -INFINITY;
-    if (p.finished && p.finished[row]) {
+    if (score == -INFINITY) {
+      if (lane < p.vocab) at = (long long)b * p.vocab + lane;      // all alike: the first ones
+    } else if (p.finished && p.finished[row]) {
       // eos at the beam's score; behind it, in order, what it does not continue with
       const int t = lane == 0 ? p.eos : lane - 1 + (lane - 1 >= p.eos);
       if (t < p.vocab) at = (long long)b * p.vocab + t;
@@ -243,10 +247,31 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const BeamSel p) {
           if (lane == k) mine = last;
         }
       }
+      auto value = [&](float x) { return x > -INFINITY ? score + ((double)x - (double)from - lsum) : (double)-INFINITY; };
       if (mine && lane < K) {
-        const float x = value_of(mine);
         at = (long long)b * p.vocab + (int)~(uint32_t)mine;
-        if (x > -INFINITY && score > -INFINITY) v = score + ((double)x - (double)from - lsum);
+        v = value(value_of(mine));
+      }
+      // Does the next smaller logit have the last candidate's value too?  Then the row may hold more of that value, ahead of those
+      // found.
+      const Key least = __shfl_sync(0xffffffffu, mine, K - 1);
+      const double floor_v = __shfl_sync(0xffffffffu, v, K - 1);
+      if (K < p.vocab && value_of(least) > -INFINITY && value(value_of(least - (1ULL << 32))) == floor_v) {
+        const int above = __popc(__ballot_sync(0xffffffffu, lane < K && v > floor_v));
+        const char* logits = (const char*)p.logits + row * p.pitch * (p.fp32 ? 4 : 2);
+        int found = above;
+        for (int i0 = 0; found < K && i0 < p.vocab; i0 += 32) {
+          const int i = min(i0 + lane, p.vocab - 1);
+          float x = p.fp32 ? ((const float*)logits)[i] : __bfloat162float(((const __nv_bfloat16*)logits)[i]);
+          x = fminf(fmaxf(x, -INFINITY), TOP);
+          const unsigned hit = __ballot_sync(0xffffffffu, i0 + lane < p.vocab && value(x) == floor_v);
+          const int nth = lane - found;                // the hit of this lane, which holds the lane-th candidate
+          if (nth >= 0 && nth < __popc(hit)) {
+            at = (long long)b * p.vocab + i0 + (int)__fns(hit, 0, nth + 1);
+            v = floor_v;
+          }
+          found += __popc(hit);
+        }
       }
     }
     if (lane < K) {
@@ -317,7 +342,7 @@ int nb_beam_select(const void* logits, const float* scores, const unsigned char*
   if (!work || work_bytes < nb_beam_select_work(requests, beams, vocab) || (reinterpret_cast<uintptr_t>(work) & 15)) return NB_ERR_BAD_ARG;
   const int each = elements_each(rows, vocab), parts = ceil_div(vocab, THREADS * each);
   if (rows * parts > 0x7fffffffLL) return NB_ERR_TOO_LARGE;
-  BeamSel p{logits, scores, finished, scores_out, parents, tokens, done, requests, beams, vocab, eos, parts, pitch, nullptr, nullptr};
+  BeamSel p{logits, scores, finished, scores_out, parents, tokens, done, requests, beams, vocab, eos, parts, fp32, pitch, nullptr, nullptr};
   p.part_key = (Key*)work;
   p.part_ms = (float2*)(p.part_key + rows * parts * beams);
   const cudaStream_t s = (cudaStream_t)stream;

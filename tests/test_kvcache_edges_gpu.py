@@ -93,3 +93,45 @@ def test_plan_reports_blocks_that_are_none(bad, place):
     clean()
     changed = (c.kv.view(torch.uint8) != before.view(torch.uint8)).any(-1)[0].any(0)[:, 0].reshape(-1).nonzero().reshape(-1).tolist()
     assert changed == sorted(s for s in want if s >= 0)
+
+
+# ------------------------------------------------------------------------------------------------ beams
+def logits_of(kind, beams, vocab):
+    """Different logits of one value in 64 bits; beam 0 is the one that counts."""
+    v = torch.arange(vocab).float()
+    x = torch.stack([torch.sin(v * (b + 1)) for b in range(beams)])
+    if kind == "infinite":
+        x[0, vocab // 2] = float("inf")
+    if kind == "infinite twice":
+        x[0, vocab - 1] = x[0, vocab // 3] = float("inf")
+    if kind == "near zero":                                   # rising, far below what a value of size log(vocab) can tell
+        x = (v * 2.0 ** -90).expand(beams, vocab).clone()
+        x[:, vocab - 1] = 1.0
+    if kind == "few":                                         # fewer finite logits than beams, and two of them equal
+        x[0] = float("-inf")
+        x[0, vocab - 1], x[0, vocab // 2], x[0, vocab // 3] = 2.0, 2.0, float("nan")
+    return x
+
+
+@pytest.mark.parametrize("kind", ["infinite", "infinite twice", "near zero", "few", "plain"])
+@pytest.mark.parametrize("beams,vocab", [(2, 4), (4, 4), (4, 5), (8, 20011), (32, 300), (5, 49152)])
+@pytest.mark.parametrize("fp32", [False, True])
+def test_select_equal_values_of_different_logits(kind, beams, vocab, fp32):
+    from noeira_b200.ops import beam
+    inf = float("inf")
+    x = logits_of(kind, beams, vocab)
+    x = x if fp32 else x.bfloat16()
+    # one beam alone; a far score, at which all its logits are one; none; a beam that is finished at -inf, one that is at 0
+    scores = torch.full((6, beams), -inf)
+    scores[0, 0], scores[1, 0], scores[2, 0], scores[4, beams - 1] = 0.0, -1e25, float("nan"), 0.0
+    scores[5] = 0.0
+    x = x.expand(6, beams, vocab).contiguous()
+    fin = torch.zeros(6, beams, dtype=torch.bool)
+    fin[3, 0] = fin[4, beams - 1] = True
+    for finished, eos in ((None, None), (fin, vocab - 1), (fin, vocab // 2)):
+        s, p, t, _ = beam.beam_select(x.cuda(), scores.cuda(), None if finished is None else finished.cuda(), eos)
+        clean()
+        for r, row in enumerate(O.select(x, scores, finished, eos)):
+            assert [(int(a), int(b)) for a, b in zip(p[r], t[r])] == [(b, v) for _, b, v in row], r
+        c = beam.beam_select(x, scores, finished, eos)
+        assert torch.equal(p.cpu(), c[1]) and torch.equal(t.cpu(), c[2])
