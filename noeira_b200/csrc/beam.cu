@@ -20,6 +20,7 @@ using namespace nb;
 
 constexpr int THREADS = 256;
 constexpr float TOP = 3.4028235e38f;
+constexpr int MOST_TOKENS = 0x7fff0000;    // a part's last index, up to 8191 behind the last token, is still one of 32 bits
 typedef unsigned long long Key;              // order of the value above, inverse index below: larger is better, all distinct
 
 struct BeamSel {
@@ -336,7 +337,7 @@ long long nb_beam_select_work(int requests, int beams, int vocab) {
 
 int nb_beam_select(const void* logits, const float* scores, const unsigned char* finished, float* scores_out, int* parents, int* tokens,
                    unsigned char* done, int requests, int beams, int vocab, int eos, int fp32, long long pitch, void* work, long long work_bytes, void* stream) {
-  if (requests <= 0 || beams <= 0 || beams > 32 || vocab <= 0 || vocab > 0x7fffff00 || eos >= vocab || pitch < vocab || (finished && eos < 0)) return NB_ERR_BAD_ARG;
+  if (requests <= 0 || beams <= 0 || beams > 32 || vocab <= 0 || vocab > MOST_TOKENS || eos >= vocab || pitch < vocab || (finished && eos < 0)) return NB_ERR_BAD_ARG;
   if (reinterpret_cast<uintptr_t>(logits) & (fp32 ? 3 : 1)) return NB_ERR_UNALIGNED;
   const long long rows = (long long)requests * beams;
   if (!work || work_bytes < nb_beam_select_work(requests, beams, vocab) || (reinterpret_cast<uintptr_t>(work) & 15)) return NB_ERR_BAD_ARG;

@@ -13,6 +13,7 @@ from .kvcache import F8, _ints, _need, _on
 from .status import status_ptr
 
 MAX_BEAMS = 32
+MAX_VOCAB = 0x7fff0000
 _TOP = 3.4028234663852886e38
 
 
@@ -32,8 +33,8 @@ def beam_select(logits, scores, finished=None, eos=None):
         raise ValueError(f"logits: [requests, beams, vocab], got {tuple(shape)}")
     requests, beams, vocab = shape
     dev = logits.get_device()
-    if beams > MAX_BEAMS or requests * beams >= 1 << 31 or vocab >= 0x7fffff00:
-        raise ValueError(f"beam_select: at most {MAX_BEAMS} beams, got {tuple(shape)}")
+    if beams > MAX_BEAMS or requests * beams >= 1 << 31 or vocab > MAX_VOCAB:
+        raise ValueError(f"beam_select: at most {MAX_BEAMS} beams and {MAX_VOCAB} tokens, got {tuple(shape)}")
     if scores.dtype is not torch.float32 or scores.shape != shape[:2] or not scores.is_contiguous() or scores.get_device() != dev:
         raise ValueError(f"scores: contiguous float32 {(requests, beams)}, got {scores.dtype} {tuple(scores.shape)}")
     if eos is not None and not 0 <= eos < vocab:

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from noeira_b200.models.gpt import GPT
-from noeira_b200.ops import kvcache
+from noeira_b200.ops import beam, kvcache
 
 I32 = torch.int32
 
@@ -49,6 +49,13 @@ def test_plan_names_blocks_that_are_none(bad, place):
     for blocks in (0, (1 << 27) + 1):
         with pytest.raises(ValueError, match="blocks"):
             kvcache.plan_tokens(c.tables, c.lengths, ints([1, 1]), c.free, c.free_count, 16, 2, blocks=blocks)
+
+
+# ------------------------------------------------------------------------------------------------ beams
+def test_select_refuses_vocabularies_whose_last_part_passes_32_bits():
+    for vocab in (0x7fff0001, 0x7ffffeff):                    # no memory behind it: the sizes alone decide
+        with pytest.raises(ValueError, match="tokens"):
+            beam.beam_select(torch.empty(1, 1, vocab, dtype=torch.bfloat16, device="meta"), torch.empty(1, 1, device="meta"))
 
 
 # ------------------------------------------------------------------------------------------------ GPT
