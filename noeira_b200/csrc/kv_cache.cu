@@ -187,13 +187,19 @@ __device__ __forceinline__ uint32_t codes4(uint32_t a, uint32_t b, float inv) {
 }
 constexpr uint32_t BF16_INF = 0x7f80;
 
+// Does slot `b` continue the block of slot `a`, which is one of the cache or none?
+__device__ __forceinline__ bool follows(const KvAppend& p, int a, int b) {
+  return (unsigned)a < (unsigned)p.limit && a >> p.block_log == b >> p.block_log && a < b;
+}
+
 // A run is a stretch of neighbouring tokens and slots inside one block.  A warp takes the runs that begin in a window of `window`
 // tokens, for one head of K or V: D / 8 lanes a token, 16 bytes each, so that a run of up to 32 tokens is read once and stays in
 // registers between the maximum and the codes (longer ones are read again, from the caches).  What continues a run in the same
-// block behind skipped tokens is done by the same warp.  One pass over the input at the copy rate is the bound; windows of eight
-// tokens spread a decode step over the GPU, windows of 32 keep warps with nothing to do few.  26k tokens of 24 prompts, 8 heads of
-// 128 (166 MB): 39 us, 4.3 TB/s; a warp has one run, whose loads, maximum and stores follow one another, and 16 warps fit an SM
-// beside the 64 registers that hold a run.  64 single tokens, 5 heads of 64: 2.6 us.
+// block, behind skipped tokens or skipped slots, is done by the same warp: the scale belongs to all of them.  One pass over the
+// input at the copy rate is the bound; windows of eight tokens spread a decode step over the GPU, windows of 32 keep warps with
+// nothing to do few.  26k tokens of 24 prompts, 8 heads of 128 (166 MB): 39 us, 4.3 TB/s; a warp has one run, whose loads, maximum
+// and stores follow one another, and 16 warps fit an SM beside the 64 registers that hold a run.  64 single tokens, 5 heads of 64:
+// 2.6 us.
 template <int D>
 __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p) {
   constexpr int LANES = D / 8, TOKENS = 32 / LANES, HELD = 32 / TOKENS;
@@ -210,14 +216,14 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p) {
   int prev = __shfl_up_sync(0xffffffffu, my_slot, 1);
   if (lane == 0) prev = w0 > 0 ? p.slots[w0 - 1] : -1;
   const bool inside = valid && (my_slot & ((1 << p.block_log) - 1)) != 0;
-  bool start = valid && !(inside && prev == my_slot - 1);
+  bool start = valid && !(inside && follows(p, prev, my_slot));
   unsigned ask = __ballot_sync(0xffffffffu, start && inside && (unsigned)prev >= (unsigned)p.limit);
   while (ask) {                        // behind skipped tokens: does the last one that counts precede this one?
     const int j = __ffs(ask) - 1;
     ask &= ask - 1;
     const long long before = valid_before(p, w0 + j);
     const int last = before >= 0 ? p.slots[before] : -1;
-    if (lane == j && last == my_slot - 1) start = false;
+    if (lane == j && follows(p, last, my_slot)) start = false;
   }
   unsigned runs = __ballot_sync(0xffffffffu, start);
   // Runs of one token, as in a decode step: several at a time, so that their loads go out together.  One that has to move earlier
@@ -227,7 +233,7 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p) {
   const bool more = behind < p.tokens;
   if (lane == 31 || lane + 1 >= p.window) next = more ? p.slots[behind] : -1;
   const bool room = ((my_slot + 1) & ((1 << p.block_log) - 1)) != 0;
-  const unsigned single = __ballot_sync(0xffffffffu, start && !(room && more && (next == my_slot + 1 || (unsigned)next >= (unsigned)p.limit)));
+  const unsigned single = __ballot_sync(0xffffffffu, start && !(room && more && (follows(p, my_slot, next) || (unsigned)next >= (unsigned)p.limit)));
   if (__popc(single) > 1) {
     constexpr int TURNS = 8 / TOKENS;
     for (int i0 = 0; i0 < p.window; i0 += 8) {
@@ -342,11 +348,12 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p) {
       }
       __syncwarp();
       old = now;
-      off += n;
-      slot += n;
-      if (off == 1 << p.block_log) break;
+      slot += n - 1;                   // the run's last
+      if (off + n == 1 << p.block_log) break;
       t0 = valid_from(p, t0 + n);
-      if (t0 >= p.tokens || p.slots[t0] != slot) break;
+      if (t0 >= p.tokens || !follows(p, slot, p.slots[t0])) break;
+      slot = p.slots[t0];
+      off = slot - (id << p.block_log);
     }
     if (lane == 0) p.scale[bh] = old;
   }

@@ -178,10 +178,11 @@ def append(kv, scale, k, v, slots) -> None:
     """Writes the keys and values of new tokens into a cache layer.
 
     ``k`` / ``v`` bf16 ``[tokens, heads, head_dim]`` (any token and head strides, e.g. views of a packed projection), ``slots``
-    int32 ``[tokens]``; tokens with a slot outside the cache (-1) are skipped.  The tokens of one block have to be
-    in ascending order with none but skipped tokens between them, and no slot may appear twice.  A block's scale is that of its largest finite magnitude; a
-    call that writes a block's first token starts the block afresh, one that continues it may raise the scale and then moves
-    the codes of the earlier tokens.  Non-finite inputs become NaN and do not count for the scale.
+    int32 ``[tokens]``; tokens with a slot outside the cache (-1) are skipped.  The tokens of one block have to be neighbours,
+    but for skipped ones, with ascending slots, which may leave places out; no slot may appear twice.  A block's scale is that
+    of its largest finite magnitude; a call that writes a block's first token starts the block afresh, one that continues it may
+    raise the scale and then moves the codes of the earlier tokens.  Non-finite inputs become NaN and do not count for the
+    scale.
     """
     dev, blocks, heads, block, dim = _check_layer(kv, scale)
     shape = k.shape

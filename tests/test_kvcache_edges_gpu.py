@@ -95,6 +95,44 @@ def test_plan_reports_blocks_that_are_none(bad, place):
     assert changed == sorted(s for s in want if s >= 0)
 
 
+# ------------------------------------------------------------------------------------------------ append
+def gaps(kind, block):
+    """Slots of a call that leaves places of a block out."""
+    b = [7 * block, 2 * block, 11 * block, 4 * block, 9 * block]
+    if kind == "every second":
+        return [s + i for s in b for i in range(0, block, 2)]
+    if kind == "from the middle":
+        return [b[0] + 3, b[0] + 5, b[1] + 1, b[2] + 2, b[2] + 3, b[2] + block - 1, b[3] + block - 1, b[4], b[4] + block - 1]
+    if kind == "behind skipped tokens":
+        return [b[0], -1, b[0] + 2, -1, 1 << 30, b[0] + 3, -1, b[0] + 9, b[1] + 4, -1, b[1] + 6] + [-1] * 40 + [b[1] + 8, b[2] + 1, b[3] + 1]
+    return [s + i for s in b for i in range(block) if i % 5] + list(range(20 * block, 20 * block + 1100))     # more than a short call's
+
+
+@pytest.mark.parametrize("kind", ["every second", "from the middle", "behind skipped tokens", "many"])
+@pytest.mark.parametrize("block", [16, 128])
+@pytest.mark.parametrize("dim,heads", [(64, 3), (128, 1)])
+@pytest.mark.parametrize("growing", [False, True])
+def test_append_leaves_places_out(kind, block, dim, heads, growing):
+    """The scale of a block is one for all tokens of the call, wherever the places between them are."""
+    import kv_cases as C
+    from noeira_b200.ops import kvcache
+    slots = gaps(kind, block)
+    n, blocks = len(slots), 20 + -(-1100 // block)
+    g = torch.Generator().manual_seed(block + dim)
+    codes, scale = C.random_codes((2, blocks, heads, block, dim), 5), torch.exp2(torch.randint(-12, -5, (2, blocks, heads), generator=g).float())
+    x = torch.randn(2, n, heads, dim, generator=g)
+    if growing:
+        x *= 1.5 ** (torch.arange(n) % 24)[None, :, None, None]
+    x = x.bfloat16()
+    want, wscale = O.append(C.values(codes), scale.numpy(), x[0].float().numpy(), x[1].float().numpy(), slots)
+    c, sc = codes.cuda(), scale.cuda()
+    kvcache.append(c, sc, x[0].cuda(), x[1].cuda(), ints(slots))
+    clean()
+    assert np.array_equal(sc.cpu().double().numpy(), wscale) and np.array_equal(C.values(c), want, equal_nan=True)
+    kvcache.append(codes, scale, x[0], x[1], torch.tensor(slots, dtype=I32))
+    assert torch.equal(codes.view(torch.uint8), c.cpu().view(torch.uint8))
+
+
 # ------------------------------------------------------------------------------------------------ beams
 def logits_of(kind, beams, vocab):
     """Different logits of one value in 64 bits; beam 0 is the one that counts."""
