@@ -326,7 +326,8 @@ class PagedKVCache:
 
     ``rows`` sequences of up to ``max_len`` tokens share ``blocks`` blocks.  ``plan`` makes room for new tokens, ``append`` and
     ``attend`` are the calls of one layer, ``reorder`` lets rows follow the beams of a search, ``reset`` empties rows.  For
-    ``reorder`` every row owns a spare block (``spares=True``).
+    ``reorder`` every row owns a spare block (``spares=True``).  The tensors stay the same all along: captured steps may be replayed
+    between other calls.
     """
 
     def __init__(self, layers, kv_heads, head_dim, blocks, rows, max_len, block=16, device="cuda", spares=False):
@@ -339,11 +340,16 @@ class PagedKVCache:
         self.scale = torch.zeros(layers, 2, blocks, kv_heads, device=self.device)
         ints = dict(dtype=torch.int32, device=self.device)
         self.width = -(-max_len // block)
-        self.tables, self._tables = (torch.full((rows, self.width), -1, **ints) for _ in range(2))
-        self.lengths, self._lengths = (torch.zeros(rows, **ints) for _ in range(2))
-        self.spare, self._spare = (torch.full((rows,), -1, **ints) for _ in range(2))
+        # tables, lengths and spare blocks lie together, so that a reorder's are put in their place by one copy: a captured step
+        # reads the same tensors before and after it
+        self._state, self._next = (torch.full((rows * (self.width + 2),), -1, **ints) for _ in range(2))
+        self.tables, self.lengths, self.spare = self._views(self._state)
         self.free, self.free_count = torch.empty(blocks, **ints), torch.empty(1, **ints)
         self.reset()
+
+    def _views(self, state):
+        tables, lengths, spare = state.split((self.rows * self.width, self.rows, self.rows))
+        return tables.view(self.rows, self.width), lengths, spare
 
     def reset(self, rows=None) -> None:
         """Empties the given rows (default: all) and collects the free blocks: every block that no row and no spare names.
@@ -387,7 +393,5 @@ class PagedKVCache:
         """Row ``r * beams + j`` continues from row ``r * beams + parents[r, j]`` (``ops.beam.beam_reorder``)."""
         from .beam import beam_reorder
         _need(self.spares, "PagedKVCache.reorder: the cache was made without spare blocks (spares=True)")
-        beam_reorder(self.kv, self.scale, self.tables, self.lengths, parents, self.spare, self._tables, self._lengths, self._spare)
-        self.tables, self._tables = self._tables, self.tables
-        self.lengths, self._lengths = self._lengths, self.lengths
-        self.spare, self._spare = self._spare, self.spare
+        beam_reorder(self.kv, self.scale, self.tables, self.lengths, parents, self.spare, *self._views(self._next))
+        self._state.copy_(self._next)

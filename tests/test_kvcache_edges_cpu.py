@@ -51,6 +51,20 @@ def test_plan_names_blocks_that_are_none(bad, place):
             kvcache.plan_tokens(c.tables, c.lengths, ints([1, 1]), c.free, c.free_count, 16, 2, blocks=blocks)
 
 
+def test_reorder_leaves_the_caches_tensors_in_their_place():
+    """A captured step holds the addresses of tables, lengths and spare blocks."""
+    c = kvcache.PagedKVCache(1, 1, 64, 12, 3, 40, 16, device="cpu", spares=True)
+    c.plan(ints([20, 0, 0]), 20)
+    held = c.tables, c.lengths, c.spare
+    at = [t.data_ptr() for t in held]
+    c.reorder(ints([[0, 0, 0]]))
+    assert [t.data_ptr() for t in (c.tables, c.lengths, c.spare)] == at
+    assert held[1].tolist() == [20] * 3 and held[0][:, 0].unique().numel() == 1 and held[0][:, 1].unique().numel() == 3
+    assert held[2][1:].tolist() == [-1, -1]
+    c.refill_spares()
+    assert int(held[2].min()) >= 0 and held[2].unique().numel() == 3
+
+
 # ------------------------------------------------------------------------------------------------ beams
 def test_select_refuses_vocabularies_whose_last_part_passes_32_bits():
     for vocab in (0x7fff0001, 0x7ffffeff):                    # no memory behind it: the sizes alone decide

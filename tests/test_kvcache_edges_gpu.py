@@ -133,6 +133,50 @@ def test_append_leaves_places_out(kind, block, dim, heads, growing):
     assert torch.equal(codes.view(torch.uint8), c.cpu().view(torch.uint8))
 
 
+@pytest.mark.parametrize("whole", [True, False])
+def test_captured_steps_with_reorders(whole):
+    """A step captured with its reorder, and one captured without it and replayed between eager reorders, leave the cache as eager
+    steps do."""
+    from noeira_b200.ops import kvcache
+    g = torch.Generator().manual_seed(7)
+    beams, heads, rows = 3, 2, 6
+    caches = [kvcache.PagedKVCache(1, heads, 64, blocks=50, rows=rows, max_len=60, block=16, spares=True) for _ in range(2)]
+    first = ints([21, 0, 0, 16, 0, 0])
+    kv = torch.randn(37, 2 * heads, 64, generator=g).bfloat16().cuda()
+    for c in caches:
+        c.append(0, kv[:, :heads], kv[:, heads:], c.plan(first, 37))
+        c.reorder(torch.zeros(2, beams, dtype=I32, device="cuda"))
+        c.refill_spares()
+    x, parents, one = torch.zeros(rows, 2 * heads, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, beams, dtype=I32, device="cuda"), ints([1] * rows)
+    q = torch.randn(rows, heads, 64, generator=g).bfloat16().cuda()
+
+    def step(c, reorder=True):
+        p = c.plan(one, rows)
+        c.append(0, x[:, :heads], x[:, heads:], p)
+        o = c.attend(0, q, p, max_new=1)
+        if reorder:
+            c.reorder(parents)
+        return o
+
+    eager, captured = caches
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        out = step(captured, whole)
+    for _ in range(25):
+        x.copy_(torch.randn(rows, 2 * heads, 64, generator=g))
+        parents.copy_(torch.randint(0, beams, (2, beams), generator=g))
+        want = step(eager)
+        graph.replay()
+        if not whole:
+            captured.reorder(parents)
+        clean()
+        assert torch.equal(out, want)
+        for a, b in ((eager.tables, captured.tables), (eager.lengths, captured.lengths), (eager.spare, captured.spare), (eager.free_count, captured.free_count),
+                     (eager.scale, captured.scale), (eager.kv.view(torch.uint8), captured.kv.view(torch.uint8))):
+            assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------------------------------------------ beams
 def logits_of(kind, beams, vocab):
     """Different logits of one value in 64 bits; beam 0 is the one that counts."""
