@@ -217,3 +217,87 @@ def test_select_equal_values_of_different_logits(kind, beams, vocab, fp32):
             assert [(int(a), int(b)) for a, b in zip(p[r], t[r])] == [(b, v) for _, b, v in row], r
         c = beam.beam_select(x, scores, finished, eos)
         assert torch.equal(p.cpu(), c[1]) and torch.equal(t.cpu(), c[2])
+
+
+# ------------------------------------------------------------------------------------------------ attention
+@pytest.mark.parametrize("tokens", [200, 1])
+def test_attention_over_a_million_keys(tokens):
+    """One row's tiles walk more than 2^24 steps between them.  Its table names four blocks again and again, so the definition is a
+    sum over 512 keys, each as often as the token sees it."""
+    from noeira_b200.ops import kvcache
+    import kv_cases as C
+    hq, hk, dim, block, keys = 32, 8, 128, 128, 1 << 20
+    g = torch.Generator(device="cuda").manual_seed(3)
+    codes = C.random_codes((2, 4, hk, block, dim), 3).cuda()
+    scale = torch.exp2(torch.randint(-10, -6, (2, 4, hk), generator=torch.Generator().manual_seed(4)).float()).cuda()
+    table = (torch.arange(keys // block, device="cuda") % 4).to(I32)[None].contiguous()
+    q = torch.randn(tokens, hq, dim, device="cuda", generator=g).bfloat16()
+    out = kvcache.paged_attention(q, codes, scale, table, ints([0, tokens]), ints([keys]))
+    clean()
+    k, v = ((codes[w].double() * scale[w].double()[..., None, None]).transpose(0, 1).reshape(hk, -1, dim).repeat_interleave(hq // hk, 0) for w in (0, 1))
+    s = q.double().transpose(0, 1) @ k.transpose(1, 2) * dim ** -0.5
+    sees = keys - tokens + 1 + torch.arange(tokens, device="cuda")
+    times = (sees[:, None] - torch.arange(4 * block, device="cuda") + 4 * block - 1) // (4 * block)
+    p = torch.exp(s - s.amax(-1, keepdim=True)) * times
+    p = p / p.sum(-1, keepdim=True)
+    want, A = (p @ v).transpose(0, 1), (p @ v.abs()).transpose(0, 1)
+    # as for shorter rows; the sums of a warp's piece: two weights and a product of 16 keys per step, one after the other
+    piece = -(-((tokens * 4 + 15) // 16) * hk * (keys // 16 + 2) // (148 * 4 * 3))
+    S = dim ** -0.5 * float((q.double().abs().sum(-1)).max() * k.abs().max())
+    most = 2.0 ** -8 * want.abs() + A * (2.0 ** -8 + 2 * (2.0 ** -24 * dim * S + 2.0 ** -21) + 2.0 ** -24 * 3 * (piece + 1776))
+    err = (out.double() - want).abs()
+    assert bool((err <= most).all()), float((err / most).max())
+
+
+@pytest.mark.parametrize("tokens,dim", [(130, 128), (100, 128), (130, 64), (1, 128)])
+def test_attention_through_very_wide_tables(tokens, dim):
+    """Tables with room for so many keys that steps are counted in 64 bits: the bits are those of narrow tables."""
+    from noeira_b200.ops import kvcache
+    import kv_cases as C
+    hq, hk, block = 32, 8, 128
+    held, new = [3000, 900, 4000, 17], [tokens, 1, 1, 2]
+    d = C.attention_inputs((held, new, hq, hk, dim, block))
+    q = d["q"][: d["T"], 1: 1 + hq].contiguous().cuda()
+    width = (1 << 30) // block
+    wide = torch.full((4, width), -1, dtype=I32, device="cuda")
+    wide[:, : d["tables"].shape[1]] = d["tables"].cuda()
+    rest = (d["starts"].cuda(), d["ends"].cuda(), d["max_new"])
+    a = kvcache.paged_attention(q, d["codes"].cuda(), d["scale"].cuda(), d["tables"].cuda(), *rest)
+    b = kvcache.paged_attention(q, d["codes"].cuda(), d["scale"].cuda(), wide, *rest)
+    clean()
+    assert torch.equal(a, b)
+
+
+def test_attention_counts_more_than_32_bits_of_steps():
+    """4200 rows of one token over the same million keys: 2.2e9 steps.  Every token sees every key, so the definition is the
+    softmax over the 512 different ones."""
+    from noeira_b200.ops import kvcache
+    import kv_cases as C
+    rows, hq, hk, dim, block, keys = 4200, 32, 8, 128, 128, 1 << 20
+    codes = C.random_codes((2, 4, hk, block, dim), 3).cuda()
+    scale = torch.exp2(torch.randint(-10, -6, (2, 4, hk), generator=torch.Generator().manual_seed(4)).float()).cuda()
+    table = (torch.arange(keys // block, device="cuda") % 4).to(I32)[None].repeat(rows, 1)
+    q = torch.randn(rows, hq, dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).bfloat16()
+    out = kvcache.paged_attention(q, codes, scale, table, torch.arange(rows + 1, dtype=I32, device="cuda"), ints([keys] * rows), max_new=1)
+    clean()
+    k, v = ((codes[w].double() * scale[w].double()[..., None, None]).transpose(0, 1).reshape(hk, -1, dim).repeat_interleave(hq // hk, 0) for w in (0, 1))
+    p = torch.softmax(q.double().transpose(0, 1) @ k.transpose(1, 2) * dim ** -0.5, -1)
+    want, A = (p @ v).transpose(0, 1), (p @ v.abs()).transpose(0, 1)
+    # a warp's sums over one job, which is shorter than its piece
+    S = dim ** -0.5 * float((q.double().abs().sum(-1)).max() * k.abs().max())
+    most = 2.0 ** -8 * want.abs() + A * (2.0 ** -8 + 2 * (2.0 ** -24 * dim * S + 2.0 ** -21) + 2.0 ** -24 * 3 * (keys // 16))
+    err = (out.double() - want).abs()
+    assert bool((err <= most).all()), float((err / most).max())
+
+
+def test_attention_reports_starts_that_are_none():
+    """Rows that all claim all tokens have more steps than their sizes allow: refused as a whole."""
+    from noeira_b200.ops import kvcache
+    rows, tokens, block = 4096, 60, 128
+    kv, scale = torch.zeros(2, 1, 1, block, 128, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn), torch.ones(2, 1, 1, device="cuda")
+    q = torch.ones(tokens, 16, 128, dtype=torch.bfloat16, device="cuda")
+    starts = ints([0, tokens] * (rows // 2) + [0])
+    out = torch.full_like(q, 7)
+    kvcache.paged_attention(q, kv, scale, torch.zeros(rows, 8192, dtype=I32, device="cuda"), starts, ints([1 << 20] * rows), out=out)
+    reported("bounds")
+    assert bool((out == 7).all())
