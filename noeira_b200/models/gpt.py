@@ -103,7 +103,11 @@ class GPT(Module):
     def forward_cached(self, ids: torch.Tensor, cache, plan, max_new: int = None):
         """New tokens ``ids [tokens]`` of the cache's rows (``plan = cache.plan(new_lens, tokens)``) → logits ``[rows, vocab]`` of each
         row's last new token.  Rows without new tokens get those of a neighbour, which mean nothing.  The cache's ``max_len`` may
-        not pass ``seq``, behind which there are no positions."""
+        not pass ``seq``, behind which there are no positions.  What the last ``forward`` keeps for ``vjp`` stays."""
+        with self.saved_kept():
+            return self._forward_cached(ids, cache, plan, max_new)
+
+    def _forward_cached(self, ids, cache, plan, max_new):
         if cache.max_len > self.seq:
             raise ValueError(f"forward_cached: a cache of rows of up to {cache.max_len} tokens, the model has {self.seq} positions")
         T = ids.numel()
@@ -125,7 +129,12 @@ class GPT(Module):
     def beam_search(self, prompts, beams: int = 4, max_new: int = 32, eos: int = None, block: int = 16):
         """The ``beams`` likeliest continuations of up to ``max_new`` tokens of each prompt (lists of token ids), best first:
         ``(sequences, scores)`` with ``sequences[r][j]`` a list that ends behind ``eos`` and ``scores [requests, beams]`` the summed
-        log-probabilities.  Keys and values live in a paged 8-bit cache that the beams of a request share."""
+        log-probabilities.  Keys and values live in a paged 8-bit cache that the beams of a request share.  What the last ``forward``
+        keeps for ``vjp`` stays."""
+        with self.saved_kept():
+            return self._beam_search(prompts, beams, max_new, eos, block)
+
+    def _beam_search(self, prompts, beams, max_new, eos, block):
         lens = [len(p) for p in prompts]
         if not lens or min(lens) == 0 or beams < 1 or max_new < 1:
             raise ValueError("beam_search: prompts of at least one token, at least one beam and one new token")
@@ -137,7 +146,7 @@ class GPT(Module):
         new[:, 0] = torch.tensor(lens)
         ids = torch.tensor([t for p in prompts for t in p], dtype=torch.int64).to(dev)
         plan = cache.plan(new.reshape(-1).to(dev), ids.numel())
-        logits = self.forward_cached(ids, cache, plan, max_new=max(lens)).unflatten(0, (R, beams))[:, :1]
+        logits = self._forward_cached(ids, cache, plan, max(lens)).unflatten(0, (R, beams))[:, :1]
         logits = logits.expand(R, beams, -1).contiguous()            # the beams of a request begin as one
         scores = torch.full((R, beams), -math.inf, device=dev)
         scores[:, 0] = 0
@@ -153,7 +162,7 @@ class GPT(Module):
                 if n == 0:
                     cache.refill_spares()                            # a beam's first own block came from its spare
             plan = cache.plan(one, rows)
-            logits = self.forward_cached(tokens.reshape(-1), cache, plan, max_new=1).unflatten(0, (R, beams))
+            logits = self._forward_cached(tokens.reshape(-1), cache, plan, 1).unflatten(0, (R, beams))
         at, back = torch.arange(beams, device=dev).expand(R, beams), []
         for parents, tokens in reversed(steps):
             back.append(torch.gather(tokens, 1, at))

@@ -18,6 +18,7 @@ dotted paths, e.g. ``actor.trunk.0.weight`` (noeira/nn/core/named_params.mojo:76
 from __future__ import annotations
 
 from collections import OrderedDict
+from contextlib import contextmanager
 from typing import Callable, Iterator, Tuple
 
 import torch
@@ -100,6 +101,27 @@ class Module:
         yield self
         for c in self._children.values():
             yield from c.modules()
+
+    @contextmanager
+    def saved_kept(self):
+        """For inference between a forward and its ``vjp``: behind the block, what the forwards of this module and of all below it
+        keep for ``vjp`` is what it was before it."""
+        found, kept, todo = {id(self)}, [], [self]
+        for m in todo:
+            held = m.__dict__
+            kept.append((held, held.copy()))
+            for v in (*m._children.values(), *held.values()):       # children, and parts without a name among the parameters
+                if isinstance(v, Module) and id(v) not in found:
+                    found.add(id(v))
+                    todo.append(v)
+        try:
+            yield
+        finally:
+            for held, before in kept:
+                held.update(before)
+                if len(held) > len(before):
+                    for k in held.keys() - before.keys():
+                        del held[k]
 
     def num_params(self) -> int:
         return sum(p.numel for p in self.params())

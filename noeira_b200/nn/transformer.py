@@ -202,8 +202,9 @@ class SelfAttention(Module):
 
     def forward_cached(self, x, cache, layer, plan, max_new=None, residual=None):
         """New tokens ``x [tokens, dim]`` of the rows of a ``PagedKVCache``: their keys and values go into cache layer ``layer``,
-        and each token attends to its row up to itself.  Inference only (nothing is kept for ``vjp``); causal blocks without
-        rotary embedding, whose positions the cache does not know."""
+        and each token attends to its row up to itself.  Inference only: there is no ``vjp`` for it, and what the projections kept
+        for that of an earlier ``forward`` is lost unless the caller holds it (``Module.saved_kept``).  Causal blocks without rotary
+        embedding, which turns all rows from one position on, not each token by its own."""
         if self.core.mask != "causal" or self.rope_theta:
             raise ValueError("forward_cached: causal attention without rotary embedding")
         T = x.shape[0]
@@ -349,7 +350,7 @@ class TransformerBlock(Module):
         return self.ffn.forward(self.n2.forward(x), residual=x)
 
     def forward_cached(self, x, cache, layer, plan, max_new=None):
-        """``forward`` for new tokens ``[tokens, dim]`` over a ``PagedKVCache`` (see ``SelfAttention.forward_cached``)."""
+        """``forward`` for new tokens ``[tokens, dim]`` over a ``PagedKVCache``, for inference (see ``SelfAttention.forward_cached``)."""
         x = self.attn.forward_cached(self.n1.forward(x), cache, layer, plan, max_new=max_new, residual=x)
         return self.ffn.forward(self.n2.forward(x), residual=x)
 

@@ -33,3 +33,25 @@ def test_rows_beside_a_refused_one_get_their_logits(new, tokens):
     assert cache.lengths.tolist() == [10, 10, 0] and bool(torch.isfinite(got).all())
     # other launches for another number of tokens: both round to bf16 (2^-8) in two layers
     assert float((got[:2].float() - want[:2].float()).norm()) <= 2 * 2 * 3 * 2.0 ** -8 * float(want[:2].float().norm())
+
+
+@pytest.mark.parametrize("tie", [False, True])
+def test_answers_between_forward_and_vjp_change_no_gradient(tie):
+    m = G.model("cuda", tie)
+    ids = torch.randint(0, 64, (2, 64), generator=torch.Generator().manual_seed(1)).cuda()
+    g = (torch.cos(torch.arange(2 * 64 * 64, device="cuda")) / 64).reshape(2, 64, 64).bfloat16()
+    got = []
+    for between in (lambda: None, lambda: None, lambda: m.generate([[1, 2, 3], [4]], max_new=4), lambda: m.beam_search([[5, 6]], beams=3, max_new=4)):
+        m.zero_grad()
+        m.forward(ids)
+        between()
+        m.vjp(g)
+        got.append({k: p.grad.clone() for k, p in m.named_params()})
+    # the embedding's rows are summed by atomics in no fixed order: fp32 sums of up to 128 terms, whose order moves a sum of
+    # magnitude A by 128 * 2^-24 A; all else repeats bit by bit
+    for other in got[1:]:
+        for k, w in got[0].items():
+            if torch.equal(other[k], w):
+                continue
+            assert "wte" in k or "wpe" in k, k
+            assert float((other[k] - w).abs().max()) <= 2 * 128 * 2.0 ** -24 * 128 * float(w.abs().max()), k

@@ -128,3 +128,48 @@ def test_gpt_refuses_prompts_of_other_tokens(bad):
         with pytest.raises(ValueError, match="32 tokens"):
             answer([[1, 2], [3, bad, 4]], max_new=2)
     assert len(m.generate([[0, 31]], max_new=2)[0]) == 2
+
+
+def gradients(m, ids, between):
+    m.zero_grad()
+    logits = m.forward(ids)
+    between()
+    m.vjp(torch.cos(torch.arange(logits.numel(), device=logits.device).reshape(logits.shape)).to(logits.dtype))
+    return {k: p.grad.clone() for k, p in m.named_params()}
+
+
+@pytest.mark.parametrize("tie", [False, True])
+def test_answers_between_forward_and_vjp_change_no_gradient(tie):
+    m = small(tie=tie)
+    ids = torch.randint(0, 32, (2, 20), generator=torch.Generator().manual_seed(1))
+    want = gradients(m, ids, lambda: None)
+    cache = m.new_cache(1, 20)
+
+    def steps():
+        plan = cache.plan(ints([3]), 3)
+        m.forward_cached(torch.tensor([1, 2, 3]), cache, plan)
+
+    for between in (lambda: m.generate([[1, 2, 3], [4]], max_new=4), lambda: m.beam_search([[5, 6]], beams=3, max_new=4), steps):
+        got = gradients(m, ids, between)
+        assert all(torch.equal(got[k], want[k]) for k in want)
+    with pytest.raises(ValueError):                           # a call that fails on its way leaves no trace either
+        m.generate([[1, 2, 3]], max_new=4, eos=32)
+    logits = m.forward(ids)
+    with pytest.raises(ValueError):
+        m.generate([[1, 2, 3]], max_new=4, eos=32)
+    m.zero_grad()
+    m.vjp(torch.cos(torch.arange(logits.numel()).reshape(logits.shape)).to(logits.dtype))
+    assert all(torch.equal(p.grad, want[k]) for k, p in m.named_params())
+
+
+def test_saved_kept_reaches_parts_without_parameters():
+    from noeira_b200 import nn
+    b = nn.TransformerBlock(64, 1, 64, norm="rms", ffn="swiglu", mask="causal")
+    x = torch.randn(1, 5, 64)
+    b.forward(x)
+    before = [dict(vars(m)) for m in (*b.modules(), b.ffn.act)]
+    with b.saved_kept():
+        b.forward(torch.randn(2, 3, 64))
+        b.late = 1
+    for m, held in zip((*b.modules(), b.ffn.act), before):
+        assert vars(m).keys() == held.keys() and all(vars(m)[k] is held[k] for k in held)
