@@ -67,3 +67,33 @@ def quantised_logits(m, ids, block):
         return m.head.forward(h).float().cpu()
     W = m.wte.weight
     return (h.float() @ (W.shadow if h.is_cuda else W.data)[: m.vocab, : m.dim].float().t()).cpu()
+
+
+@torch.no_grad()
+def attention_block(device, heads=4, kv_heads=2, head_dim=128):
+    """Cached attention of a block with grouped heads, prompts and single tokens of two rows, and the definition in 64 bits."""
+    from noeira_b200 import nn
+    from noeira_b200.ops.kvcache import PagedKVCache
+    nn.manual_seed(3)
+    a = nn.SelfAttention(256, heads, kv_heads, head_dim, mask="causal").to(device).eval()
+    cache = PagedKVCache(1, kv_heads, head_dim, 20, 2, 60, 16, device=device)
+    g = torch.Generator().manual_seed(9)
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    x = [torch.randn(n, 256, generator=g).to(device=device, dtype=dtype) for n in (40, 23)]
+    got, at = [[], []], [0, 0]
+    for new in ([30, 0], [1, 17], *[[1, 1]] * 6, [3, 0]):
+        tokens = torch.cat([x[r][at[r]: at[r] + n] for r, n in enumerate(new)])
+        plan = cache.plan(torch.tensor(new, dtype=torch.int32, device=device), len(tokens))
+        o = a.forward_cached(tokens, cache, 0, plan, max_new=max(new))
+        for r, n in enumerate(new):
+            got[r].append(o[sum(new[:r]): sum(new[:r]) + n])
+            at[r] += n
+    want = []
+    for r in range(2):
+        S = at[r]
+        qkv = a.qkv.forward(x[r][:S]).reshape(S, heads + 2 * kv_heads, head_dim)
+        k, v = (torch.from_numpy(rounded(t.float().cpu().numpy(), 16)).repeat_interleave(heads // kv_heads, 1) for t in (qkv[:, heads: heads + kv_heads], qkv[:, heads + kv_heads:]))
+        s = torch.einsum("qhd,khd->hqk", qkv[:, :heads].double().cpu(), k) / head_dim ** 0.5
+        o = torch.einsum("hqk,khd->qhd", torch.softmax(s.masked_fill(torch.ones(S, S).triu(1).bool(), float("-inf")), -1), v).reshape(S, -1)
+        want.append(a.out.forward(o.to(device=device, dtype=dtype)).float().cpu())
+    return [torch.cat(t).float().cpu() for t in got], want

@@ -55,3 +55,9 @@ def test_answers_between_forward_and_vjp_change_no_gradient(tie):
                 continue
             assert "wte" in k or "wpe" in k, k
             assert float((other[k] - w).abs().max()) <= 2 * 128 * 2.0 ** -24 * 128 * float(w.abs().max()), k
+
+
+def test_block_with_grouped_heads():
+    """Attention's output and its weights round by 2^-8 each, the projection's output once more, and a flipped code doubles it."""
+    for got, want in zip(*G.attention_block("cuda")):
+        assert float((got - want).norm()) <= 2 * 3 * 2.0 ** -8 * float(want.norm())

@@ -173,3 +173,11 @@ def test_saved_kept_reaches_parts_without_parameters():
         b.late = 1
     for m, held in zip((*b.modules(), b.ffn.act), before):
         assert vars(m).keys() == held.keys() and all(vars(m)[k] is held[k] for k in held)
+
+
+def test_block_with_grouped_heads():
+    """Prompts in pieces and single tokens.  Sums in fp32, and codes that a growing scale moved below 2^-6 once more: see the
+    logits' test, of which this is one layer."""
+    import gpt_serving as G
+    for got, want in zip(*G.attention_block("cpu")):
+        assert float((got - want).abs().max()) <= 1e-4 * float(want.abs().max())
