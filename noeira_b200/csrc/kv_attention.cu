@@ -5,8 +5,10 @@
 //   * A tile has 8 or 16 query rows: all query heads of one cache head, of as many tokens as fit.  The products are transposed,
 //     S^T = K Q^T and O^T += V^T P^T, as m16n8k16 in f16 with fp32 sums: the 16 rows of an instruction are keys or dimensions,
 //     which there are enough of, and its 8 columns are query rows, which in a decode step there are not.  e4m3 codes are exact
-//     in f16; q (bf16) is exact in f16 down to 2^-38 of the row's largest element after a power-of-two scaling of the row; P
-//     keeps 11 bits.
+//     in f16; q (bf16), after a power-of-two scaling of the row, is exact in f16 down to 2^-31 of the row's largest element, and
+//     below that off by 2^-39 of it at most (f16's subnormals).  P keeps 11 bits (2^-11, an eighth of the bf16 output's own
+//     rounding): more would need a second product for the lower bits.  P times the ratio of the values' scales is f16 as well: exact,
+//     as ratios are powers of two, but below 2^-21 of the row's largest, where it is off by 2^-32 of that at most.
 //   * A warp works by itself: TMA brings the codes into its own ring in shared memory, 4 KB a step (two boxes of 16 keys each for
 //     keys and values at D = 64, one at 128; a block id that is none becomes a box outside the tensor, which arrives as zeros),
 //     and from there they go as they are into the fragments.  The order of the contraction is free as long as q has the same,

@@ -6,10 +6,13 @@
 // A code is exact in f16, and turning one into f16 is one instruction for two, so a key block is turned into f16 once per CTA
 // without its scales:
 //   * keys: the scale of each 16 keys multiplies their scores, which the exponent's multiply-add does at no cost;
-//   * queries: bf16 is exact in f16 down to 2^-38 of a row's largest element after a power-of-two scaling of the row;
+//   * queries: after a power-of-two scaling of the row bf16 is exact in f16 down to 2^-31 of the row's largest element, and below
+//     that off by 2^-39 of it at most;
 //   * values: the weights P carry the scale relative to the largest that the CTA sees, 2^lr, as an addition to the exponent, and
-//     the sum of the weights takes it out again, 16 keys at a time.  f16 weights lose bits below 2^-14; where scales differ by
-//     more than 2^20 the CTA takes values times their scale and P in bf16, which has the exponents.
+//     the sum of the weights takes it out again, 16 keys at a time.  f16 weights have 11 bits,
+//     an eighth of the bf16 output's own rounding, and lose some below 2^-14; where scales differ by more than 2^20 the CTA takes
+//     values times their scale and P in bf16, which has the exponents but 8 bits: a weight's rounding is then as large as the
+//     output's.  What a CTA sees decides, so rows of one call can differ in that.
 //
 //   warp 0       MMA issuer: S_t = Q_t K^T, O_t += P_t V, P from tensor memory (the schedule of attention_fwd2_tcgen05.cu)
 //   warp 1       TMA producer: looks up the blocks of 128 keys a step ahead and brings their codes, 16 rows a copy, into one buffer

@@ -240,7 +240,9 @@ def paged_attention(q, kv, scale, tables, starts, ends, max_new=None, softmax_sc
     ``q`` bf16 ``[tokens, q_heads, head_dim]`` (any token and head strides); ``q_heads`` a multiple of the cache's heads;
     ``starts`` / ``ends`` as in ``TokenPlan``; the token ``t`` of row ``i`` sees the keys at places ``0 .. ends[i] -
     (starts[i + 1] - t)`` of its row.  ``max_new``: an upper bound of the tokens of one row (default: all); 1 in a decode step.
-    Tokens behind ``starts[rows]`` are left as they are in ``out``; a token that sees nothing gets zeros.
+    Tokens behind ``starts[rows]`` are left as they are in ``out``; a token that sees nothing gets zeros.  Scores, maxima and sums
+    are fp32; the softmax's weights are rounded to f16 (2^-11) before they multiply the values, and for rows with more than 64
+    query rows per head whose values' scales differ by more than 2^20 to bf16 (2^-8).
     """
     dev, blocks, hk, block, dim = _check_layer(kv, scale)
     shape = q.shape
