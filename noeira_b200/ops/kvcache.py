@@ -9,7 +9,7 @@ blocks that its line of ``tables`` int32 ``[rows, width]`` names; token number `
 
 None of the calls synchronises.  What only the device can see (no free block, a bad block id) is reported through the status
 word (``ops.check_status``) and never touches memory outside the tensors; on CPU tensors, whose forms compute in fp32, the same
-raises ``RuntimeError`` or ``ValueError``.
+raises ``RuntimeError`` or ``ValueError`` (a plan before it changes anything).
 """
 from __future__ import annotations
 
@@ -110,6 +110,7 @@ def plan_tokens(tables, lengths, new_lens, free, free_count, block, tokens, free
 
 
 def _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_count_out, limit, blocks):
+    given, tables = tables, tables.clone()                   # a call that raises changes nothing
     rows = tables.shape[0]
     count = max(0, min(int(free_count), free.numel()))
     starts, ends = torch.zeros(rows + 1, dtype=torch.int32), lengths.clone()
@@ -147,6 +148,7 @@ def _plan_cpu(tables, lengths, new_lens, free, free_count, block, tokens, free_c
     _need(not bad, f"tables, free: rows {sorted(set(bad))} were given blocks outside the cache")
     out = free_count if free_count_out is None else free_count_out
     out.fill_(count - taken)
+    given.copy_(tables)
     return TokenPlan(starts, ends, row_of, positions, slots, out)
 
 

@@ -51,6 +51,23 @@ def test_plan_names_blocks_that_are_none(bad, place):
             kvcache.plan_tokens(c.tables, c.lengths, ints([1, 1]), c.free, c.free_count, 16, 2, blocks=blocks)
 
 
+def test_a_plan_that_raises_changes_nothing():
+    """Blocks that a refused plan wrote into tables were neither free nor a row's after a reset of other rows."""
+    c = kvcache.PagedKVCache(1, 1, 64, 3, 2, 64, 16, device="cpu")
+    c.plan(ints([16, 0]), 16)
+    before = [t.clone() for t in (c.tables, c.lengths, c.free, c.free_count)]
+    with pytest.raises(RuntimeError, match=r"rows \[1\]"):
+        c.plan(ints([20, 33]), 53)
+    c.free[0] = 3                                             # no block of the cache
+    before[2][0] = 3
+    with pytest.raises(ValueError, match=r"rows \[1\]"):
+        c.plan(ints([1, 1]), 2)
+    assert all(torch.equal(a, b) for a, b in zip(before, (c.tables, c.lengths, c.free, c.free_count)))
+    c.reset([1])
+    assert int(c.free_count) == 2
+    c.plan(ints([0, 32]), 32)
+
+
 def test_reorder_leaves_the_caches_tensors_in_their_place():
     """A captured step holds the addresses of tables, lengths and spare blocks."""
     c = kvcache.PagedKVCache(1, 1, 64, 12, 3, 40, 16, device="cpu", spares=True)
