@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const BeamSel p) {
 template <bool FP32, int EACH, bool WIDE>
 int launch_parts(const BeamSel& p, cudaStream_t s) {
   const int smem = THREADS / 32 * p.beams * EACH * 8;
-  if (smem > 48 * 1024) {
+  if (smem > 47 * 1024) {              // 48 KB hold the kernel's own arrays too
     static bool configured[64] = {};
     int dev = 0;
     NB_CUDA(cudaGetDevice(&dev));

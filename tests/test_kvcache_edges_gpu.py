@@ -219,6 +219,27 @@ def test_select_equal_values_of_different_logits(kind, beams, vocab, fp32):
         assert torch.equal(p.cpu(), c[1]) and torch.equal(t.cpu(), c[2])
 
 
+@pytest.mark.parametrize("fp32", [False, True])
+@pytest.mark.parametrize("pad", [0, 1])
+def test_select_takes_every_number_of_beams(fp32, pad):
+    """In ascending order: none may depend on what a larger one has set up before it.  Rows enough for long parts."""
+    from noeira_b200.ops import beam
+    vocab = 9000
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for beams in range(1, 33):
+        rows = -(-160 // beams)
+        wide = torch.randn(rows, beams, vocab + pad, generator=g, device="cuda")
+        x = (wide if fp32 else wide.bfloat16())[..., :vocab]
+        s, p, t, _ = beam.beam_select(x, torch.zeros(rows, beams, device="cuda"))
+        clean()
+        value = torch.log_softmax(x.double(), -1)
+        assert torch.equal(torch.sort(s, 1, descending=True).values, s) and bool((p < beams).all())
+        # fp32 sums of exponentials of 2^-22 each, their logarithm, and the value's own rounding
+        assert bool(((value.gather(2, t.long().clamp(0, vocab - 1)[:, None].expand(rows, beams, beams)).gather(1, p.long()[:, None])[:, 0] - s).abs() <= 2.0 ** -20 + 2.0 ** -24 * 40).all())
+        top = value.reshape(rows, -1).topk(beams).values
+        assert bool(((top - s).abs() <= 2.0 ** -20 + 2.0 ** -24 * 40).all())
+
+
 # ------------------------------------------------------------------------------------------------ attention
 @pytest.mark.parametrize("tokens", [200, 1])
 def test_attention_over_a_million_keys(tokens):
