@@ -319,7 +319,9 @@ def _attention_cpu(q, kv, scale, tables, starts, ends, softmax_scale, out):
         s = (q[a:b].float().transpose(0, 1) @ k.transpose(1, 2) * softmax_scale).masked_fill(~see, -math.inf)
         m = s.amax(-1, keepdim=True) if end else torch.zeros(hq, b - a, 1)
         p = torch.exp(s - torch.where(m == -math.inf, torch.zeros_like(m), m))
-        o = p @ v / p.sum(-1, keepdim=True).clamp_min(1e-30)
+        nan = torch.isnan(v)                                 # a weight of zero does not hide it
+        o = p @ v.masked_fill(nan, 0.0) / p.sum(-1, keepdim=True).clamp_min(1e-30)
+        o = o.masked_fill(see.float() @ nan.float() > 0, math.nan)
         out[a:b] = o.transpose(0, 1).to(out.dtype)
     return out
 

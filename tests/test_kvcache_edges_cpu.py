@@ -82,6 +82,23 @@ def test_reorder_leaves_the_caches_tensors_in_their_place():
     assert int(held[2].min()) >= 0 and held[2].unique().numel() == 3
 
 
+# ------------------------------------------------------------------------------------------------ attention
+@pytest.mark.parametrize("tokens", [1, 20, 60])
+def test_attention_nan_in_the_cache_reaches_only_who_sees_it(tokens):
+    import kv_cases as C
+    d = C.attention_inputs(([50, 10], [tokens, tokens], 4, 2, 64, 16))
+    q, rest = d["q"][: d["T"], 1:5], (d["scale"], d["tables"], d["starts"], d["ends"])
+    want = kvcache.paged_attention(q, d["codes"], *rest)
+    raw = d["codes"].view(torch.uint8)
+    raw[1, d["tables"][1, 0], 1, 12, 5] = 0x7F                # a value: row 1, place 12, head 1, dimension 5
+    raw[0, d["tables"][0, 3], 0, 4, 9] = 0xFF                 # a key: row 0, place 52, head 0
+    got = kvcache.paged_attention(q, d["codes"], *rest)
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[tokens + 2:, 2:, 5] = True
+    bad[2: tokens, :2] = True
+    assert torch.equal(torch.isnan(got), bad) and torch.equal(got[~bad], want[~bad])
+
+
 # ------------------------------------------------------------------------------------------------ beams
 def test_select_refuses_vocabularies_whose_last_part_passes_32_bits():
     for vocab in (0x7fff0001, 0x7ffffeff):                    # no memory behind it: the sizes alone decide
