@@ -37,6 +37,10 @@ constexpr int LEAST = 2;               // a piece has at least so many steps
 constexpr float RAISE = 8.f;           // the running maximum is raised when it falls behind by more than 2^8 ...
 constexpr float LIFT = 7.f;            // ... and weights are at most 2^(8 + 7), below f16's largest, so that small ones stay normal
 constexpr float NONE = -3e38f;         // the running maximum of a row that has seen nothing
+// Scores whose maximum (log2) lies beyond this are rounded before the maximum is taken off: a multiply-add would leave the product's
+// rounding, up to 2^-24 of the score, in the exponent, and a weight of 2^(8 + 7) and that much more passes f16's largest.  Costs nothing
+// where it is not needed, 110 -> 129 us for the eight tokens above where it is.
+constexpr float FAR = 1048576.f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -117,11 +121,11 @@ __device__ __forceinline__ int job_cost(const KvAttn& p, int end) {
   return p.team ? 1 : LEAD + ceil_div(max(1, min(end, p.width << p.block_log)), KEYS);
 }
 template <int KEYS>
-__device__ __forceinline__ long long row_cost(const KvAttn& p, int i) {
+__device__ __forceinline__ long long row_cost(const KvAttn& p, int few, int i) {
   const int first = __ldg(p.starts + i), next = __ldg(p.starts + i + 1), end = __ldg(p.ends + i);
   const long long n = first < 0 ? 0 : (long long)min(next, p.tokens) - first;
   // rows with more query rows than `few` belong to the kernel of prompts
-  const long long tiles = n <= 0 || n * p.group > p.few ? 0 : (n * p.group + p.tile - 1) >> (p.tile == 8 ? 3 : 4);
+  const long long tiles = n <= 0 || n * p.group > few ? 0 : (n * p.group + p.tile - 1) >> (p.tile == 8 ? 3 : 4);
   return tiles * p.hk * job_cost<KEYS>(p, end);
 }
 // Only first tokens that are none (`starts` not ascending) make more steps than the sizes allow: reported, and nothing is done.
@@ -130,8 +134,15 @@ __device__ __forceinline__ Cut<I> cut_batch(const KvAttn& p, I* upto, I* sh) {
   constexpr long long MOST = most_steps<I>();
   const int tid = threadIdx.x, per = ceil_div(p.rows, THREADS);
   const int lo = min(p.rows, tid * per), hi = min(p.rows, lo + per);
+  int few = p.few;
+  if (p.far_size) {                    // the kernel of prompts was here before: did it meet scores that are this one's?
+    int far = 0;
+#pragma unroll 4
+    for (int i = tid; i < p.far_size; i += THREADS) far |= p.far[i];
+    if (__syncthreads_or(far)) few = 0x7fffffff;
+  }
   long long sum = 0;
-  for (int i = lo; i < hi; ++i) sum += row_cost<KEYS>(p, i);
+  for (int i = lo; i < hi; ++i) sum += row_cost<KEYS>(p, few, i);
   const bool large = sum > MOST;
   const I mine = large ? 0 : (I)sum;
   auto add = [](I a, I b) { return sizeof(I) == 4 ? (I)min((unsigned)a + (unsigned)b, (unsigned)MOST + 1) : a + b; };   // 128 of 2^49 fit in 64 bits
@@ -160,7 +171,7 @@ __device__ __forceinline__ Cut<I> cut_batch(const KvAttn& p, I* upto, I* sh) {
   I begin = at - mine;
   for (int i = lo; i < hi; ++i) {
     upto[i] = begin;
-    if (per > 1) begin += (I)row_cost<KEYS>(p, i);
+    if (per > 1) begin += (I)row_cost<KEYS>(p, few, i);
   }
   if (tid == 0) upto[p.rows] = c.total;
   __syncthreads();
@@ -308,6 +319,7 @@ struct Tile {                          // what a warp keeps of a tile of 8 NB qu
   float m[NB][2], l[NB][2], f[NB][2];  // rows 2c, 2c + 1: maximum (log2), this lane's sum, factor of a raw score
   int lim[NB][2];                      // keys that the row sees
   float vref, vinv;                    // the largest scale of the values so far, and its inverse
+  float kick;                          // +inf where some row's maximum lies beyond FAR, else -inf
 };
 
 // The query rows of a tile as they are in memory: 16 dimensions of each 64, of row g of each 8.
@@ -373,6 +385,7 @@ __device__ __forceinline__ void open_tile(const KvAttn& p, const Part<Shape<D>::
       for (int i = 0; i < 4; ++i) t.o[b][j][i] = 0.f;
   }
   t.vref = t.vinv = 0.f;
+  t.kick = -INFINITY;
 }
 
 // V^T P^T of one sub-tile: acc += V^T (D x 16 keys) P^T (16 keys x 8 rows)
@@ -448,7 +461,12 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
       }
   }
   // exponents; where one is too large for f16 the maxima are raised first.  A NaN lets itself through.
-  float big = -INFINITY;
+  float big = t.kick, base[NB][2];     // base: what is added to a score
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    base[b][0] = LIFT - t.m[b][0];
+    base[b][1] = LIFT - t.m[b][1];
+  }
 #pragma unroll
   for (int u = 0; u < SUB; ++u)
 #pragma unroll
@@ -456,6 +474,8 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
 #pragma unroll
       for (int i = 0; i < 4; ++i) big = fmaxf(big, fmaf(s[u][b][i], f[u][b][i & 1], -t.m[b][i & 1]));
   if (__any_sync(0xffffffffu, big > RAISE) || vtop > t.vref) {
+    bool far = false;
+    const float over = t.kick > 0.f ? 0.f : RAISE;
     const float v = t.vref > 0.f ? t.vref / vtop : 0.f;
     t.vref = vtop;
     t.vinv = vtop > 0.f ? 1.f / vtop : 0.f;
@@ -468,9 +488,11 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
 #pragma unroll
         for (int u = 0; u < SUB; ++u) top = fmaxf(top, fmaxf(s[u][b][i], s[u][b][2 + i]) * f[u][b][i]);
         top = column_max(top);
-        const bool raise = top > t.m[b][i] + RAISE;
+        const bool raise = top > t.m[b][i] + over;
         a[i] = raise ? ex2(t.m[b][i] - top) : 1.f;
         if (raise) t.m[b][i] = top;
+        far |= fabsf(t.m[b][i]) > FAR && t.m[b][i] != NONE;
+        base[b][i] = LIFT - t.m[b][i];
         t.l[b][i] *= a[i];
         a[i] *= v;
       }
@@ -478,6 +500,21 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
       for (int j = 0; j < D / 16; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) t.o[b][j][i] *= a[i & 1];
+    }
+    if (__any_sync(0xffffffffu, far)) {
+      t.kick = INFINITY;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[u][b][i] = __fsub_rn(__fmul_rn(s[u][b][i], f[u][b][i & 1]), t.m[b][i & 1]);
+          f[u][b][0] = f[u][b][1] = 1.f;
+        }
+        base[b][0] = base[b][1] = LIFT;
+      }
+    } else {
+      t.kick = -INFINITY;
     }
   }
 #pragma unroll
@@ -509,7 +546,7 @@ __device__ __forceinline__ void step_tile(const KvAttn& p, Tile<D, NB>& t, const
       float e[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        e[i] = ex2(fmaf(s[u][b][i], f[u][b][i & 1], LIFT - t.m[b][i & 1]));
+        e[i] = ex2(fmaf(s[u][b][i], f[u][b][i & 1], base[b][i & 1]));
         t.l[b][i & 1] += e[i];
       }
       pt[b][0] = times(transposed(f16_pair(e[0], e[1])), w2);
@@ -886,10 +923,14 @@ static Plan plan_for(int dim, int rows, int tokens, int max_new, int hq, int hk,
 
 extern "C" {
 
-// Floats of work space that nb_kv_attention needs for these sizes: partial results, where rows are cut into pieces.
+static long long part_floats(const Plan& plan, int dim) { return plan.team ? 0 : (long long)PIECES * (2 * 16 * (dim + 2) + 4); }
+
+// Floats of work space that nb_kv_attention needs for these sizes: partial results, where rows are cut into pieces, and a byte per
+// block of the kernel of prompts.
 long long nb_kv_attention_work(int dim, int rows, int tokens, int max_new, int hq, int hk, int block, int width) {
   if (hk <= 0 || hq < hk || tokens <= 0) return 0;
-  return plan_for(dim, rows, tokens, max_new, hq, hk, (long long)width * block).team ? 0 : (long long)PIECES * (2 * 16 * (dim + 2) + 4);
+  const Plan plan = plan_for(dim, rows, tokens, max_new, hq, hk, (long long)width * block);
+  return part_floats(plan, dim) + (plan.tiles ? ((long long)plan.units * hk + 3) / 4 : 0);
 }
 
 int nb_kv_attention(const void* q, void* out, const void* codes, const float* scale, const int* tables, const int* starts,
@@ -927,6 +968,8 @@ int nb_kv_attention(const void* q, void* out, const void* codes, const float* sc
   p.tile = plan.one ? 8 : 16;
   p.team = plan.team;
   if (plan.tiles) {
+    p.far = (uint8_t*)(work + part_floats(plan, dim));
+    p.far_size = plan.units * hk;
     const int rc = kv_launch_prompts(p, dim, plan.units, s);
     if (rc) return rc;
   }

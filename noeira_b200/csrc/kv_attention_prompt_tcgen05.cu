@@ -14,6 +14,11 @@
 //     values times their scale and P in bf16, which has the exponents but 8 bits: a weight's rounding is then as large as the
 //     output's.  What a CTA sees decides, so rows of one call can differ in that.
 //
+// The exponent's multiply-add leaves the rounding of the maximum, up to 2^-24 of it, in the weights.  A CTA that may have scores
+// (log2) beyond 2^22, by its largest query element and the largest scale of its keys, says so, and prompts are done over by the other
+// kernel, which rounds such scores before the maximum is taken off (the prompts below: 1756 us instead of 228); in here, in whatever
+// form, it cost all prompts 4 to 7 %.
+//
 //   warp 0       MMA issuer: S_t = Q_t K^T, O_t += P_t V, P from tensor memory (the schedule of attention_fwd2_tcgen05.cu)
 //   warp 1       TMA producer: looks up the blocks of 128 keys a step ahead and brings their codes, 16 rows a copy, into one buffer
 //                for keys and one for values, with the scale of each 16 rows; a block that is none arrives as zeros
@@ -122,6 +127,7 @@ template <int HD>
 __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid_constant__ CUtensorMap map, const KvAttn p) {
   using S = Smem<HD>;
   constexpr float RESCALE_THRESHOLD = 4.f, LIFT = 11.f;   // weights are at most 2^15, below f16's largest
+  constexpr float FAR = 4194304.f;     // up to here roundings add a quarter each: of the maximum, of what is added, of the threshold
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // of the last four key blocks, for each 16 keys: scale of the keys [8], lr [8], 2^-lr [8], scale of the values [8]
@@ -145,6 +151,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
     misc[3] = -1;
     misc[6] = 0;                       // largest scale of the values (its bits), smallest that is not zero
     misc[7] = 0x7f800000;
+    misc[24] = 0;                      // largest scale of the keys (its bits)
+    misc[25] = 0;                      // scores may lie beyond FAR
   }
   if (threadIdx.x < HD) s_nan[threadIdx.x] = 0x7fffffff;
   if (p.rows <= THREADS) {
@@ -192,7 +200,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
     }
   }
   __syncthreads();
-  if (misc[3] < 0) return;             // the grid is an upper bound
+  if (misc[3] < 0) {                   // the grid is an upper bound
+    if (threadIdx.x == 0) p.far[blockIdx.x] = 0;
+    return;
+  }
   const uint32_t aS = smem_u32(smem), aB = smem_u32(bars);
   auto q_full = aB;
   auto raw_full = [&](int w) { return aB + 8u * (1 + w); };
@@ -246,10 +257,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
   const int nmax = max(nkb[0], nkb[1]);
   const int seen = sees(min(tile0 + 2 * BQ, qrows) - 1), sure = sees(tile0);   // the most that a row of this CTA sees, and the fewest
 
-  // scales of the values that this CTA will see
+  // scales of the keys and values that this CTA will see
   for (int pg = threadIdx.x; (long long)pg << p.block_log < seen; pg += THREADS) {
     const int b = p.tables[(long long)row * p.width + pg];
-    const float v = (unsigned)b < (unsigned)p.blocks ? p.scale[p.s_stride + b * p.hk + head] : 0.f;
+    const bool is = (unsigned)b < (unsigned)p.blocks;
+    const float v = is ? p.scale[p.s_stride + b * p.hk + head] : 0.f, k = is ? p.scale[b * p.hk + head] : 0.f;
+    if (k > 0.f) atomicMax(&misc[24], __float_as_int(k));
     if (v > 0.f) {
       atomicMax(&misc[6], __float_as_int(v));
       atomicMin(&misc[7], __float_as_int(v));
@@ -457,6 +470,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
     {
       constexpr int LANES = HD / 8, STEP = 128 / LANES, BATCH = 8;   // lanes of a query row, rows of a turn, turns whose loads go out together
       const int tid = threadIdx.x - 128 - t * 128, ch = tid % LANES;
+      float most = 0.f;                // largest element
 #pragma unroll 1
       for (int r0 = tid / LANES; r0 < BQ; r0 += STEP * BATCH) {
         uint4 w[BATCH];
@@ -481,6 +495,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
           for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(x[e] << 16)), fabsf(__uint_as_float(x[e] & 0xffff0000u))));
 #pragma unroll
           for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          most = fmaxf(most, top);
           int e2 = (int)(__float_as_uint(top) >> 23) - 127;
           e2 = top > 0.f && e2 < 128 ? max(-100, min(112, e2 - 14)) : 0;
           const float by = __uint_as_float((uint32_t)(127 - e2) << 23);
@@ -493,6 +508,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
           *reinterpret_cast<uint4*>(smem + t * S::Q + (ch / 8) * (BQ * 128) + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
         }
       }
+      if (p.scale_log2 * most * (448.f * HD * __int_as_float(misc[24])) > FAR) misc[25] = 1;
     }
     fence_proxy_async();
     __syncwarp();
@@ -621,6 +637,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_prompt_kernel(const __grid
   if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+    if (lane == 0) p.far[blockIdx.x] = (uint8_t)misc[25];
   }
 }
 

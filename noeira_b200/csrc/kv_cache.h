@@ -49,6 +49,8 @@ struct KvAttn {
   int kv_rows;                                  // blocks * hk * block
   int q_vec, o_vec, o_vec16;                    // 16-byte loads of q, 8- and 16-byte stores of out are aligned
   int few;                                      // rows of the batch with at most this many query rows per head are done here
+  uint8_t* far;                                 // all of them, if a CTA of the kernel of prompts said so: a byte each, far_size of them
+  int far_size;
   int tile;                                     // query rows of a tile
   int pieces, team;                             // warps; every tile is one block's
   long long q_token, q_head, o_token, o_head;

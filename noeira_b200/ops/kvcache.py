@@ -29,6 +29,7 @@ LEAST_EXPONENT = -118
 BLOCKS = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
 MAX_ROWS = 8192
+FEW = 64              # query rows of a row and head, up to which the kernel of few query rows does it in any case
 
 
 class TokenPlan(NamedTuple):
@@ -242,7 +243,7 @@ def paged_attention(q, kv, scale, tables, starts, ends, max_new=None, softmax_sc
     ``q`` bf16 ``[tokens, q_heads, head_dim]`` (any token and head strides); ``q_heads`` a multiple of the cache's heads;
     ``starts`` / ``ends`` as in ``TokenPlan``; the token ``t`` of row ``i`` sees the keys at places ``0 .. ends[i] -
     (starts[i + 1] - t)`` of its row.  ``max_new``: an upper bound of the tokens of one row (default: all); 1 in a decode step.
-    Tokens behind ``starts[rows]`` are left as they are in ``out``; a token that sees nothing gets zeros.  Scores, maxima and sums
+    Tokens behind ``starts[rows]`` are left as they are in ``out``, which may be ``q``; a token that sees nothing gets zeros.  Scores, maxima and sums
     are fp32; the softmax's weights are rounded to f16 (2^-11) before they multiply the values, and for rows with more than 64
     query rows per head whose values' scales differ by more than 2^20 to bf16 (2^-8).
     """
@@ -267,6 +268,8 @@ def paged_attention(q, kv, scale, tables, starts, ends, max_new=None, softmax_sc
         return _attention_cpu(q, kv, scale, tables, starts, ends, softmax_scale, out)
     if out is None:
         out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
+    elif out.data_ptr() == q.data_ptr() and max_new * (hq // hk) > FEW:
+        q = q.clone()                                        # rows with many query rows may be done twice
     qs, os_ = q.stride(), out.stride()
     if q.dtype is not torch.bfloat16 or qs[2] != 1:
         raise ValueError("q: bf16 with unit stride over head_dim")

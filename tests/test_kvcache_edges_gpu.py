@@ -322,3 +322,61 @@ def test_attention_reports_starts_that_are_none():
     kvcache.paged_attention(q, kv, scale, torch.zeros(rows, 8192, dtype=I32, device="cuda"), starts, ints([1 << 20] * rows), out=out)
     reported("bounds")
     assert bool((out == 7).all())
+
+
+@pytest.mark.parametrize("mode", [0, 1, 2])
+@pytest.mark.parametrize("held,new,dim,power", [([700, 5], [1, 1], 64, 30), ([90], [1], 128, 24), ([3000, 40], [3, 17], 128, 40), ([60, 2100, 0], [500, 1, 300], 128, 27),
+                                                ([16, 700], [600, 257], 64, 40), ([5000, 31, 2], [1, 1, 1], 64, 21)])
+def test_attention_of_far_scores(mode, held, new, dim, power):
+    """Scores of 2^20 to 2^45: what rounding leaves of a maximum must not become a weight.  Where the largest score leads by more
+    than any rounding of it, the output is that key's value."""
+    import kv_cases as C
+    from noeira_b200.ops import kvcache
+    hq, hk, block = 8, 2, 32
+    d = C.attention_inputs((held, new, hq, hk, dim, block), seed=power)
+    g = torch.Generator().manual_seed(power)
+    scale = torch.exp2(torch.randint(-9, -5, d["scale"].shape, generator=g).float())
+    scale[0] *= torch.exp2(torch.randint(power - 3, power + 1, scale.shape[1:], generator=g).float())
+    q, codes = d["q"][: d["T"], 1: 1 + hq].contiguous().cuda(), d["codes"].cuda()
+    old = kvcache.set_attention_mode(mode)
+    try:
+        out = kvcache.paged_attention(q, codes, scale.cuda(), d["tables"].cuda(), d["starts"].cuda(), d["ends"].cuda(), max_new=d["max_new"])
+        clean()
+    finally:
+        kvcache.set_attention_mode(old)
+    assert bool(torch.isfinite(out).all())
+    scale, st, clear = scale.cuda().double(), d["starts"].tolist(), 0
+    for i, end in enumerate(d["ends"].tolist()):
+        a, b = st[i], st[i + 1]
+        ids = d["tables"][i, : -(-end // block)].long().cuda()
+        k, v = ((codes[w, ids].double() * scale[w, ids][..., None, None]).transpose(0, 1).reshape(hk, -1, dim)[:, :end].repeat_interleave(hq // hk, 0) for w in (0, 1))
+        see = torch.arange(end, device="cuda")[None] <= (end - (b - torch.arange(a, b, device="cuda")))[:, None]
+        s = (q[a:b].double().transpose(0, 1) @ k.transpose(1, 2) * dim ** -0.5).masked_fill(~see, float("-inf"))
+        first, at = s.topk(min(2, end), -1)
+        off = 2.0 ** -24 * (dim + 4) * dim ** -0.5 * q[a:b].double().abs().transpose(0, 1) @ k.abs().amax(1)[..., None]      # of one score
+        lead = (first[..., 0] - first[..., -1] if end > 1 else torch.full_like(first[..., 0], 1e30))
+        lead = torch.where(torch.isnan(lead), torch.full_like(lead, 1e30), lead)                                            # a token that sees one key
+        leads = lead > 2 * off[..., 0] + 40                                                                                 # e^-40 of 2^45 keys is nothing
+        want = v.gather(1, at[..., :1].expand(-1, -1, dim)).transpose(0, 1)
+        got, leads = out[a:b].double(), leads.transpose(0, 1)
+        clear += int(leads.sum())
+        assert bool(((got - want).abs() <= 2.0 ** -8 * want.abs() + 1e-9 * v.abs().max())[leads].all())
+    assert clear > 0.5 * d["T"] * hq
+
+
+@pytest.mark.parametrize("held,new,hq,hk,dim", [([3000, 17], [1, 1], 8, 2, 64), ([300, 0, 40], [20, 1, 33], 32, 8, 128), ([500, 0, 0], [700, 300, 1], 16, 8, 64)])
+@pytest.mark.parametrize("power", [0, 30])
+def test_attention_in_place(held, new, hq, hk, dim, power):
+    """``out`` may be ``q``, also where far scores make the rows of prompts be done over."""
+    import kv_cases as C
+    from noeira_b200.ops import kvcache
+    d = C.attention_inputs((held, new, hq, hk, dim, 32))
+    d["scale"][0] *= 2.0 ** power
+    wide = torch.zeros(d["T"], 3 * hq, dim, dtype=torch.bfloat16, device="cuda")          # a packed projection's queries
+    wide[:, :hq] = d["q"][: d["T"], 1: 1 + hq].cuda()
+    q = wide[:, :hq]
+    rest = (d["codes"].cuda(), d["scale"].cuda(), d["tables"].cuda(), d["starts"].cuda(), d["ends"].cuda(), d["max_new"])
+    want = kvcache.paged_attention(q, *rest)
+    got = kvcache.paged_attention(q, *rest, out=q)
+    clean()
+    assert got.data_ptr() == wide.data_ptr() and torch.equal(got, want) and bool((wide[:, hq:] == 0).all())
