@@ -20,7 +20,7 @@
 // Eight tokens over 275k keys, 32/8 heads of 128 (594 MB): 110 us, 5.4 TB/s; a warp spends about 1000 clocks on a step's 320
 // instructions (a third of them turn codes into f16), twelve warps an SM.  96 tokens over 81k keys, 15/5 heads of 64 (53 MB): 28 us,
 // of which the steps are 12: a warp has seven of them, and starting, the first look into the table and joining take the rest.  One
-// token over 640 keys, 6 heads of 64: 10 us.
+// token over 640 keys, 6 heads of 64: 10.5 us.
 #include <cuda.h>
 
 #include "common.cuh"
